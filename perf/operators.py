@@ -317,10 +317,10 @@ def run(st):
         if case["op"] == "attend":
             return cache.attend(batch, st["q"], scale=st["scale"], window=case["window"])
         if case["op"] == "read":
-            return cache.read(batch, dtype=DTYPES[case["dtype"]])
+            return cache.read(batch, tokens=sum(st["new"]), dtype=DTYPES[case["dtype"]])
         cache.write(batch, st["new_k"], st["new_v"])
         if case["kind"] == "q8_0":
-            return cache.read(batch, dtype=DTYPES[case["dtype"]])
+            return cache.read(batch, tokens=sum(st["new"]), dtype=DTYPES[case["dtype"]])
         return cache.k, cache.v
     return {"store": _plain_store, "read": _plain_read, "attend": _plain_attend}[case["op"]](st, case)
 
