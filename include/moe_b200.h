@@ -2,7 +2,7 @@
  * moe_b200.h -- C ABI of libmoe_b200.so, the B200 (sm_100a) routed-expert
  * MoE library.
  *
- * Two groups of entry points:
+ * Three groups of entry points:
  *
  * 1. Drop-ins for the reference's native exports.  Same names, argument
  *    meaning, return codes and synchronous behaviour as the functions of
@@ -15,6 +15,9 @@
  *    every pointer is a device pointer, every call is asynchronous on the
  *    given cudaStream_t (passed as void*), and argument errors are returned
  *    before anything is enqueued.
+ *
+ * 3. The paged key/value cache and the attention over it, in the manner of
+ *    the second group.
  *
  * Status codes (all functions returning int): 0 success;
  *   -1 bad argument (null pointer, size <= 0 or out of range, bad flag),
@@ -408,6 +411,112 @@ MOE_B200_API int moe_b200_last_cuda_error(void);
 
 /* Library version, major * 10000 + minor * 100 + patch. */
 MOE_B200_API int moe_b200_version(void);
+
+/* ------------------------------------------------------------------------
+ * 3. Paged key/value cache and the attention over it
+ * ---------------------------------------------------------------------- */
+
+/* The full-attention mixer's cache and product, beside the DeltaNet step.  No
+ * counterpart in the reference's native library (its attention keeps a
+ * contiguous fp16 buffer and runs in NumPy/OpenVINO,
+ * src/flash_moe/attention.py:86-591).  Every pointer is device memory, every
+ * call is asynchronous on `stream` and capturable in a CUDA graph, lengths
+ * and page tables are read on the device. */
+
+/* ggml type ids of the plain types (Q8_0 is 8). */
+#define MOE_B200_F32 0
+#define MOE_B200_F16 1
+#define MOE_B200_BF16 30
+
+/* A cache of num_pages pages of page_size rows (a power of two, 16 to 256):
+ * k and v are [num_pages][kv_heads][page_size][head_dim] of `type` (F16,
+ * BF16, or Q8_0: int8 codes), head_dim a multiple of 32, 32 to 256.  A Q8_0
+ * cache has binary16 scales [num_pages][kv_heads][page_size][head_dim / 32]
+ * (a value is scale * code), other caches NULL there.  16-byte aligned;
+ * num_pages * kv_heads below 2^31. */
+typedef struct moe_b200_kv_cache {
+    int32_t type;
+    int32_t num_pages, page_size, kv_heads, head_dim;
+    int32_t reserved;
+    void* k;
+    void* v;
+    void* k_scales;
+    void* v_scales;
+} moe_b200_kv_cache;
+
+/* `tokens` new rows of `sequences` sequences: rows q_start[b] ..
+ * q_start[b + 1] - 1 belong to sequence b (q_start ascending, sequences + 1
+ * entries), kv_lens[b] is its cached length with the new rows, and row i of
+ * them stands at position kv_lens[b] - (q_start[b + 1] - q_start[b]) + i.
+ * Position p lives in row p % page_size of page
+ * page_table[b * table_stride + p / page_size] (max_pages entries a row).
+ * Rows at negative positions and rows behind q_start[sequences] belong to no
+ * cached token. */
+typedef struct moe_b200_kv_batch {
+    int32_t sequences, tokens, max_pages, reserved;
+    int64_t table_stride;
+    const int32_t* q_start;
+    const int32_t* kv_lens;
+    const int32_t* page_table;
+} moe_b200_kv_batch;
+
+/* status (device int32, may be NULL) receives 0 or a sum of these: a page id
+ * outside the cache was met (the rows of that page are skipped), a length
+ * reaches past the page table (the rest is skipped), a bounded device-side
+ * wait gave up (the outputs are not valid). */
+#define MOE_B200_KV_BAD_PAGE 1
+#define MOE_B200_KV_BAD_LENGTH 2
+#define MOE_B200_KV_TIMEOUT 4
+
+/* Store the batch's new keys and values [tokens][kv_heads][head_dim] (type
+ * F32, F16 or BF16; strides in elements, rows of a head contiguous, pointers
+ * and strides multiples of 16 bytes) in their pages.  16-bit caches round to
+ * nearest; Q8_0 takes d = max|x| / 127 rounded up to binary16 (at most
+ * 515.5: larger values saturate) and code = x / d to the nearest integer; a
+ * block that holds a NaN or an infinity reads back as NaN.  Rows that belong
+ * to no cached token are skipped.  Two rows that name the same place leave
+ * one of them, or parts of both, there: pages that receive rows must not be
+ * shared.  Returns 0, -1, -2 (type or head_dim), -6, -7. */
+MOE_B200_API int moe_b200_kv_write(const moe_b200_kv_cache* cache, const moe_b200_kv_batch* batch,
+                                   int32_t type, const void* k, int64_t k_token_stride,
+                                   int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                                   int64_t v_head_stride, int32_t* status, void* stream);
+
+/* The mirror of moe_b200_kv_write: the cached values at the batch's rows,
+ * rounded to `type`, into k and v.  With q_start the running sum of kv_lens
+ * it gathers whole sequences.  Rows at negative positions or in refused
+ * pages read as zeros; rows behind the last sequence are left as they are. */
+MOE_B200_API int moe_b200_kv_read(const moe_b200_kv_cache* cache, const moe_b200_kv_batch* batch,
+                                  int32_t type, void* k, int64_t k_token_stride,
+                                  int64_t k_head_stride, void* v, int64_t v_token_stride,
+                                  int64_t v_head_stride, int32_t* status, void* stream);
+
+/* Bytes of workspace (256-byte aligned device memory, no initial contents
+ * needed, free for other use once the call's work is done) of
+ * moe_b200_attend for this cache, batch shape and number of query heads.
+ * Calls that may run at the same time need workspaces of their own. */
+MOE_B200_API int moe_b200_attend_workspace(const moe_b200_kv_cache* cache,
+                                           const moe_b200_kv_batch* batch, int32_t q_heads,
+                                           size_t* bytes);
+
+/* out[row][h] = sum_j softmax_j(scale * q[row][h] . k_j) v_j over the cached
+ * tokens j of the row's sequence, with key/value head h / (q_heads /
+ * kv_heads): all of them (causal 0), or those up to the row's own position
+ * (causal 1) and, when window > 0, only the last `window` of these.  q and
+ * out [tokens][q_heads][head_dim] of `type` F16 or BF16 (the cache's own type
+ * unless that is Q8_0), strides as for moe_b200_kv_write.  lse ([tokens x
+ * q_heads] fp32, or NULL) receives the logarithm of the softmax sum.  A row
+ * that attends no token gets zeros and -infinity; rows behind the last
+ * sequence are left as they are.  Tokens that a row does not attend never
+ * reach its result, whatever they hold.  Scores, softmax and sums are fp32;
+ * Q8_0 values enter as scale * code rounded to binary16, probabilities as
+ * 16-bit values. */
+MOE_B200_API int moe_b200_attend(const moe_b200_kv_cache* cache, const moe_b200_kv_batch* batch,
+                                 int32_t type, const void* q, int64_t q_token_stride,
+                                 int64_t q_head_stride, int32_t q_heads, void* out,
+                                 int64_t out_token_stride, int64_t out_head_stride, float* lse,
+                                 float scale, int32_t causal, int32_t window, void* workspace,
+                                 size_t workspace_bytes, int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

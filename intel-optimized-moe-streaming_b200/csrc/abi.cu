@@ -22,6 +22,8 @@ static int fail(cudaError_t e, int code) {
     return code;
 }
 
+int cuda_fail(cudaError_t e) { return fail(e, ST_CUDA); }
+
 int sm_count() {
     static int cache[64] = {0};
     int dev = 0;

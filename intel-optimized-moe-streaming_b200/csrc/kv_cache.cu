@@ -1,0 +1,232 @@
+// kv_cache.cu -- writing new keys and values into the pages of a key/value
+// cache (16-bit, or quantised to Q8_0 on the way) and reading rows back.
+//
+// Row i of sequence b stands at position p = kv_len - q_len + i, in row
+// p % page_size of page table[b][p / page_size].  Q8_0, per 32 values:
+//   d = max|x| / 127 rounded up to binary16 (at most 515.5), code = rint(x / d)
+// so |x - d * code| <= d / 2: a scale rounded to nearest could fall below
+// max|x| / 127 and push the largest value past code 127.  A block that holds
+// a NaN or an infinity gets a NaN scale and reads back as NaN.
+//
+// Both kernels move each value once: bound by HBM.  A thread owns 16 values
+// of a head (two 16-byte loads of a 16-bit row, one 16-byte store of codes),
+// two threads own a Q8_0 block.  A CTA first looks up the slots of its
+// tokens, one warp per token, then all its threads walk the units of those
+// tokens, keys and values in the same iteration so that both loads are in
+// flight.
+#include "kv.cuh"
+#include "launch.h"
+
+namespace moeb200 {
+
+namespace {
+
+constexpr int kKvThreads = 256;
+constexpr int kKvMaxTokens = 16;   // tokens per CTA at most
+
+struct KvRows {
+    void* k;
+    void* v;
+    int64_t k_ts, k_hs, v_ts, v_hs;   // strides in elements
+};
+
+template <typename T> struct alignas(16) Vec16 {
+    T v[16];
+};
+
+template <typename T>
+__device__ __forceinline__ void load16(Vec16<T>& d, const T* p) {
+    const uint4* s = reinterpret_cast<const uint4*>(p);
+    uint4* r = reinterpret_cast<uint4*>(d.v);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i) r[i] = __ldcs(s + i);
+}
+
+template <typename T>
+__device__ __forceinline__ void store16(T* p, const Vec16<T>& d) {
+    uint4* s = reinterpret_cast<uint4*>(p);
+    const uint4* r = reinterpret_cast<const uint4*>(d.v);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i) s[i] = r[i];
+}
+
+// One thread's half of a Q8_0 block: codes of x[0..15] and the block's scale
+// (the other half sits in the neighbouring lane; both lanes must call).
+__device__ __forceinline__ __half quantise16(const float (&x)[16], Vec16<int8_t>& q, unsigned mask) {
+    float top = 0.f;
+    bool finite = true;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float a = fabsf(x[i]);
+        finite = finite && a <= 3.402823466e38f;
+        top = fmaxf(top, a);
+    }
+    top = fmaxf(top, __shfl_xor_sync(mask, top, 1));
+    finite = __shfl_xor_sync(mask, (int)finite, 1) && finite;
+    if (!finite) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) q.v[i] = 0;
+        return __ushort_as_half(0x7fff);
+    }
+    const float step = fminf(__half2float(__float2half_ru(__fdiv_rn(top, 127.f))), kKvScaleMax);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float c = step > 0.f ? rintf(__fdiv_rn(x[i], step)) : 0.f;
+        q.v[i] = (int8_t)__float2int_rn(fminf(fmaxf(c, -127.f), 127.f));
+    }
+    return __float2half_rn(step);
+}
+
+// Slot (page * heads * page_size + row, in rows of one head; -1: none) of
+// the CTA's tokens.
+__device__ __forceinline__ void cta_slots(const KvBatch& b, const KvCache& c, int t0, int n,
+                                          int64_t* slots, unsigned* status) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int i = warp; i < n; i += kKvThreads / 32) {
+        const int t = t0 + i;
+        const int s = kv_find_seq(b, t);
+        int64_t slot = -1;
+        if (s >= 0 && lane == 0) {
+            const int pos = __ldg(b.kv_lens + s) - __ldg(b.q_start + s + 1) + t;
+            if (pos >= 0) {
+                const int page = kv_page(b, c, s, pos >> c.page_shift, status);
+                if (page >= 0)
+                    slot = ((int64_t)page * c.heads << c.page_shift) + (pos & (c.page_size - 1));
+            }
+        }
+        if (lane == 0) slots[i] = s < 0 ? -2 : slot;
+    }
+    __syncthreads();
+}
+
+// TI: type of the rows, TC: type of the cache (int8_t: Q8_0).
+template <typename TI, typename TC>
+__global__ void __launch_bounds__(kKvThreads)
+k_kv_write(KvBatch b, KvCache c, KvRows in, int tokens, unsigned* status) {
+    __shared__ int64_t slots[kKvMaxTokens];
+    const int t0 = blockIdx.x * tokens;
+    const int n = b.T - t0 < tokens ? b.T - t0 : tokens;
+    cta_slots(b, c, t0, n, slots, status);
+    const int per_head = c.dim >> 4;
+    const int per_token = per_head * c.heads;
+    for (int u = threadIdx.x; u < n * per_token; u += kKvThreads) {
+        const int i = u / per_token;
+        const int64_t slot = slots[i];
+        if (slot < 0) continue;   // both lanes of a block share the token
+        const int r = u - i * per_token;
+        const int h = r / per_head;
+        const int d = (r - h * per_head) << 4;
+        Vec16<TI> x[2];
+        load16(x[0], static_cast<const TI*>(in.k) + (t0 + i) * in.k_ts + h * in.k_hs + d);
+        load16(x[1], static_cast<const TI*>(in.v) + (t0 + i) * in.v_ts + h * in.v_hs + d);
+        const int64_t row = slot + ((int64_t)h << c.page_shift);
+        const unsigned mask = __activemask();
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            Vec16<TC> y;
+            if constexpr (sizeof(TC) == 1) {
+                float f[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) f[j] = kv_to_f<TI>(x[w].v[j]);
+                const __half s = quantise16(f, y, mask);
+                if (!(d & 16)) (w ? c.vs : c.ks)[row * (c.dim >> 5) + (d >> 5)] = s;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) y.v[j] = kv_from_f<TC>(kv_to_f<TI>(x[w].v[j]));
+            }
+            store16(static_cast<TC*>(w ? c.v : c.k) + row * c.dim + d, y);
+        }
+    }
+}
+
+// Rows whose position is negative, or whose page is refused, read as zeros.
+template <typename TO, typename TC>
+__global__ void __launch_bounds__(kKvThreads)
+k_kv_read(KvBatch b, KvCache c, KvRows out, int tokens, unsigned* status) {
+    __shared__ int64_t slots[kKvMaxTokens];
+    const int t0 = blockIdx.x * tokens;
+    const int n = b.T - t0 < tokens ? b.T - t0 : tokens;
+    cta_slots(b, c, t0, n, slots, status);
+    const int per_head = c.dim >> 4;
+    const int per_token = per_head * c.heads;
+    for (int u = threadIdx.x; u < n * per_token; u += kKvThreads) {
+        const int i = u / per_token;
+        const int64_t slot = slots[i];
+        if (slot == -2) continue;   // behind the last sequence: left as it is
+        const int r = u - i * per_token;
+        const int h = r / per_head;
+        const int d = (r - h * per_head) << 4;
+        const int64_t row = slot + ((int64_t)h << c.page_shift);
+        Vec16<TC> x[2];
+        float s[2] = {0.f, 0.f};
+        if (slot >= 0) {
+            load16(x[0], static_cast<const TC*>(c.k) + row * c.dim + d);
+            load16(x[1], static_cast<const TC*>(c.v) + row * c.dim + d);
+            if constexpr (sizeof(TC) == 1) {
+                s[0] = __half2float(c.ks[row * (c.dim >> 5) + (d >> 5)]);
+                s[1] = __half2float(c.vs[row * (c.dim >> 5) + (d >> 5)]);
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            Vec16<TO> y;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                float f;
+                if constexpr (sizeof(TC) == 1)
+                    f = s[w] * (float)x[w].v[j];
+                else
+                    f = kv_to_f<TC>(x[w].v[j]);
+                y.v[j] = kv_from_f<TO>(slot >= 0 ? f : 0.f);
+            }
+            TO* p = w ? static_cast<TO*>(out.v) + (t0 + i) * out.v_ts + h * out.v_hs + d
+                      : static_cast<TO*>(out.k) + (t0 + i) * out.k_ts + h * out.k_hs + d;
+            store16(p, y);
+        }
+    }
+}
+
+// Tokens per CTA: as many as leave four CTAs per SM, so that small calls
+// spread over the GPU and large ones look several slots up at once.
+int tokens_per_cta(int T) {
+    int n = T / (4 * sm_count());
+    return n < 1 ? 1 : n > kKvMaxTokens ? kKvMaxTokens : n;
+}
+
+template <bool WRITE, typename A, typename B>
+cudaError_t launch_rows(const KvBatch& b, const KvCache& c, const KvRows& r, unsigned* status,
+                        cudaStream_t s) {
+    const int n = tokens_per_cta(b.T);
+    const int grid = (b.T + n - 1) / n;
+    if constexpr (WRITE)
+        k_kv_write<A, B><<<grid, kKvThreads, 0, s>>>(b, c, r, n, status);
+    else
+        k_kv_read<A, B><<<grid, kKvThreads, 0, s>>>(b, c, r, n, status);
+    return cudaGetLastError();
+}
+
+template <bool WRITE, typename A>
+cudaError_t launch_cache(const KvBatch& b, const KvCache& c, const KvRows& r, unsigned* status,
+                         cudaStream_t s) {
+    if (c.type == KV_F16) return launch_rows<WRITE, A, __half>(b, c, r, status, s);
+    if (c.type == KV_BF16) return launch_rows<WRITE, A, __nv_bfloat16>(b, c, r, status, s);
+    return launch_rows<WRITE, A, int8_t>(b, c, r, status, s);
+}
+
+}  // namespace
+
+cudaError_t launch_kv_rows(bool write, const KvBatch& b, const KvCache& c, int type, void* k,
+                           int64_t k_ts, int64_t k_hs, void* v, int64_t v_ts, int64_t v_hs,
+                           unsigned* status, cudaStream_t s) {
+    const KvRows r{k, v, k_ts, k_hs, v_ts, v_hs};
+    if (write) {
+        if (type == KV_F32) return launch_cache<true, float>(b, c, r, status, s);
+        if (type == KV_F16) return launch_cache<true, __half>(b, c, r, status, s);
+        return launch_cache<true, __nv_bfloat16>(b, c, r, status, s);
+    }
+    if (type == KV_F32) return launch_cache<false, float>(b, c, r, status, s);
+    if (type == KV_F16) return launch_cache<false, __half>(b, c, r, status, s);
+    return launch_cache<false, __nv_bfloat16>(b, c, r, status, s);
+}
+
+}  // namespace moeb200

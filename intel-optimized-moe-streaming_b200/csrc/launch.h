@@ -17,6 +17,7 @@ struct moe_b200_ep {
 namespace moeb200 {
 
 int sm_count();  // multiprocessors of the current device (cached per device)
+int cuda_fail(cudaError_t e);  // records e as this thread's last CUDA error; ST_CUDA
 
 // Lays out regions (256-byte aligned) inside one buffer.
 struct Stager {

@@ -29,6 +29,9 @@ EXACT = 4
 SHARED_ONLY = 8
 TCGEN05 = 16
 EP_BLOB_BYTES = 128  # MOE_B200_EP_BLOB_BYTES
+KV_BAD_PAGE = 1     # status bits of the paged cache calls
+KV_BAD_LENGTH = 2
+KV_TIMEOUT = 4
 STEP_CHAIN = 1
 STEP_BLOCK = 2
 
@@ -55,6 +58,26 @@ class Step(C.Structure):
     _fields_ = [
         ("layer", C.c_int32), ("flags", C.c_int32), ("x", C.c_void_p), ("y", C.c_void_p),
         ("topk_ids", C.c_void_p), ("topk_weights", C.c_void_p),
+    ]
+
+
+class KVCacheStruct(C.Structure):
+    """Mirror of ``struct moe_b200_kv_cache``."""
+
+    _fields_ = [
+        ("type", C.c_int32), ("num_pages", C.c_int32), ("page_size", C.c_int32),
+        ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("reserved", C.c_int32),
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+    ]
+
+
+class KVBatchStruct(C.Structure):
+    """Mirror of ``struct moe_b200_kv_batch``."""
+
+    _fields_ = [
+        ("sequences", C.c_int32), ("tokens", C.c_int32), ("max_pages", C.c_int32),
+        ("reserved", C.c_int32), ("table_stride", C.c_int64), ("q_start", C.c_void_p),
+        ("kv_lens", C.c_void_p), ("page_table", C.c_void_p),
     ]
 
 
@@ -101,6 +124,15 @@ def _bind(lib: C.CDLL) -> None:
         "moe_delta_heads": (i, [vp] * 7 + [i] * 3),
         "moe_b200_delta_heads": (i, [vp] * 7 + [i] * 3 + [vp, vp]),
         "moe_b200_expert_noalloc": (i, [i, vp, i64] * 3 + [vp, i, i, vp, i, vp]),
+        "moe_b200_kv_write": (i, [C.POINTER(KVCacheStruct), C.POINTER(KVBatchStruct), C.c_int32]
+                              + [vp, i64, i64] * 2 + [vp, vp]),
+        "moe_b200_kv_read": (i, [C.POINTER(KVCacheStruct), C.POINTER(KVBatchStruct), C.c_int32]
+                             + [vp, i64, i64] * 2 + [vp, vp]),
+        "moe_b200_attend_workspace": (i, [C.POINTER(KVCacheStruct), C.POINTER(KVBatchStruct),
+                                          C.c_int32, C.POINTER(C.c_size_t)]),
+        "moe_b200_attend": (i, [C.POINTER(KVCacheStruct), C.POINTER(KVBatchStruct), C.c_int32,
+                                vp, i64, i64, C.c_int32, vp, i64, i64, vp, f, C.c_int32,
+                                C.c_int32, vp, C.c_size_t, vp, vp]),
         "moe_b200_last_cuda_error": (i, []),
         "moe_b200_workspace_init": (i, [vp, C.c_size_t, vp]),
         "moe_b200_set_trace": (i, [vp, i]),
@@ -113,7 +145,6 @@ def _bind(lib: C.CDLL) -> None:
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args
-    del f
 
 
 def library_path() -> Path:

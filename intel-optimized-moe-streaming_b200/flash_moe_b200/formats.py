@@ -6,6 +6,9 @@ Type ids and block geometry are those of the reference's dispatcher
 """
 from __future__ import annotations
 
+F32 = 0    # plain types: rows and caches of paged_kv, not expert weights
+F16 = 1
+BF16 = 30
 Q8_0 = 8
 Q3_K = 11
 Q4_K = 12
