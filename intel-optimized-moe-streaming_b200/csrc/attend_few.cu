@@ -1,0 +1,746 @@
+// attend_few.cu -- attention over a paged cache for calls of few rows per
+// sequence: single decoded tokens, drafted tokens, short chunks.
+//
+// Such a call reads every key and value once and does little with them, so
+// it is bound by HBM.  Tiles of 16 rows (the query heads of a group, times
+// tokens) are one M = 16 operand of mma.sync: with 8 heads to a group the
+// tensor cores do 16 multiply-adds per value read, far below their rate, while
+// the CUDA cores would need all of theirs.  tcgen05's smallest M is 64 and its
+// operands go through shared and tensor memory, which 16 rows do not repay.
+//
+// A warp walks subtiles of 16 keys on its own: a ring of NS shared-memory
+// entries per warp (a subtile's keys, then its values) filled by tensor copies
+// with a 128-byte swizzle, one lane issuing, no block barrier in the loop.
+// The scores of 16 rows x 16 keys stay in registers as the accumulator, become
+// the A operand of the value product in place, and the running maximum, sum
+// and 16 x DP output are the warp's own until the tile ends; then the four
+// warps' sums are added through shared memory.  Two CTAs per SM, so that one
+// loads while the other starts or ends a tile.
+//
+// Q8_0: codes become binary16 by a byte permute (1024 + 128 + code, exact) and
+// one subtraction, times the block's scale, rounded once: the value of
+// scale * code in binary16.  The order of head dimensions within the key
+// product, and of output columns, is permuted so that a thread takes its codes
+// as 16 consecutive bytes and no transposing load is needed.
+#include <cuda.h>
+
+#include <type_traits>
+
+#include "attend.h"
+#include "launch.h"
+#include "umma.cuh"
+
+namespace moeb200 {
+
+namespace {
+
+constexpr int kFewWarps = 4;
+constexpr int kFewThreads = kFewWarps * 32;
+constexpr int kFewKeys = 16;                     // keys of a subtile
+constexpr int kFewUnit = kFewKeys * kFewWarps;   // keys of a unit
+constexpr uint32_t kFewPolls = 1u << 21;
+constexpr float kLog2e = 1.4426950408889634f;
+
+enum : int { KIND_F16 = 0, KIND_BF16 = 1, KIND_Q8 = 2 };
+
+template <int DP, int KIND>
+struct Few {
+    static constexpr bool Q8 = KIND == KIND_Q8;
+    static constexpr int EB = Q8 ? 1 : 2;
+    static constexpr int ROWB = DP * EB;                       // bytes of a cached row
+    static constexpr int SLABB = ROWB < 128 ? ROWB : 128;      // bytes of a row in one copy
+    static constexpr int SLABS = ROWB / SLABB;
+    static constexpr int TILEB = kFewKeys * ROWB;
+    static constexpr int SCALEB = Q8 ? DP : 0;                 // 16 rows x DP / 32 scales
+    // ring entries: at most 96 KB per CTA, and 8
+    static constexpr int FIT = 96 * 1024 / (kFewWarps * (TILEB + SCALEB));
+    static constexpr int NS = FIT > 8 ? 8 : FIT;
+    static constexpr int VB = Q8 ? (DP >= 128 ? 16 : 8) : 8;   // codes a thread takes of a value row
+    static constexpr int TILES = DP / 8;
+    // binary16 probabilities are taken 2^15 times as large (the largest is
+    // 2^15, below 65504), so that those down to 2^-29 keep all their bits
+    static constexpr float SHIFT = KIND == KIND_BF16 ? 0.f : 15.f;
+    static constexpr int PD = DP < 128 ? DP : 128;             // columns joined per pass
+    static constexpr int o_scale = kFewWarps * NS * TILEB;
+    static constexpr int o_q = o_scale + kFewWarps * NS * SCALEB;
+    static constexpr int o_bar = o_q + DP * 32;
+    static constexpr int o_m = o_bar + kFewWarps * NS * 8;
+    static constexpr int o_l = o_m + kFewWarps * 16 * 4;
+    static constexpr int o_rs = o_l + kFewWarps * 16 * 4;
+    static constexpr int smem = o_rs + 16 * 4 + 1024;          // 1024: base alignment
+    static_assert(NS >= 3, "");
+    static_assert(kFewWarps * 16 * (PD + 4) * 4 <= o_q, "join buffer inside the ring");
+};
+
+template <int KIND>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+    if constexpr (KIND == KIND_BF16)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+            "{%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+            "{%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <bool TRANS>
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    if constexpr (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "r"(addr)
+                     : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "r"(addr)
+                     : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z,
+                                            uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <int KIND>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+    if constexpr (KIND == KIND_BF16) {
+        __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<uint32_t*>(&v);
+    } else {
+        __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<uint32_t*>(&v);
+    }
+}
+
+// Four codes times their block's scale: binary16 pairs (c0, c1), (c2, c3).
+__device__ __forceinline__ void codes4(uint32_t codes, __half2 d, uint32_t& lo, uint32_t& hi) {
+    const uint32_t u = codes ^ 0x80808080u;   // code + 128
+    uint32_t a = __byte_perm(u, 0x64646464u, 0x4140);   // binary16 1024 + 128 + code
+    uint32_t b = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 off = __float2half2_rn(1152.f);
+    __half2 x = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&a), off), d);
+    __half2 y = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&b), off), d);
+    lo = *reinterpret_cast<uint32_t*>(&x);
+    hi = *reinterpret_cast<uint32_t*>(&y);
+}
+
+template <int KIND>
+__device__ __forceinline__ bool odd16(uint32_t pair) {   // a NaN or an infinity in a pair
+    constexpr uint32_t e = KIND == KIND_BF16 ? 0x7f80u : 0x7c00u;
+    return (pair & e) == e || ((pair >> 16) & e) == e;
+}
+
+// Key of column n of an 8-key score tile.  Q8_0 swaps odd keys n and n ^ 4:
+// the 16-byte chunks that a quarter warp reads of the keys (columns 2 q and
+// 2 q + 1) and of the values (rows of the keys of the even, or the odd,
+// columns) then lie in different banks of the swizzled rows.
+template <int KIND>
+__device__ __forceinline__ int column_key(int n) {
+    return KIND == KIND_Q8 ? n ^ ((n & 1) << 2) : n;
+}
+
+// Head dimension of output tile i, column n.
+template <int DP, int KIND>
+__device__ __forceinline__ int out_dim(int i, int n) {
+    using F = Few<DP, KIND>;
+    if constexpr (F::Q8) return (i / F::VB) * (F::VB * 8) + n * F::VB + i % F::VB;
+    return i * 8 + n;
+}
+
+// TQ: type of q and out.
+template <int DP, int KIND, typename TQ>
+__global__ void __launch_bounds__(kFewThreads, 2)
+k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+             const __grid_constant__ AttendArgs a, void* wsp) {
+    using F = Few<DP, KIND>;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* sm = reinterpret_cast<unsigned char*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint4* qf = reinterpret_cast<uint4*>(sm + F::o_q);
+    float* sm_m = reinterpret_cast<float*>(sm + F::o_m);
+    float* sm_l = reinterpret_cast<float*>(sm + F::o_l);
+    float* sm_rs = reinterpret_cast<float*>(sm + F::o_rs);
+    float* joinb = reinterpret_cast<float*>(sm);
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int n8 = lane >> 2, c4 = lane & 3;
+    unsigned char* ring = sm + warp * F::NS * F::TILEB;
+    unsigned char* sring = sm + F::o_scale + warp * F::NS * F::SCALEB;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + F::o_bar) + warp * F::NS;
+    const int nb = a.c.dim >> 5;   // scale blocks of a row
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (lane == 0)
+        for (int i = 0; i < F::NS; ++i) mbar_init(&bars[i], 1);
+    mbar_fence_init();
+
+    const int ctas = gridDim.x;
+    AttendWs ws(wsp, ctas);
+    AttendCursor cur = attend_place<kFewRows, kFewUnit, kFewThreads>(a, blockIdx.x, ctas, 1,
+                                                                      a.status);
+    AttendRecord rec{};
+    int in_slot = 0, out_slot = 0;        // ring positions to fill and to read next
+    uint32_t out_phase = 0;
+    bool lost = false;
+    AttendSeq s{};
+    if (cur.left > 0) s = attend_seq(a, cur.seq, nullptr);
+
+    while (cur.left > 0) {
+        int u_lo, u_hi;
+        attend_units<kFewRows, kFewUnit>(a, s, cur.tile, u_lo, u_hi);
+        const int units = u_hi - u_lo;
+        const int64_t room = units - cur.unit;
+        const int take = (int)(room < cur.left ? room : cur.left);
+        const int u0 = u_lo + cur.unit;
+        const int rows = s.n * a.group - cur.tile * kFewRows;   // valid rows: the first `rows`
+
+        // queries as A fragments; bf16 ones over a Q8_0 cache become binary16
+        // after an exact scaling of the row to a maximum in [1, 2)
+        if constexpr (F::Q8) {
+            for (int r = warp; r < 16; r += kFewWarps) {
+                float f = 1.f;
+                if constexpr (std::is_same<TQ, __nv_bfloat16>::value) {
+                    float top = 0.f;
+                    if (r < rows) {
+                        const int rr = cur.tile * kFewRows + r;
+                        const TQ* q = static_cast<const TQ*>(a.q) +
+                                      (int64_t)(s.q0 + rr / a.group) * a.q_ts +
+                                      (int64_t)(cur.kvh * a.group + rr % a.group) * a.q_hs;
+                        for (int d = lane; d < a.c.dim; d += 32) top = fmaxf(top, fabsf(kv_to_f<TQ>(q[d])));
+                    }
+                    top = warp_max(top);
+                    const uint32_t e = __float_as_uint(top) >> 23;
+                    if (e > 1 && e < 254) f = __uint_as_float((254u - e) << 23);   // 2^(127 - e)
+                }
+                if (lane == 0) sm_rs[r] = f;
+            }
+            __syncthreads();
+        }
+        for (int i = tid; i < DP / 16 * 32; i += kFewThreads) {
+            const int st = i >> 5, l = i & 31, lr = l >> 2, lc = l & 3;
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int r = lr + (j & 1) * 8;
+                const int d = F::Q8 ? (st >> 2) * 64 + lc * 16 + (st & 3) * 4 + (j >> 1) * 2
+                                    : st * 16 + lc * 2 + (j >> 1) * 8;
+                w[j] = 0;
+                if (r < rows && d < a.c.dim) {
+                    const int rr = cur.tile * kFewRows + r;
+                    const TQ* q = static_cast<const TQ*>(a.q) +
+                                  (int64_t)(s.q0 + rr / a.group) * a.q_ts +
+                                  (int64_t)(cur.kvh * a.group + rr % a.group) * a.q_hs + d;
+                    w[j] = *reinterpret_cast<const uint32_t*>(q);
+                    if constexpr (F::Q8 && std::is_same<TQ, __nv_bfloat16>::value)
+                        w[j] = pack16<KIND_F16>(kv_to_f<TQ>(q[0]) * sm_rs[r],
+                                                kv_to_f<TQ>(q[1]) * sm_rs[r]);
+                }
+            }
+            qf[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        // the two rows of this thread: the keys they attend, the factor that
+        // takes a score to units of log 2
+        int lo[2], hi[2];
+        float mul[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = n8 + 8 * i;
+            lo[i] = hi[i] = 0;
+            if (r < rows)
+                attend_range(s.first + (cur.tile * kFewRows + r) / a.group, s.len, a.causal,
+                             a.window, lo[i], hi[i]);
+        }
+        // keys that any row of the tile attends, and those that all attend
+        int t_lo, t_hi, all_lo, all_hi;
+        {
+            const int r0 = cur.tile * kFewRows, r1 = r0 + (rows < 16 ? rows : 16) - 1;
+            attend_range(s.first + r0 / a.group, s.len, a.causal, a.window, t_lo, all_hi);
+            attend_range(s.first + r1 / a.group, s.len, a.causal, a.window, all_lo, t_hi);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            mul[i] = a.scale * kLog2e;
+            if constexpr (F::Q8 && std::is_same<TQ, __nv_bfloat16>::value)
+                mul[i] /= sm_rs[n8 + 8 * i];
+        }
+        uint32_t qreg[DP <= 128 ? DP / 16 : 1][4];
+        if constexpr (DP <= 128) {
+#pragma unroll
+            for (int st = 0; st < DP / 16; ++st) {
+                const uint4 w = qf[st * 32 + lane];
+                qreg[st][0] = w.x;
+                qreg[st][1] = w.y;
+                qreg[st][2] = w.z;
+                qreg[st][3] = w.w;
+            }
+        }
+
+        float o[F::TILES][4];
+#pragma unroll
+        for (int i = 0; i < F::TILES; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+        // Page ids of 32 subtiles at a time, one per lane (-1: nothing there).
+        int page_of = -1, win = 0;
+        uint32_t there = 0;   // bit j % 32: subtile j was fetched
+        auto look_up = [&](int j0) {
+            win = j0;
+            page_of = -1;
+            const int key = ((u0 + j0 + lane) * kFewWarps + warp) * kFewKeys;
+            if (j0 + lane < take && key < t_hi && key + kFewKeys > t_lo)
+                page_of = kv_page(a.b, a.c, cur.seq, key >> a.c.page_shift, a.status);
+        };
+        // entry e: the keys (even) or values (odd) of subtile e / 2
+        auto fetch = [&](int e) {
+            const int j = e >> 1, w = e & 1;
+            if (j >= take) return;
+            if (j - win >= 32) look_up(j);
+            const int page = __shfl_sync(0xffffffffu, page_of, j - win);
+            if (!w) there = (there & ~(1u << (j & 31))) | ((page >= 0 ? 1u : 0u) << (j & 31));
+            if (page < 0) return;
+            const int key = ((u0 + j) * kFewWarps + warp) * kFewKeys;
+            const int row = key & (a.c.page_size - 1);
+            const int z = page * a.c.heads + cur.kvh;
+            if (lane == 0) {
+                uint64_t* bar = &bars[in_slot];
+                unsigned char* dst = ring + in_slot * F::TILEB;
+                mbar_arrive_expect_tx(bar, F::TILEB + (F::Q8 ? a.c.dim : 0));
+#pragma unroll
+                for (int sl = 0; sl < F::SLABS; ++sl)
+                    tma_load_3d(dst + sl * kFewKeys * F::SLABB, w ? &vmap : &kmap,
+                                sl * (F::SLABB / F::EB), row, z, bar);
+                if constexpr (F::Q8)
+                    bulk_g2s(sring + in_slot * F::SCALEB,
+                             (w ? a.c.vs : a.c.ks) + (((int64_t)z << a.c.page_shift) + row) * nb,
+                             a.c.dim, bar);
+            }
+            in_slot = in_slot + 1 == F::NS ? 0 : in_slot + 1;
+        };
+        auto await = [&]() {
+            if (!mbar_wait(&bars[out_slot], out_phase, lost ? 64u : kFewPolls)) lost = true;
+        };
+        auto release = [&]() {
+            out_slot = out_slot + 1 == F::NS ? 0 : out_slot + 1;
+            out_phase ^= out_slot == 0;
+        };
+        look_up(0);
+#pragma unroll 1
+        for (int e = 0; e < F::NS; ++e) fetch(e);
+
+#pragma unroll 1
+        for (int j = 0; j < take; ++j) {
+            if (!((there >> (j & 31)) & 1)) {
+                fetch(2 * j + F::NS);
+                fetch(2 * j + 1 + F::NS);
+                continue;
+            }
+            const int key0 = ((u0 + j) * kFewWarps + warp) * kFewKeys;
+            // ---- scores
+            float sc[2][4] = {}, sx[2][4] = {};
+            await();
+            {
+                const unsigned char* kt = ring + out_slot * F::TILEB;
+                const uint32_t kaddr = smem_u32(kt);
+                if constexpr (!F::Q8) {
+                    const int key = (lane >> 4) * 8 + (lane & 7), half = (lane >> 3) & 1;
+#pragma unroll
+                    for (int st = 0; st < DP / 16; ++st) {
+                        uint32_t b[4], qa[4];
+                        const int slab = st >> 2, ch = (st & 3) * 2 + half;
+                        ldsm4<false>(b, kaddr + slab * 2048 + key * 128 + ((ch ^ (key & 7)) << 4));
+                        if constexpr (DP <= 128) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) qa[i] = qreg[st][i];
+                        } else {
+                            const uint4 w = qf[st * 32 + lane];
+                            qa[0] = w.x; qa[1] = w.y; qa[2] = w.z; qa[3] = w.w;
+                        }
+                        if (st & 1) {
+                            mma16816<KIND>(sx[0], qa, b[0], b[1]);
+                            mma16816<KIND>(sx[1], qa, b[2], b[3]);
+                        } else {
+                            mma16816<KIND>(sc[0], qa, b[0], b[1]);
+                            mma16816<KIND>(sc[1], qa, b[2], b[3]);
+                        }
+                    }
+                } else {
+                    const __half* ks = reinterpret_cast<const __half*>(sring + out_slot * F::SCALEB);
+#pragma unroll
+                    for (int sp = 0; sp < DP / 64; ++sp) {
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            const int key = t * 8 + column_key<KIND>(n8);
+                            uint32_t addr;
+                            if constexpr (F::SLABB == 128)
+                                addr = kaddr + (sp >> 1) * 2048 + key * 128 +
+                                       ((((sp & 1) * 4 + c4) ^ (key & 7)) << 4);
+                            else
+                                addr = kaddr + key * 64 + c4 * 16;
+                            uint32_t w[4];
+                            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                                         : "r"(addr)
+                                         : "memory");
+                            const int blk = sp * 2 + (c4 >> 1);
+                            const __half2 d = __half2half2(blk < nb ? ks[key * nb + blk]
+                                                                    : __ushort_as_half(0));
+#pragma unroll
+                            for (int st = 0; st < 4; ++st) {
+                                uint32_t b0, b1, qa[4];
+                                codes4(w[st], d, b0, b1);
+                                if constexpr (DP <= 128) {
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) qa[i] = qreg[sp * 4 + st][i];
+                                } else {
+                                    const uint4 x = qf[(sp * 4 + st) * 32 + lane];
+                                    qa[0] = x.x; qa[1] = x.y; qa[2] = x.z; qa[3] = x.w;
+                                }
+                                mma16816<KIND>(st & 1 ? sx[t] : sc[t], qa, b0, b1);
+                            }
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            release();
+            fetch(2 * j + F::NS);
+            // ---- softmax of this subtile
+            const bool whole = key0 >= all_lo && key0 + kFewKeys <= all_hi;
+            float p[2][4];
+            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float v = (sc[t][e] + sx[t][e]) * mul[e >> 1];
+                    const int key = key0 + t * 8 + column_key<KIND>(c4 * 2 + (e & 1));
+                    if (!whole && (key < lo[e >> 1] || key >= hi[e >> 1])) v = -INFINITY;
+                    p[t][e] = v;
+                    top[e >> 1] = fmaxf(top[e >> 1], v);
+                }
+            bool grew = false;
+            float keep[2], base[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+                const float mn = fmaxf(m[i], top[i]);
+                base[i] = mn == -INFINITY ? 0.f : mn - F::SHIFT;
+                keep[i] = ex2(m[i] - (mn == -INFINITY ? 0.f : mn));
+                grew = grew || mn > m[i];
+                m[i] = mn;
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[t][e] = ex2(p[t][e] - base[e >> 1]);
+            if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) l[i] *= keep[i];
+#pragma unroll
+                for (int i = 0; i < F::TILES; ++i) {
+                    o[i][0] *= keep[0];
+                    o[i][1] *= keep[0];
+                    o[i][2] *= keep[1];
+                    o[i][3] *= keep[1];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                l[i] += p[0][2 * i] + p[0][2 * i + 1] + p[1][2 * i] + p[1][2 * i + 1];
+            uint32_t pa[4];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                pa[2 * t] = pack16<KIND>(p[t][0], p[t][1]);
+                pa[2 * t + 1] = pack16<KIND>(p[t][2], p[t][3]);
+            }
+            // ---- values
+            await();
+            unsigned char* vt = ring + out_slot * F::TILEB;
+            __half* vs = reinterpret_cast<__half*>(sring + out_slot * F::SCALEB);
+            if (!whole) {
+                // A key that only some rows attend, or none: 0 * NaN would
+                // reach the others.  Values that are not finite are added to
+                // the rows that attend them one by one and leave the tile.
+                bool odd = false;
+                if constexpr (F::Q8) {
+                    for (int i = lane; i < kFewKeys * nb; i += 32)
+                        odd = odd || odd16<KIND_F16>(__half_as_ushort(vs[i]));
+                } else {
+                    const uint4* v4 = reinterpret_cast<const uint4*>(vt);
+                    for (int i = lane; i < F::TILEB / 16; i += 32) {
+                        const uint4 w = v4[i];
+                        odd = odd || odd16<KIND>(w.x) || odd16<KIND>(w.y) || odd16<KIND>(w.z) ||
+                              odd16<KIND>(w.w);
+                    }
+                }
+                if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll 1
+                    for (int k = 0; k < kFewKeys; ++k) {
+                        const int col = column_key<KIND>(k & 7);   // its own inverse
+                        const int from = (lane & ~3) | (col >> 1);
+                        const bool t1 = k >= 8, e1 = col & 1;
+                        float pk[2];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float a0 = __shfl_sync(0xffffffffu, p[0][2 * i], from);
+                            const float a1 = __shfl_sync(0xffffffffu, p[0][2 * i + 1], from);
+                            const float b0 = __shfl_sync(0xffffffffu, p[1][2 * i], from);
+                            const float b1 = __shfl_sync(0xffffffffu, p[1][2 * i + 1], from);
+                            pk[i] = t1 ? (e1 ? b1 : b0) : (e1 ? a1 : a0);
+                        }
+                        const bool at0 = key0 + k >= lo[0] && key0 + k < hi[0];
+                        const bool at1 = key0 + k >= lo[1] && key0 + k < hi[1];
+#pragma unroll
+                        for (int i = 0; i < F::TILES; ++i)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int d = out_dim<DP, KIND>(i, c4 * 2 + e);
+                                float v = 0.f;
+                                if constexpr (F::Q8) {
+                                    if (d < a.c.dim && odd16<KIND_F16>(__half_as_ushort(vs[k * nb + (d >> 5)]))) {
+                                        const int byte = F::SLABB == 128
+                                            ? (d >> 7) * 2048 + k * 128 + ((((d >> 4) & 7) ^ (k & 7)) << 4) + (d & 15)
+                                            : k * 64 + d;
+                                        v = __half2float(vs[k * nb + (d >> 5)]) *
+                                            (float)reinterpret_cast<const int8_t*>(vt)[byte];
+                                    }
+                                } else {
+                                    const int byte = (d >> 6) * 2048 + k * 128 +
+                                                     ((((d >> 3) & 7) ^ (k & 7)) << 4) + (d & 7) * 2;
+                                    const uint16_t w = *reinterpret_cast<const uint16_t*>(vt + byte);
+                                    if (odd16<KIND>(w))
+                                        v = KIND == KIND_BF16
+                                                ? __bfloat162float(__ushort_as_bfloat16(w))
+                                                : __half2float(__ushort_as_half(w));
+                                }
+                                if (v != 0.f) {   // NaN or infinite
+                                    if (at0) o[i][e] += pk[0] * v;
+                                    if (at1) o[i][2 + e] += pk[1] * v;
+                                }
+                            }
+                    }
+                    __syncwarp();
+                    if constexpr (F::Q8) {
+                        for (int i = lane; i < kFewKeys * nb; i += 32)
+                            if (odd16<KIND_F16>(__half_as_ushort(vs[i]))) vs[i] = __ushort_as_half(0);
+                    } else {
+                        uint16_t* v2 = reinterpret_cast<uint16_t*>(vt);
+                        for (int i = lane; i < F::TILEB / 2; i += 32)
+                            if (odd16<KIND>(v2[i])) v2[i] = 0;
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                }
+            }
+            const uint32_t vaddr = smem_u32(vt);
+            if constexpr (!F::Q8) {
+                const int key = ((lane >> 3) & 1) * 8 + (lane & 7), half = lane >> 4;
+#pragma unroll
+                for (int d = 0; d < DP / 16; ++d) {
+                    uint32_t b[4];
+                    const int ch = (d & 3) * 2 + half;
+                    ldsm4<true>(b, vaddr + (d >> 2) * 2048 + key * 128 + ((ch ^ (key & 7)) << 4));
+                    mma16816<KIND>(o[2 * d], pa, b[0], b[1]);
+                    mma16816<KIND>(o[2 * d + 1], pa, b[2], b[3]);
+                }
+            } else {
+                constexpr int W = F::VB / 4;   // 32-bit words of codes per key
+#pragma unroll
+                for (int sl = 0; sl < DP / (F::VB * 8); ++sl) {
+                    uint32_t w[4][W];
+                    __half2 d[4];
+                    const int blk = (sl * F::VB * 8 + n8 * F::VB) >> 5;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = column_key<KIND>(c4 * 2 + (i & 1)) + (i >> 1) * 8;
+                        d[i] = __half2half2(blk < nb ? vs[key * nb + blk] : __ushort_as_half(0));
+                        if constexpr (F::VB == 16)
+                            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                                         : "=r"(w[i][0]), "=r"(w[i][1]), "=r"(w[i][2]), "=r"(w[i][3])
+                                         : "r"(vaddr + sl * 2048 + key * 128 + ((n8 ^ (key & 7)) << 4))
+                                         : "memory");
+                        else
+                            asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];"
+                                         : "=r"(w[i][0]), "=r"(w[i][1])
+                                         : "r"(vaddr + key * 64 + n8 * 8)
+                                         : "memory");
+                    }
+#pragma unroll
+                    for (int g = 0; g < W; ++g) {
+                        uint32_t x[4][2];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) codes4(w[i][g], d[i], x[i][0], x[i][1]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const unsigned sel = e & 1 ? 0x7632u : 0x5410u;
+                            mma16816<KIND>(o[sl * F::VB + g * 4 + e], pa,
+                                           __byte_perm(x[0][e >> 1], x[1][e >> 1], sel),
+                                           __byte_perm(x[2][e >> 1], x[3][e >> 1], sel));
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            release();
+            fetch(2 * j + 1 + F::NS);
+        }
+
+        // ---- the warps' sums of the tile, or of this piece of it
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+            m[i] -= F::SHIFT;   // l and o belong to this exponent
+            if (c4 == 0) {
+                sm_m[warp * 16 + n8 + 8 * i] = m[i];
+                sm_l[warp * 16 + n8 + 8 * i] = l[i];
+            }
+        }
+        __syncthreads();
+        float keep[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float mm = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kFewWarps; ++w) mm = fmaxf(mm, sm_m[w * 16 + n8 + 8 * i]);
+            keep[i] = m[i] == -INFINITY ? 0.f : ex2(m[i] - mm);
+            if (lost) keep[i] = 0.f;
+        }
+        const bool full = cur.unit == 0 && take == units;
+        const int which = cur.unit == 0;   // 1: tail slot, 0: head slot
+        float* slot = ws.slot(blockIdx.x, which, kFewRows, DP);
+        if (!full) {
+            if (which) {
+                rec.tail = 1;
+                rec.seq = cur.seq;
+                rec.tile = cur.tile;
+                rec.kvh = cur.kvh;
+            } else {
+                rec.head = cur.unit + take == units ? 2 : 1;
+            }
+        }
+#pragma unroll
+        for (int pass = 0; pass < DP / F::PD; ++pass) {
+#pragma unroll
+            for (int i = 0; i < F::TILES; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int d = out_dim<DP, KIND>(i, c4 * 2 + e);
+                    if (d / F::PD == pass) {
+                        float* p = joinb + (warp * 16 + n8) * (F::PD + 4) + d % F::PD;
+                        p[0] = o[i][e] * keep[0];
+                        p[8 * (F::PD + 4)] = o[i][2 + e] * keep[1];
+                    }
+                }
+            __syncthreads();
+            for (int i = tid; i < 16 * F::PD / 4; i += kFewThreads) {
+                const int r = i / (F::PD / 4), x = i % (F::PD / 4) * 4;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+                for (int w = 0; w < kFewWarps; ++w) {
+                    const float4 t = *reinterpret_cast<const float4*>(
+                        joinb + (w * 16 + r) * (F::PD + 4) + x);
+                    v.x += t.x;
+                    v.y += t.y;
+                    v.z += t.z;
+                    v.w += t.w;
+                    mm = fmaxf(mm, sm_m[w * 16 + r]);
+                }
+                const int d = pass * F::PD + x;
+#pragma unroll
+                for (int w = 0; w < kFewWarps; ++w)
+                    ll += sm_l[w * 16 + r] *
+                          (sm_m[w * 16 + r] == -INFINITY ? 0.f : ex2(sm_m[w * 16 + r] - mm));
+                if (!full) {
+                    *reinterpret_cast<float4*>(slot + r * DP + d) = v;
+                    if (d == 0) {
+                        slot[kFewRows * DP + 2 * r] = mm;
+                        slot[kFewRows * DP + 2 * r + 1] = ll;
+                    }
+                } else if (r < rows) {
+                    const int rr = cur.tile * kFewRows + r;
+                    const int tok = rr / a.group, h = cur.kvh * a.group + rr % a.group;
+                    int l0, h0;
+                    attend_range(s.first + tok, s.len, a.causal, a.window, l0, h0);
+                    const bool none = l0 >= h0;
+                    const float inv = none ? 0.f : 1.f / ll;
+                    if (d < a.c.dim) {
+                        TQ y[4] = {kv_from_f<TQ>(v.x * inv), kv_from_f<TQ>(v.y * inv),
+                                   kv_from_f<TQ>(v.z * inv), kv_from_f<TQ>(v.w * inv)};
+                        TQ* out = static_cast<TQ*>(a.out) + (int64_t)(s.q0 + tok) * a.o_ts +
+                                  (int64_t)h * a.o_hs + d;
+                        *reinterpret_cast<uint2*>(out) = *reinterpret_cast<uint2*>(y);
+                    }
+                    if (a.lse && d == 0)
+                        a.lse[(int64_t)(s.q0 + tok) * a.q_heads + h] =
+                            none ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
+                }
+            }
+            fence_async_smem();   // the ring's next copies come after these writes
+            __syncthreads();
+        }
+        cur.left -= take;
+        if (cur.left > 0) attend_next<kFewRows>(a, cur, s);
+    }
+    if (lost) kv_flag(a.status, KV_TIMEOUT);
+    if (tid == 0) ws.rec[blockIdx.x] = rec;
+}
+
+template <int DP, int KIND, typename TQ>
+cudaError_t launch_few(const AttendArgs& a, void* ws, cudaStream_t s) {
+    using F = Few<DP, KIND>;
+    CUtensorMap kmap, vmap;
+    if (!attend_map(&kmap, a.c, a.c.k, F::SLABB / F::EB, kFewKeys) ||
+        !attend_map(&vmap, a.c, a.c.v, F::SLABB / F::EB, kFewKeys))
+        return cudaErrorInvalidValue;
+    cudaError_t e = cudaFuncSetAttribute(k_attend_few<DP, KIND, TQ>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, F::smem);
+    if (e != cudaSuccess) return e;
+    k_attend_few<DP, KIND, TQ><<<attend_few_ctas(), kFewThreads, F::smem, s>>>(kmap, vmap, a, ws);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    return launch_attend_join(a, ws, attend_few_ctas(), kFewRows, DP, s);
+}
+
+template <int DP>
+cudaError_t launch_dim(const AttendArgs& a, void* ws, cudaStream_t s) {
+    if (a.c.type == KV_F16) return launch_few<DP, KIND_F16, __half>(a, ws, s);
+    if (a.c.type == KV_BF16) return launch_few<DP, KIND_BF16, __nv_bfloat16>(a, ws, s);
+    if (a.type == KV_F16) return launch_few<DP, KIND_Q8, __half>(a, ws, s);
+    return launch_few<DP, KIND_Q8, __nv_bfloat16>(a, ws, s);
+}
+
+}  // namespace
+
+int attend_few_ctas() { return 2 * sm_count(); }
+
+cudaError_t launch_attend_few(const AttendArgs& a, void* ws, cudaStream_t s) {
+    const int dp = attend_dim(a.c.dim);
+    if (dp == 64) return launch_dim<64>(a, ws, s);
+    if (dp == 128) return launch_dim<128>(a, ws, s);
+    return launch_dim<256>(a, ws, s);
+}
+
+}  // namespace moeb200

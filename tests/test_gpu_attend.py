@@ -8,7 +8,11 @@ The allowed error of an output, per element (mass = sum_j p_j |v_j|):
   D 2^-23 sum|q k| (the tensor cores may cut instead of round), plus 2^-21 for
   the exponential and the running rescales; numerator and denominator both
   move by that, so 2 delta mass;
-* the fp32 sums over n keys, n 2^-23 mass.
+* the fp32 sums over n keys, n 2^-23 mass;
+* probabilities below binary16's normal range: the row's largest one is held
+  as at least 2^7 (2^15, or up to 2^8 less while a larger maximum has not been
+  taken over yet), so a smallest binary16 step, 2^-24, is 2^-31 of it, half of
+  that 2^-32 per key: 2^-32 sum_j |v_j|.
 """
 from __future__ import annotations
 
@@ -61,6 +65,9 @@ def check(cache, batch, q, out, lse, new, kv, scale, causal=True, window=0, skip
                 qk = torch.zeros(q[lo:lo + n].shape[:2], device=DEV, dtype=torch.float64)
             delta = (q.shape[2] * 2.0 ** -23 * qk + 2.0 ** -21)[..., None]
             tol = eps_o * want.abs() + (eps_p + 2 * delta + length * 2.0 ** -23) * mass * 1.01
+            if kind == torch.float16:
+                total = v.abs().sum(0).repeat_interleave(group, 0) if length else 0.0
+                tol = tol + 2.0 ** -32 * total
             # a 16-bit output below its smallest normal rounds to half of its smallest step
             tol = tol + (2.0 ** -25 if q.dtype == torch.float16 else 1e-40)
             err = (out[lo:lo + n].double() - want).abs()
