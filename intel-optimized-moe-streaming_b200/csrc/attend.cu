@@ -152,12 +152,21 @@ bool attend_map(void* map, const KvCache& c, const void* base, int cols, int row
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-size_t attend_workspace_bytes(const KvBatch&, const KvCache& c, int) {
-    return AttendWs::bytes(attend_few_ctas(), kFewRows, attend_dim(c.dim));
+namespace {
+
+// Tiles of many rows from 33 rows per sequence on average.
+bool use_many(const KvBatch& b, int group) { return (int64_t)b.T * group > 32 * (int64_t)b.B; }
+
+}  // namespace
+
+size_t attend_workspace_bytes(const KvBatch& b, const KvCache& c, int q_heads) {
+    const int dp = attend_dim(c.dim);
+    return use_many(b, q_heads / c.heads) ? AttendWs::bytes(sm_count(), many_rows(dp), dp)
+                                          : AttendWs::bytes(attend_few_ctas(), kFewRows, dp);
 }
 
 cudaError_t launch_attend(const AttendArgs& a, void* ws, cudaStream_t s) {
-    return launch_attend_few(a, ws, s);
+    return use_many(a.b, a.group) ? launch_attend_many(a, ws, s) : launch_attend_few(a, ws, s);
 }
 
 }  // namespace moeb200

@@ -73,6 +73,11 @@ constexpr int kFewRows = 16;
 int attend_few_ctas();
 cudaError_t launch_attend_few(const AttendArgs& a, void* ws, cudaStream_t s);
 
+// Tiles of 256 rows (128 for a head dimension above 128) on tcgen05
+// (attend_many.cu): chunks of prompts.
+inline int many_rows(int dp) { return dp > 128 ? 128 : 256; }
+cudaError_t launch_attend_many(const AttendArgs& a, void* ws, cudaStream_t s);
+
 // Tensor map over a cache plane [pages * heads][page_size][dim]: boxes of
 // `cols` values x `rows` rows, 128-byte swizzle when a box row has 128 bytes.
 bool attend_map(void* map, const KvCache& c, const void* base, int cols, int rows);
@@ -150,12 +155,18 @@ struct AttendCursor {
 // Finds the stretch of CTA `cta` of `ctas`: every thread sums the units of its
 // share of the sequences, a block scan places the shares, and the thread whose
 // share holds the stretch's first unit walks to it.  At least `least` units go
-// to a CTA.  Returns in every thread; left = 0: nothing to do.
+// to a CTA.  Returns in every thread; left = 0: nothing to do.  The scratch is
+// shared memory that the caller may use for something else afterwards.
+struct AttendScratch {
+    int64_t warp_total[16];
+    AttendCursor found;
+};
+
 template <int M, int KT, int THREADS>
-__device__ AttendCursor attend_place(const AttendArgs& a, int cta, int ctas, int least,
-                                     unsigned* status) {
-    __shared__ int64_t warp_total[THREADS / 32];
-    __shared__ AttendCursor found;
+__device__ AttendCursor attend_place(const AttendArgs& a, AttendScratch& scratch, int cta,
+                                     int ctas, int least, unsigned* status) {
+    int64_t* warp_total = scratch.warp_total;
+    AttendCursor& found = scratch.found;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int share = (a.b.B + THREADS - 1) / THREADS;
     const int b0 = tid * share;
@@ -217,7 +228,9 @@ __device__ AttendCursor attend_place(const AttendArgs& a, int cta, int ctas, int
         }
     }
     __syncthreads();
-    return found;
+    const AttendCursor c = found;
+    __syncthreads();   // the scratch may be overwritten
+    return c;
 }
 
 // Moves to the next tile that has rows (head, then tile, then sequence); `s`

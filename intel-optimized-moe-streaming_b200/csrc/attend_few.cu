@@ -22,13 +22,8 @@
 // scale * code in binary16.  The order of head dimensions within the key
 // product, and of output columns, is permuted so that a thread takes its codes
 // as 16 consecutive bytes and no transposing load is needed.
-#include <cuda.h>
-
-#include <type_traits>
-
-#include "attend.h"
+#include "attend_mma.cuh"
 #include "launch.h"
-#include "umma.cuh"
 
 namespace moeb200 {
 
@@ -39,9 +34,6 @@ constexpr int kFewThreads = kFewWarps * 32;
 constexpr int kFewKeys = 16;                     // keys of a subtile
 constexpr int kFewUnit = kFewKeys * kFewWarps;   // keys of a unit
 constexpr uint32_t kFewPolls = 1u << 21;
-constexpr float kLog2e = 1.4426950408889634f;
-
-enum : int { KIND_F16 = 0, KIND_BF16 = 1, KIND_Q8 = 2 };
 
 template <int DP, int KIND>
 struct Few {
@@ -103,50 +95,6 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
                      : "memory");
 }
 
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z,
-                                            uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-        : "memory");
-}
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-template <int KIND>
-__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
-    if constexpr (KIND == KIND_BF16) {
-        __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-        return *reinterpret_cast<uint32_t*>(&v);
-    } else {
-        __half2 v = __floats2half2_rn(lo, hi);
-        return *reinterpret_cast<uint32_t*>(&v);
-    }
-}
-
-// Four codes times their block's scale: binary16 pairs (c0, c1), (c2, c3).
-__device__ __forceinline__ void codes4(uint32_t codes, __half2 d, uint32_t& lo, uint32_t& hi) {
-    const uint32_t u = codes ^ 0x80808080u;   // code + 128
-    uint32_t a = __byte_perm(u, 0x64646464u, 0x4140);   // binary16 1024 + 128 + code
-    uint32_t b = __byte_perm(u, 0x64646464u, 0x4342);
-    const __half2 off = __float2half2_rn(1152.f);
-    __half2 x = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&a), off), d);
-    __half2 y = __hmul2(__hsub2(*reinterpret_cast<__half2*>(&b), off), d);
-    lo = *reinterpret_cast<uint32_t*>(&x);
-    hi = *reinterpret_cast<uint32_t*>(&y);
-}
-
-template <int KIND>
-__device__ __forceinline__ bool odd16(uint32_t pair) {   // a NaN or an infinity in a pair
-    constexpr uint32_t e = KIND == KIND_BF16 ? 0x7f80u : 0x7c00u;
-    return (pair & e) == e || ((pair >> 16) & e) == e;
-}
-
 // Key of column n of an 8-key score tile.  Q8_0 swaps odd keys n and n ^ 4:
 // the 16-byte chunks that a quarter warp reads of the keys (columns 2 q and
 // 2 q + 1) and of the values (rows of the keys of the even, or the odd,
@@ -193,8 +141,9 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
 
     const int ctas = gridDim.x;
     AttendWs ws(wsp, ctas);
-    AttendCursor cur = attend_place<kFewRows, kFewUnit, kFewThreads>(a, blockIdx.x, ctas, 1,
-                                                                      a.status);
+    AttendCursor cur = attend_place<kFewRows, kFewUnit, kFewThreads>(
+        a, *reinterpret_cast<AttendScratch*>(sm), blockIdx.x, ctas, 1, a.status);
+    fence_async_smem();   // the scratch lies in the ring
     AttendRecord rec{};
     int in_slot = 0, out_slot = 0;        // ring positions to fill and to read next
     uint32_t out_phase = 0;
@@ -226,8 +175,7 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
                         for (int d = lane; d < a.c.dim; d += 32) top = fmaxf(top, fabsf(kv_to_f<TQ>(q[d])));
                     }
                     top = warp_max(top);
-                    const uint32_t e = __float_as_uint(top) >> 23;
-                    if (e > 1 && e < 254) f = __uint_as_float((254u - e) << 23);   // 2^(127 - e)
+                    f = row_factor(top);
                 }
                 if (lane == 0) sm_rs[r] = f;
             }

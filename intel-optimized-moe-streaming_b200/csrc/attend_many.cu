@@ -1,0 +1,862 @@
+// attend_many.cu -- attention of chunks of new rows over a paged cache on
+// tcgen05.
+//
+// 4 D operations per (row, key, head) against 2 D values read per key of a
+// whole tile: bound by the tensor cores, and next to them by the exponentials
+// (128 x 128 scores take 1024 cycles of an SM's special function units, the
+// two products of a 128-value head 1024 cycles of its tensor core).
+//
+// A CTA (one per SM) holds the query tile of a group's rows -- two of 128 rows
+// for head dimensions up to 128, one above -- and walks units of 128 keys.
+// Tensor memory has the two score tiles S (128 columns each) and the output
+// sums O (2 x DP columns, or 256); the probabilities overwrite their scores as
+// 16-bit values and are the value product's A operand from there.
+//   warps 0-7   softmax: a thread owns a row (one of two tiles; or, with one
+//               tile, half the columns of a row, the two halves agreeing on
+//               the maximum through shared memory).  The maximum in use is
+//               only replaced when it grows by more than 2^8, so O is rarely
+//               rescaled; the same threads do that, load the queries, and
+//               divide and store the rows at a tile's end.
+//   warp 8      copies: a ring of NST stages of up to 32 KB (keys x 64-value
+//               slabs, 128-byte swizzle) filled by tensor copies, one lane per
+//               page piece and slab
+//   warp 9      one lane issues all products: with two tiles S_t(j + 1) follows
+//               the value product of tile t, so that a tile's softmax runs
+//               under the other tile's products; with one tile S(j + 1) comes
+//               before the value product of j
+//   warps 12-15 (Q8_0) instead of the copies: codes are loaded a stage ahead
+//               into registers, become binary16 and go to the ring
+#include "attend_mma.cuh"
+#include "launch.h"
+
+namespace moeb200 {
+
+namespace {
+
+constexpr int kManyKeys = 128;               // keys of a unit
+constexpr uint32_t kManyPolls = 1u << 21;
+constexpr float kManyGrow = 8.f;             // log 2 of the growth that replaces the maximum
+
+template <int DP, int KIND>
+struct Many {
+    static constexpr bool Q8 = KIND == KIND_Q8;
+    static constexpr int NQ = DP > 128 ? 1 : 2;          // query tiles of 128 rows
+    static constexpr int M = 128 * NQ;
+    static constexpr int SLABS = DP / 64;
+    static constexpr int KPARTS = DP > 128 ? 2 : 1;      // stages of a unit's keys, and values
+    static constexpr int KSLABS = SLABS / KPARTS;        // slabs of a stage of keys (by dimension)
+    static constexpr int VKEYS = kManyKeys / KPARTS;     // keys of a stage of values
+    static constexpr int STAGEB = KSLABS * kManyKeys * 128;
+    static constexpr int QB = NQ * SLABS * 128 * 128;
+    static constexpr int NST = DP == 64 ? 8 : 5;
+    static constexpr int NC = NQ == 2 ? 128 : 64;        // score columns of a thread
+    static constexpr int OC = NQ == 2 ? DP : DP / 2;     // output columns of a thread
+    static constexpr int THREADS = Q8 ? 512 : 384;
+    // binary16 probabilities: 2^7 of the maximum in use, at most 2^15
+    static constexpr float SHIFT = KIND == KIND_BF16 ? 0.f : 7.f;
+    static constexpr int o_stage = QB;
+    static constexpr int o_bar = QB + NST * STAGEB;
+    static constexpr int o_fac = o_bar + 256;            // row factors
+    static constexpr int o_max = o_fac + M * 4;          // maxima and sums of half rows
+    static constexpr int smem = o_max + (NQ == 1 ? 2048 : 0);
+    static_assert(smem <= 232448, "shared memory of a CTA");
+    static constexpr uint32_t IDESC_S = umma_idesc_f16(128, kManyKeys) |
+                                        (KIND == KIND_BF16 ? (1u << 7) | (1u << 10) : 0u);
+    static constexpr uint32_t IDESC_O = umma_idesc_f16(128, DP) | (1u << 16) |   // B: N-major
+                                        (KIND == KIND_BF16 ? (1u << 7) | (1u << 10) : 0u);
+};
+
+struct ManyBars {
+    uint64_t full[8], empty[8], s_full[2], p_full[2], pv_done[2], q_full[2];
+    uint32_t tmem, lost;
+    uint32_t odd[4];   // keys of the unit whose values are not all finite
+};
+static_assert(sizeof(ManyBars) <= 256, "");
+
+// D (+)= A . B with A in tensor memory.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                            uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, 1, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc)
+        : "memory");
+}
+
+// Descriptor of an N-major SWIZZLE_128B operand (values: 64 dimensions of a
+// key are 128 contiguous bytes): 8-key atoms 1024 bytes apart along K, slabs
+// of 64 dimensions `slab` bytes apart along N.
+__device__ __forceinline__ uint64_t umma_desc_nmajor(uint32_t saddr, uint32_t slab) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(slab >> 4) << 16) |
+           ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)),
+          "l"(reinterpret_cast<uint64_t&>(c)));
+    return d;
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(d))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return d;
+}
+
+template <int ID, int N>
+__device__ __forceinline__ void bar_sync() {
+    asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory");
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+                 "r"(valid ? 16 : 0)
+                 : "memory");
+}
+
+// One role's walk over the segments (stretch of one tile) of its CTA.
+template <int DP, int KIND>
+struct Walk {
+    AttendCursor cur;
+    AttendSeq s;
+    int u0, take, units;
+    __device__ bool open(const AttendArgs& a) {   // the current segment's units
+        if (cur.left <= 0) return false;
+        int lo, hi;
+        attend_units<Many<DP, KIND>::M, kManyKeys>(a, s, cur.tile, lo, hi);
+        units = hi - lo;
+        u0 = lo + cur.unit;
+        const int room = units - cur.unit;
+        take = room < cur.left ? room : (int)cur.left;
+        return true;
+    }
+    __device__ void next(const AttendArgs& a) {
+        cur.left -= take;
+        if (cur.left > 0) attend_next<Many<DP, KIND>::M>(a, cur, s);
+    }
+};
+
+// Stage of the ring, counted over the segment: two tiles take keys and values
+// in turn; one tile takes the keys of j + 1 before the values of j.
+template <int NQ>
+__device__ __forceinline__ int stage_k(int j) {
+    return NQ == 2 ? 2 * j : j == 0 ? 0 : 4 * j - 2;
+}
+template <int NQ>
+__device__ __forceinline__ int stage_v(int j, int take) {
+    return NQ == 2 ? 2 * j + 1 : j + 1 < take ? 4 * j + 4 : 4 * j + 2;
+}
+
+// Queries of this warp's rows of a tile into the swizzled operand layout.
+// TQ values are copied as they are (cp.async); or, for bfloat16 over Q8_0 and
+// for negative scales, through registers: scaled to binary16, sign flipped.
+template <int DP, int KIND, typename TQ>
+struct QueryRows {
+    using F = Many<DP, KIND>;
+    static constexpr bool CONVERT = F::Q8 && std::is_same<TQ, __nv_bfloat16>::value;
+    static constexpr int LPR = DP / 8;        // lanes of a row, 16 bytes each
+    static constexpr int RPI = 32 / LPR;      // rows of an iteration
+    static constexpr int BATCH = 4;
+
+    // rows [0, n) relative to row0 of the tile; the warp takes 32 / split rows
+    __device__ static void load(const AttendArgs& a, const Walk<DP, KIND>& w, int row0, int n_rows,
+                                unsigned char* tile, float* fac, int valid) {
+        const int lane = threadIdx.x & 31;
+        const int ch = lane % LPR, sub = lane / LPR;
+        const bool in_dim = ch * 8 < a.c.dim;
+        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+        const bool copy = !CONVERT && flip == 0;
+        for (int i0 = 0; i0 < n_rows; i0 += RPI * BATCH) {
+            uint4 x[BATCH];
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+                const int r = row0 + i0 + b * RPI + sub;
+                const bool ok = in_dim && r < valid;
+                const int rr = w.cur.tile * F::M + (ok ? r : 0);
+                const TQ* q = static_cast<const TQ*>(a.q) +
+                              (int64_t)(w.s.q0 + rr / a.group) * a.q_ts +
+                              (int64_t)(w.cur.kvh * a.group + rr % a.group) * a.q_hs +
+                              (ok ? ch * 8 : 0);
+                if (copy) {
+                    const int t = r & 127;
+                    cp_async16(smem_u32(tile + (r >> 7) * (F::SLABS * 16384) + (ch >> 3) * 16384) +
+                                   sw128_offset(t, ch & 7), q, ok);
+                } else {
+                    x[b] = make_uint4(0, 0, 0, 0);
+                    if (ok) x[b] = __ldg(reinterpret_cast<const uint4*>(q));
+                }
+            }
+            if (copy) continue;
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+                const int r = row0 + i0 + b * RPI + sub, t = r & 127;
+                uint32_t* w32 = reinterpret_cast<uint32_t*>(&x[b]);
+                if constexpr (CONVERT) {
+                    float v[8], top = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        v[2 * i] = __uint_as_float(w32[i] << 16);
+                        v[2 * i + 1] = __uint_as_float(w32[i] & 0xffff0000u);
+                        top = fmaxf(top, fmaxf(fabsf(v[2 * i]), fabsf(v[2 * i + 1])));
+                    }
+#pragma unroll
+                    for (int o = LPR / 2; o > 0; o >>= 1)
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    const float f = row_factor(top);
+                    if (ch == 0) fac[r] = f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w32[i] = pack16<KIND_F16>(v[2 * i] * f, v[2 * i + 1] * f);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w32[i] ^= flip;
+                *reinterpret_cast<uint4*>(tile + (r >> 7) * (F::SLABS * 16384) + (ch >> 3) * 16384 +
+                                          sw128_offset(t, ch & 7)) = x[b];
+            }
+        }
+    }
+};
+
+template <int DP, int KIND, typename TQ>
+__global__ void __launch_bounds__(Many<DP, KIND>::THREADS, 1)
+k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+              const __grid_constant__ AttendArgs a, void* wsp) {
+    using F = Many<DP, KIND>;
+    extern __shared__ __align__(1024) unsigned char smem_many[];
+    unsigned char* sm = smem_many;
+    ManyBars* bars = reinterpret_cast<ManyBars*>(sm + F::o_bar);
+    float* fac = reinterpret_cast<float*>(sm + F::o_fac);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (tid == 0) {
+        for (int i = 0; i < F::NST; ++i) {
+            mbar_init(&bars->full[i], F::Q8 ? 4 : 1);
+            mbar_init(&bars->empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars->s_full[i], 1);
+            mbar_init(&bars->p_full[i], F::NQ == 2 ? 4 : 8);
+            mbar_init(&bars->pv_done[i], 1);
+            mbar_init(&bars->q_full[i], F::NQ == 2 ? 4 : 8);
+        }
+        bars->lost = 0;
+        for (int i = 0; i < 4; ++i) bars->odd[i] = 0;
+        mbar_fence_init();
+    }
+    if (warp == 9) tmem_alloc(&bars->tmem, 512);
+    const int ctas = gridDim.x;
+    AttendWs ws(wsp, ctas);
+    Walk<DP, KIND> w;
+    w.cur = attend_place<F::M, kManyKeys, F::THREADS>(
+        a, *reinterpret_cast<AttendScratch*>(sm), blockIdx.x, ctas, 1, a.status);
+    fence_async_smem();   // the scratch lies where the queries go
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars->tmem);
+    if (w.cur.left > 0) w.s = attend_seq(a, w.cur.seq, nullptr);
+
+    bool lost = false;
+    auto await = [&](uint64_t* bar, uint32_t parity) {
+        if (!mbar_wait(bar, parity & 1u, lost ? 64u : kManyPolls)) {
+            lost = true;
+            *reinterpret_cast<volatile uint32_t*>(&bars->lost) = 1;
+        }
+    };
+
+    if (warp < 8) {
+        // ------------------------------------------------------------ softmax
+        if constexpr (F::Q8)
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+        else
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int wg = warp >> 2, quarter = warp & 3;
+        const int row = quarter * 32 + lane;                       // of the 128-row tile
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;     // TMEM lane offset
+        const int trow = F::NQ == 2 ? wg * 128 + row : row;        // of the CTA's rows
+        const int col0 = F::NQ == 2 ? 0 : wg * 64;                 // first score column
+        const uint32_t t_o = tmem + lanes + 256 + (F::NQ == 2 ? wg * DP : wg * 128);
+        const int q0 = F::NQ == 2 ? wg * 128 + quarter * 32 : quarter * 32 + wg * 16;
+        constexpr int QN = F::NQ == 2 ? 32 : 16;                   // query rows the warp loads
+        float* xmax = reinterpret_cast<float*>(sm + F::o_max);     // [2][2][128]
+        AttendRecord rec{};
+        uint32_t it = 0;       // units done by the CTA
+        int stage0 = 0;        // ring stages before this segment
+
+        auto load_queries = [&](int n_valid) {
+            QueryRows<DP, KIND, TQ>::load(a, w, q0, QN, sm, fac, n_valid);
+        };
+        auto hand_queries = [&]() {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->q_full[F::NQ == 2 ? wg : 0]);
+        };
+        bool more = w.open(a);
+        if (more) {
+            load_queries(w.s.n * a.group - w.cur.tile * F::M);
+            hand_queries();
+        }
+        while (more) {
+            const AttendSeq s = w.s;
+            const AttendCursor cur = w.cur;
+            const int u0 = w.u0, take = w.take, units = w.units;
+            const int rows = s.n * a.group - cur.tile * F::M;   // valid rows: the first `rows`
+            // keys that every row attends, and those of this thread's row
+            int all_lo, all_hi, lo = 0, hi = 0, x;
+            {
+                const int r0 = cur.tile * F::M, r1 = r0 + (rows < F::M ? rows : F::M) - 1;
+                attend_range(s.first + r0 / a.group, s.len, a.causal, a.window, x, all_hi);
+                attend_range(s.first + r1 / a.group, s.len, a.causal, a.window, all_lo, x);
+                if (trow < rows)
+                    attend_range(s.first + (r0 + trow) / a.group, s.len, a.causal, a.window, lo, hi);
+            }
+            float m = -INFINITY, l = 0.f;
+            float mul = 0.f;
+            {   // O starts from zeros
+                uint32_t z[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) z[i] = 0;
+#pragma unroll
+                for (int c = 0; c < F::OC / 32; ++c) tmem_st32(t_o + c * 32, z);
+                tmem_wait_st();
+            }
+#pragma unroll 1
+            for (int j = 0; j < take; ++j, ++it) {
+                const int buf = F::NQ == 2 ? wg : (int)(it & 1);
+                const uint32_t ph = F::NQ == 2 ? it : it >> 1;
+                const uint32_t t_s = tmem + lanes + buf * 128;
+                await(&bars->s_full[buf], ph);
+                tc_fence_after();
+                if (j == 0) {
+                    mul = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);   // 0: equal weights
+                    if constexpr (QueryRows<DP, KIND, TQ>::CONVERT) mul /= fac[trow];
+                }
+                uint32_t sv[F::NC];
+#pragma unroll
+                for (int c = 0; c < F::NC / 32; ++c) tmem_ld32(t_s + col0 + c * 32, sv + c * 32);
+                tmem_wait_ld();
+                const int key0 = (u0 + j) * kManyKeys;
+                const bool whole = key0 >= all_lo && key0 + kManyKeys <= all_hi;
+                if (!whole) {
+                    const int from = lo - key0 - col0, to = hi - key0 - col0;
+#pragma unroll
+                    for (int i = 0; i < F::NC; ++i)
+                        if (i < from || i >= to) sv[i] = 0xff800000u;   // -infinity
+                }
+                float t0 = __uint_as_float(sv[0]), t1 = __uint_as_float(sv[1]);
+                float t2 = __uint_as_float(sv[2]), t3 = __uint_as_float(sv[3]);
+#pragma unroll
+                for (int i = 4; i < F::NC; i += 8) {
+                    t0 = fmaxf(fmaxf(t0, __uint_as_float(sv[i])), __uint_as_float(sv[i + 1]));
+                    t1 = fmaxf(fmaxf(t1, __uint_as_float(sv[i + 2])), __uint_as_float(sv[i + 3]));
+                    if (i + 4 < F::NC) {
+                        t2 = fmaxf(fmaxf(t2, __uint_as_float(sv[i + 4])), __uint_as_float(sv[i + 5]));
+                        t3 = fmaxf(fmaxf(t3, __uint_as_float(sv[i + 6])), __uint_as_float(sv[i + 7]));
+                    }
+                }
+                float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * mul;
+                if constexpr (F::NQ == 1) {
+                    float* xm = xmax + (it & 1) * 256;
+                    xm[wg * 128 + row] = top;
+                    bar_sync<1, 256>();
+                    top = fmaxf(top, xm[(wg ^ 1) * 128 + row]);
+                }
+                const bool grow = top > m + kManyGrow || (m == -INFINITY && top > m);
+                if (__any_sync(0xffffffffu, grow && j > 0)) {
+                    const float f = grow ? ex2(m - top) : 1.f;
+                    l *= f;
+                    await(&bars->pv_done[F::NQ == 2 ? wg : 0], it - 1);
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < F::OC / 32; ++c) {
+                        uint32_t o[32];
+                        tmem_ld32(t_o + c * 32, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tmem_st32(t_o + c * 32, o);
+                    }
+                    tmem_wait_st();
+                }
+                if (grow) m = top;
+                const float base = m == -INFINITY ? 0.f : m - F::SHIFT;
+                const float2 mul2 = make_float2(mul, mul), base2 = make_float2(-base, -base);
+                float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+#pragma unroll
+                for (int c = 0; c < F::NC / 32; ++c) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        float2 v = make_float2(__uint_as_float(sv[c * 32 + 2 * i]),
+                                               __uint_as_float(sv[c * 32 + 2 * i + 1]));
+                        v = fma2(v, mul2, base2);
+                        v.x = ex2(v.x);
+                        v.y = ex2(v.y);
+                        if (i & 1) sum1 = add2(sum1, v); else sum0 = add2(sum0, v);
+                        pk[i] = pack16<KIND>(v.x, v.y);
+                    }
+                    tmem_st16(t_s + col0 / 2 + c * 16, pk);
+                }
+                sum0 = add2(sum0, sum1);
+                l += sum0.x + sum0.y;
+                tmem_wait_st();
+                if (!whole) {
+                    // A key that only some rows attend, or none: 0 * NaN would
+                    // reach the others.  Values that are not finite are added to
+                    // the rows that attend them one by one and leave the stage.
+                    unsigned char* st[F::KPARTS];
+                    bool odd = false;
+#pragma unroll
+                    for (int h = 0; h < F::KPARTS; ++h) {
+                        const int n = stage0 + stage_v<F::NQ>(j, take) + h;
+                        st[h] = sm + F::o_stage + (n % F::NST) * F::STAGEB;
+                        await(&bars->full[n % F::NST], (uint32_t)(n / F::NST));
+                        for (int i = tid; i < F::STAGEB / 16; i += 256) {
+                            const uint4 v = reinterpret_cast<const uint4*>(st[h])[i];
+                            if (odd16<KIND>(v.x) || odd16<KIND>(v.y) || odd16<KIND>(v.z) ||
+                                odd16<KIND>(v.w)) {
+                                odd = true;
+                                const int k = h * F::VKEYS + (i >> 3) % F::VKEYS;
+                                atomicOr(&bars->odd[k >> 5], 1u << (k & 31));
+                            }
+                        }
+                    }
+                    tc_fence_before();
+                    int any;
+                    asm volatile(
+                        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+                        "bar.red.or.pred q, 2, 256, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+                        : "=r"(any)
+                        : "r"((int)odd)
+                        : "memory");
+                    if (any) {
+                        tc_fence_after();
+                        if (j > 0) {
+                            await(&bars->pv_done[F::NQ == 2 ? wg : 0], it - 1);
+                            tc_fence_after();
+                        }
+#pragma unroll 1
+                        for (int k = 0; k < kManyKeys; ++k) {
+                            if (!((bars->odd[k >> 5] >> (k & 31)) & 1)) continue;
+                            const uint32_t pw = tmem_ld1(t_s + k / 2);
+                            tmem_wait_ld();
+                            const uint16_t ph16 = (uint16_t)(k & 1 ? pw >> 16 : pw);
+                            const float p = KIND == KIND_BF16
+                                                ? __bfloat162float(__ushort_as_bfloat16(ph16))
+                                                : __half2float(__ushort_as_half(ph16));
+                            const bool at = key0 + k >= lo && key0 + k < hi;
+                            const unsigned char* vt = st[k / F::VKEYS];
+                            const int kr = k % F::VKEYS;
+#pragma unroll 1
+                            for (int c = 0; c < F::OC / 16; ++c) {
+                                uint32_t o[16];
+                                tmem_ld16(t_o + c * 16, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) {
+                                    const int d = (F::NQ == 1 ? wg * 128 : 0) + c * 16 + i;
+                                    const uint16_t v16 = *reinterpret_cast<const uint16_t*>(
+                                        vt + (d >> 6) * (F::VKEYS * 128) +
+                                        sw128_offset(kr, (d >> 3) & 7) + (d & 7) * 2);
+                                    if (at && odd16<KIND>(v16))
+                                        o[i] = __float_as_uint(
+                                            __uint_as_float(o[i]) +
+                                            p * (KIND == KIND_BF16
+                                                     ? __bfloat162float(__ushort_as_bfloat16(v16))
+                                                     : __half2float(__ushort_as_half(v16))));
+                                }
+                                __syncwarp();
+                                tmem_st16(t_o + c * 16, o);
+                            }
+                            tmem_wait_st();
+                        }
+                        bar_sync<2, 256>();
+#pragma unroll
+                        for (int h = 0; h < F::KPARTS; ++h)
+                            for (int i = tid; i < F::STAGEB / 2; i += 256) {
+                                uint16_t* v = reinterpret_cast<uint16_t*>(st[h]) + i;
+                                if (odd16<KIND>(*v)) *v = 0;
+                            }
+                        if (tid < 4) bars->odd[tid] = 0;
+                        fence_async_smem();
+                        bar_sync<2, 256>();
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars->p_full[buf]);
+            }
+            // the next segment's queries are on their way while this one ends
+            w.next(a);
+            more = w.open(a);
+            if (more) load_queries(w.s.n * a.group - w.cur.tile * F::M);
+            await(&bars->pv_done[F::NQ == 2 ? wg : 0], it - 1);
+            tc_fence_after();
+            if constexpr (F::NQ == 1) {   // both halves' sums
+                float* xl = xmax + (it & 1) * 256;
+                xl[wg * 128 + row] = l;
+                bar_sync<1, 256>();
+                l = xl[row] + xl[128 + row];
+                bar_sync<1, 256>();
+            }
+            const bool full = cur.unit == 0 && take == units;
+            const int which = cur.unit == 0;   // 1: tail slot, 0: head slot
+            if (!full) {
+                if (which) {
+                    rec.tail = 1;
+                    rec.seq = cur.seq;
+                    rec.tile = cur.tile;
+                    rec.kvh = cur.kvh;
+                } else {
+                    rec.head = cur.unit + take == units ? 2 : 1;
+                }
+            }
+            m -= F::SHIFT;
+            const bool valid = trow < rows;
+            const bool none = lo >= hi;
+            const float inv = none ? 0.f : 1.f / l;
+            const int rr = cur.tile * F::M + (valid ? trow : 0);
+            const int tok = s.q0 + rr / a.group, h = cur.kvh * a.group + rr % a.group;
+            float* slot = ws.slot(blockIdx.x, which, F::M, DP);
+            const int d0 = F::NQ == 1 ? wg * 128 : 0;
+#pragma unroll 1
+            for (int c = 0; c < F::OC / 32; ++c) {
+                uint32_t o[32];
+                __syncwarp();
+                tmem_ld32(t_o + c * 32, o);
+                tmem_wait_ld();
+                const int d = d0 + c * 32;
+                if (!valid) {
+                } else if (!full) {
+                    float* dst = slot + (size_t)trow * DP + d;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        reinterpret_cast<uint4*>(dst)[i] =
+                            make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                } else if (d < a.c.dim) {
+                    TQ* dst = static_cast<TQ*>(a.out) + (int64_t)tok * a.o_ts + (int64_t)h * a.o_hs + d;
+                    constexpr int OK = std::is_same<TQ, __nv_bfloat16>::value ? KIND_BF16 : KIND_F16;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t y[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float v0 = __uint_as_float(o[8 * i + 2 * e]) * inv;
+                            const float v1 = __uint_as_float(o[8 * i + 2 * e + 1]) * inv;
+                            y[e] = none ? 0u : pack16<OK>(v0, v1);
+                        }
+                        reinterpret_cast<uint4*>(dst)[i] = make_uint4(y[0], y[1], y[2], y[3]);
+                    }
+                }
+            }
+            if (valid && d0 == 0) {
+                if (!full) {
+                    slot[(size_t)F::M * DP + 2 * trow] = m;
+                    slot[(size_t)F::M * DP + 2 * trow + 1] = l;
+                } else if (a.lse) {
+                    a.lse[(int64_t)tok * a.q_heads + h] =
+                        none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+                }
+            }
+            __syncwarp();
+            tc_fence_before();
+            if (more) hand_queries();
+            stage0 += 2 * F::KPARTS * take;
+        }
+        if (tid == 0) ws.rec[blockIdx.x] = rec;
+    } else if (warp < 12) {
+        if constexpr (F::Q8)
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        else
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (warp == 9 && lane == 0) {
+            // ------------------------------------------------------- products
+            uint32_t it = 0, seg = 0;
+            int stage0 = 0;
+            auto stage_at = [&](int n) { return smem_u32(sm + F::o_stage + (n % F::NST) * F::STAGEB); };
+            auto wait_stage = [&](int n) {
+                await(&bars->full[n % F::NST], (uint32_t)(n / F::NST));
+            };
+            auto free_stage = [&](int n) { umma_commit(&bars->empty[n % F::NST]); };
+            // S = Q K^T of one query tile with one stage of keys
+            auto score = [&](int tile, int part, uint32_t d, uint32_t kst) {
+                const uint32_t q = smem_u32(sm) + (tile * F::SLABS + part * F::KSLABS) * 16384;
+#pragma unroll
+                for (int sl = 0; sl < F::KSLABS; ++sl)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        umma_f16(d, umma_desc_sw128(q + sl * 16384 + k * 32),
+                                 umma_desc_sw128(kst + sl * 16384 + k * 32), F::IDESC_S,
+                                 part > 0 || sl > 0 || k > 0);
+            };
+            // O += P V with one stage of values
+            auto value = [&](uint32_t d, uint32_t p, uint32_t vst) {
+#pragma unroll
+                for (int k = 0; k < F::VKEYS / 16; ++k)
+                    umma_f16_ts(d, p + k * 8, umma_desc_nmajor(vst + k * 2048, F::VKEYS * 128),
+                                F::IDESC_O);
+            };
+            while (w.open(a)) {
+                const int take = w.take;
+                await(&bars->q_full[0], seg);
+                if constexpr (F::NQ == 2) await(&bars->q_full[1], seg);
+                tc_fence_after();
+                auto scores_of = [&](int j) {   // one tile: S(j) from its stages of keys
+                    const uint32_t b = (it + (j > 0)) & 1;
+#pragma unroll
+                    for (int h = 0; h < F::KPARTS; ++h) {
+                        const int n = stage0 + stage_k<F::NQ>(j) + h;
+                        wait_stage(n);
+                        tc_fence_after();
+                        score(0, h, tmem + b * 128, stage_at(n));
+                        free_stage(n);
+                    }
+                    umma_commit(&bars->s_full[b]);
+                };
+                if constexpr (F::NQ == 2) {
+                    const int n = stage0;
+                    wait_stage(n);
+                    tc_fence_after();
+                    for (int t = 0; t < 2; ++t) {
+                        score(t, 0, tmem + t * 128, stage_at(n));
+                        umma_commit(&bars->s_full[t]);
+                    }
+                    free_stage(n);
+                } else {
+                    scores_of(0);
+                }
+                for (int j = 0; j < take; ++j) {
+                    if constexpr (F::NQ == 2) {
+                        const int nv = stage0 + stage_v<2>(j, take), nk = stage0 + stage_k<2>(j + 1);
+                        wait_stage(nv);
+                        for (int t = 0; t < 2; ++t) {
+                            await(&bars->p_full[t], it);
+                            tc_fence_after();
+                            value(tmem + 256 + t * DP, tmem + t * 128, stage_at(nv));
+                            umma_commit(&bars->pv_done[t]);
+                            if (t == 1) free_stage(nv);
+                            if (j + 1 < take) {
+                                if (t == 0) {
+                                    wait_stage(nk);
+                                    tc_fence_after();
+                                }
+                                score(t, 0, tmem + t * 128, stage_at(nk));
+                                umma_commit(&bars->s_full[t]);
+                                if (t == 1) free_stage(nk);
+                            }
+                        }
+                    } else {
+                        if (j + 1 < take) scores_of(j + 1);
+                        const uint32_t b = it & 1;
+                        await(&bars->p_full[b], it >> 1);
+                        tc_fence_after();
+#pragma unroll
+                        for (int h = 0; h < F::KPARTS; ++h) {
+                            const int n = stage0 + stage_v<1>(j, take) + h;
+                            wait_stage(n);
+                            tc_fence_after();
+                            value(tmem + 256, tmem + b * 128 + h * (F::VKEYS / 2), stage_at(n));
+                            free_stage(n);
+                        }
+                        umma_commit(&bars->pv_done[0]);
+                    }
+                    ++it;
+                }
+                stage0 += 2 * F::KPARTS * take;
+                ++seg;
+                w.next(a);
+            }
+            // every product has been waited for by the softmax warps
+        } else if (!F::Q8 && warp == 8) {
+            // --------------------------------------------------------- copies
+            int stage0 = 0;
+            const int piece = a.c.page_size < kManyKeys ? a.c.page_size : kManyKeys;
+            const int vpiece = piece < F::VKEYS ? piece : F::VKEYS;
+            const int pieces = kManyKeys / piece;
+            while (w.open(a)) {
+                const int take = w.take;
+                // lane i: page of the unit's i-th piece
+                auto page_at = [&](int j) {
+                    const int key = (w.u0 + j) * kManyKeys + lane * piece;
+                    if (j >= take || lane >= pieces || key >= w.s.len) return -1;
+                    return kv_page(a.b, a.c, w.cur.seq, key >> a.c.page_shift, a.status);
+                };
+                auto fill = [&](int n, const CUtensorMap* map, int page_id, int key0, int keys,
+                                int step, int x0, int slabs) {
+                    const int slot = n % F::NST;
+                    if (n >= F::NST) await(&bars->empty[slot], (uint32_t)(n / F::NST) + 1);
+                    const int boxes = keys / step;
+                    const int b = lane % boxes, sl = lane / boxes;
+                    const int key = key0 + b * step;
+                    const int page = __shfl_sync(0xffffffffu, page_id,
+                                                 (key & (kManyKeys - 1)) / piece);
+                    const bool go = sl < slabs && page >= 0;
+                    const int n_go = __popc(__ballot_sync(0xffffffffu, go));
+                    if (lane == 0) mbar_arrive_expect_tx(&bars->full[slot], n_go * step * 128);
+                    __syncwarp();
+                    if (go)
+                        tma_load_3d(sm + F::o_stage + slot * F::STAGEB + sl * keys * 128 + b * step * 128,
+                                    map, x0 + sl * 64, key & (a.c.page_size - 1),
+                                    page * a.c.heads + w.cur.kvh, &bars->full[slot]);
+                };
+                int page = page_at(0);
+                auto keys_of = [&](int j, int pg) {
+                    for (int h = 0; h < F::KPARTS; ++h)
+                        fill(stage0 + stage_k<F::NQ>(j) + h, &kmap, pg, (w.u0 + j) * kManyKeys,
+                             kManyKeys, piece, h * 128, F::KSLABS);
+                };
+                keys_of(0, page);
+                for (int j = 0; j < take; ++j) {
+                    const int ahead = page_at(j + 1);
+                    if (F::NQ == 1 && j + 1 < take) keys_of(j + 1, ahead);
+                    for (int h = 0; h < F::KPARTS; ++h)
+                        fill(stage0 + stage_v<F::NQ>(j, take) + h, &vmap, page,
+                             (w.u0 + j) * kManyKeys + h * F::VKEYS, F::VKEYS, vpiece, 0, F::SLABS);
+                    if (F::NQ == 2 && j + 1 < take) keys_of(j + 1, ahead);
+                    page = ahead;
+                }
+                stage0 += 2 * F::KPARTS * take;
+                w.next(a);
+            }
+        }
+    } else if constexpr (F::Q8) {
+        // ------------------------------------------------------ Q8_0 decoding
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        const int t = tid - 384, nb = a.c.dim >> 5;
+        constexpr int CH = F::STAGEB / 32 / 128;   // 16-code chunks of a thread and stage
+        constexpr int KC = F::KSLABS * 4;          // chunks of a row in a stage of keys
+        constexpr int VC = F::SLABS * 4;           // chunks of a row in a stage of values
+        int stage0 = 0;
+        while (w.open(a)) {
+            const int take = w.take;
+            const int total = 2 * F::KPARTS * take;
+            uint4 code[2][CH];
+            uint32_t scl[2][(CH + 1) / 2];
+            // loads the codes of the segment's n-th stage
+            auto load = [&](int n, uint4 (&cd)[CH], uint32_t (&sc)[(CH + 1) / 2], bool& is_v) {
+                if (n >= total) return;
+                int j, h;
+                if (F::NQ == 2) {
+                    j = n >> 1;
+                    is_v = n & 1;
+                    h = 0;
+                } else {
+                    const int g = n >> 1;   // K0 | K1 V0 | K2 V1 | ... | V(take-1)
+                    h = n & 1;
+                    is_v = g > 0 && (!(g & 1) || g == 2 * take - 1);
+                    j = g == 0 ? 0 : g == 2 * take - 1 ? take - 1 : is_v ? g / 2 - 1 : (g + 1) / 2;
+                }
+                const int key0 = (w.u0 + j) * kManyKeys + (is_v ? h * F::VKEYS : 0);
+                const int x0 = is_v ? 0 : h * 128;
+                const int per = is_v ? VC : KC;
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    const int idx = c * 128 + t;
+                    const int key = key0 + idx / per, d = x0 + idx % per * 16;
+                    cd[c] = make_uint4(0, 0, 0, 0);
+                    uint32_t sc16 = 0;
+                    if (key < w.s.len && d < a.c.dim) {
+                        const int page = kv_page(a.b, a.c, w.cur.seq, key >> a.c.page_shift, a.status);
+                        if (page >= 0) {
+                            const int64_t r = (((int64_t)page * a.c.heads + w.cur.kvh) << a.c.page_shift) +
+                                              (key & (a.c.page_size - 1));
+                            cd[c] = __ldg(reinterpret_cast<const uint4*>(
+                                static_cast<const int8_t*>(is_v ? a.c.v : a.c.k) + r * a.c.dim + d));
+                            sc16 = __half_as_ushort((is_v ? a.c.vs : a.c.ks)[r * nb + (d >> 5)]);
+                        }
+                    }
+                    if (c & 1) sc[c / 2] |= sc16 << 16; else sc[c / 2] = sc16;
+                }
+            };
+            auto store = [&](int n, uint4 (&cd)[CH], uint32_t (&sc)[(CH + 1) / 2], bool is_v) {
+                const int slot = (stage0 + n) % F::NST;
+                if (stage0 + n >= F::NST) await(&bars->empty[slot], (uint32_t)((stage0 + n) / F::NST) + 1);
+                unsigned char* st = sm + F::o_stage + slot * F::STAGEB;
+                const int per = is_v ? VC : KC, keys = is_v ? F::VKEYS : kManyKeys;
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    const int idx = c * 128 + t;
+                    const int r = idx / per, q = idx % per;
+                    const __half2 d = __half2half2(
+                        __ushort_as_half((unsigned short)(c & 1 ? sc[c / 2] >> 16 : sc[c / 2])));
+                    uint32_t x[8];
+                    const uint32_t* cw = reinterpret_cast<const uint32_t*>(&cd[c]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) codes4(cw[i], d, x[2 * i], x[2 * i + 1]);
+                    unsigned char* slab = st + (q >> 2) * keys * 128;
+                    const int c0 = (q & 3) * 2;
+                    // lanes of the odd slabs store their second half first, so
+                    // that eight lanes cover eight different 16-byte columns
+                    const int first = (q >> 2) & 1;
+                    const uint4 lo4 = make_uint4(x[0], x[1], x[2], x[3]);
+                    const uint4 hi4 = make_uint4(x[4], x[5], x[6], x[7]);
+                    *reinterpret_cast<uint4*>(slab + sw128_offset(r, c0 + first)) = first ? hi4 : lo4;
+                    *reinterpret_cast<uint4*>(slab + sw128_offset(r, c0 + 1 - first)) = first ? lo4 : hi4;
+                }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars->full[slot]);
+            };
+            bool v0 = false, v1 = false;
+            load(0, code[0], scl[0], v0);
+            for (int n = 0; n < total; n += 2) {
+                load(n + 1, code[1], scl[1], v1);
+                store(n, code[0], scl[0], v0);
+                load(n + 2, code[0], scl[0], v0);
+                if (n + 1 < total) store(n + 1, code[1], scl[1], v1);
+            }
+            stage0 += total;
+            w.next(a);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (tid == 0 && *reinterpret_cast<volatile uint32_t*>(&bars->lost)) kv_flag(a.status, KV_TIMEOUT);
+    if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+template <int DP, int KIND, typename TQ>
+cudaError_t launch_many(const AttendArgs& a, void* ws, cudaStream_t s) {
+    using F = Many<DP, KIND>;
+    CUtensorMap kmap{}, vmap{};
+    if (!F::Q8) {
+        const int piece = a.c.page_size < kManyKeys ? a.c.page_size : kManyKeys;
+        if (!attend_map(&kmap, a.c, a.c.k, 64, piece) ||
+            !attend_map(&vmap, a.c, a.c.v, 64, piece < F::VKEYS ? piece : F::VKEYS))
+            return cudaErrorInvalidValue;
+    }
+    cudaError_t e = cudaFuncSetAttribute(k_attend_many<DP, KIND, TQ>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, F::smem);
+    if (e != cudaSuccess) return e;
+    k_attend_many<DP, KIND, TQ><<<sm_count(), F::THREADS, F::smem, s>>>(kmap, vmap, a, ws);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    return launch_attend_join(a, ws, sm_count(), F::M, DP, s);
+}
+
+template <int DP>
+cudaError_t launch_dim(const AttendArgs& a, void* ws, cudaStream_t s) {
+    if (a.c.type == KV_F16) return launch_many<DP, KIND_F16, __half>(a, ws, s);
+    if (a.c.type == KV_BF16) return launch_many<DP, KIND_BF16, __nv_bfloat16>(a, ws, s);
+    if (a.type == KV_F16) return launch_many<DP, KIND_Q8, __half>(a, ws, s);
+    return launch_many<DP, KIND_Q8, __nv_bfloat16>(a, ws, s);
+}
+
+}  // namespace
+
+cudaError_t launch_attend_many(const AttendArgs& a, void* ws, cudaStream_t s) {
+    const int dp = attend_dim(a.c.dim);
+    if (dp == 64) return launch_dim<64>(a, ws, s);
+    if (dp == 128) return launch_dim<128>(a, ws, s);
+    return launch_dim<256>(a, ws, s);
+}
+
+}  // namespace moeb200
