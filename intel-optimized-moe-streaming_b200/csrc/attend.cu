@@ -13,101 +13,150 @@ namespace moeb200 {
 
 namespace {
 
-constexpr int kJoinThreads = 256;
+constexpr int kJoinWarps = 8;
 
 // Adds the pieces of the tiles that were split over CTAs, in CTA order: the
 // CTA with a tail owns its tile, the pieces are its tail and the heads of the
-// CTAs behind it up to the one that finished the tile.  grid (ctas, slices of
-// rows); a row is spread over DP / 4 threads, several groups of threads take
-// every other piece and are added in order.
-template <typename TO, int DP>
-__global__ void __launch_bounds__(kJoinThreads) k_attend_join(AttendArgs a, void* wsp, int ctas,
-                                                              int M, int rows_per_block) {
-    constexpr int kCols = DP / 4;                    // threads of a row
-    constexpr int kGroups = kJoinThreads / kCols;    // pieces taken at once
-    __shared__ float4 part[kGroups][kCols];
-    __shared__ float part_l[kGroups];
+// CTAs behind it up to the one that finished the tile.  grid (ctas, rows /
+// rows of a block); WPR warps share a row, each taking every WPR-th piece,
+// and are added in order.  A chain of four dependent loads and one pass over
+// the pieces: latency, so rows are spread over as many warps as there are.
+template <typename TO, int DP, int WPR>
+__global__ void __launch_bounds__(kJoinWarps * 32) k_attend_join(AttendArgs a, void* wsp, int ctas,
+                                                                 int M) {
+    constexpr int V = DP / 64;   // float2 of a lane
+    __shared__ float2 part[WPR > 1 ? kJoinWarps : 1][V][32];
+    __shared__ float part_l[kJoinWarps], part_m[kJoinWarps];
     pdl_enter();
     const AttendWs ws(wsp, ctas);
-    const int cta = blockIdx.x;
+    const int cta = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const AttendRecord rec = ws.rec[cta];
     if (!rec.tail) return;
-    int pieces = 1;
-    for (int i = cta + 1; i < ctas; ++i) {
-        ++pieces;
-        if (ws.rec[i].head == 2) break;
-    }
     const AttendSeq s = attend_seq(a, rec.seq, nullptr);
-    const int col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
-    for (int i = 0; i < rows_per_block; ++i) {
-        const int row = blockIdx.y * rows_per_block + i;
-        const int r = rec.tile * M + row;
-        if (row >= M || r >= s.n * a.group) return;
-        // the pieces' maxima first, then one pass over their sums
-        float top = -INFINITY;
-        for (int p = 0; p < pieces; ++p) {
-            const float* sl = ws.slot(cta + p, p == 0, M, DP);
-            top = fmaxf(top, sl[(size_t)M * DP + 2 * row]);
+    const int row = blockIdx.y * (kJoinWarps / WPR) + warp / WPR;
+    const int sub = warp % WPR;
+    const int r = rec.tile * M + row;
+    const bool valid = row < M && r < s.n * a.group;
+    int pieces = 1;
+    for (int i = cta + 1; i < ctas; i += 32) {   // up to the first head that ends the tile
+        const bool last = i + lane < ctas && ws.rec[i + lane].head == 2;
+        const unsigned found = __ballot_sync(0xffffffffu, last);
+        if (found) {
+            pieces += __ffs(found);
+            break;
         }
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        float l = 0.f;
-        for (int p = grp; p < pieces; p += kGroups) {
-            const float* sl = ws.slot(cta + p, p == 0, M, DP);
-            const float m = sl[(size_t)M * DP + 2 * row];
-            const float f = m == -INFINITY ? 0.f : exp2f(m - top);
-            const float4 v = reinterpret_cast<const float4*>(sl + (size_t)row * DP)[col];
-            l += f * sl[(size_t)M * DP + 2 * row + 1];
-            o.x += f * v.x;
-            o.y += f * v.y;
-            o.z += f * v.z;
-            o.w += f * v.w;
-        }
-        part[grp][col] = o;
-        if (col == 0) part_l[grp] = l;
-        __syncthreads();
-        if (grp == 0) {
-            for (int g = 1; g < kGroups; ++g) {
-                const float4 v = part[g][col];
-                o.x += v.x;
-                o.y += v.y;
-                o.z += v.z;
-                o.w += v.w;
-                l += part_l[g];
-            }
-            const int tok = r / a.group, h = rec.kvh * a.group + r % a.group;
-            int lo, hi;
-            attend_range(s.first + tok, s.len, a.causal, a.window, lo, hi);
-            const bool none = lo >= hi;
-            const float inv = none ? 0.f : 1.f / l;
-            if (none) o = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (col * 4 < a.c.dim) {
-                TO y[4] = {kv_from_f<TO>(o.x * inv), kv_from_f<TO>(o.y * inv),
-                           kv_from_f<TO>(o.z * inv), kv_from_f<TO>(o.w * inv)};
-                TO* out = static_cast<TO*>(a.out) + (int64_t)(s.q0 + tok) * a.o_ts +
-                          (int64_t)h * a.o_hs + col * 4;
-                *reinterpret_cast<uint2*>(out) = *reinterpret_cast<uint2*>(y);
-            }
-            if (a.lse && col == 0)
-                a.lse[(int64_t)(s.q0 + tok) * a.q_heads + h] =
-                    none ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
-        }
-        __syncthreads();
+        pieces += 32;
     }
+    pieces = pieces < ctas - cta ? pieces : ctas - cta;
+    float top = -INFINITY, l = 0.f;
+    float2 o[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) o[v] = make_float2(0.f, 0.f);
+    if (valid) {
+        // lane p holds the maximum and the sum of piece p of a group of 32
+        for (int p0 = sub; p0 < pieces; p0 += 32 * WPR) {
+            const int p = p0 + lane * WPR;
+            float2 ml = make_float2(-INFINITY, 0.f);
+            if (p < pieces)
+                ml = *reinterpret_cast<const float2*>(ws.slot(cta + p, p == 0, M, DP) +
+                                                      (size_t)M * DP + 2 * row);
+            const float high = fmaxf(top, warp_max(ml.x));
+            if (high > top) {
+                const float f = exp2f(top - high);
+                l *= f;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    o[v].x *= f;
+                    o[v].y *= f;
+                }
+                top = high;
+            }
+            const float mine = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
+            l += warp_sum(mine * ml.y);
+            const int left = (pieces - p0 + WPR - 1) / WPR;
+            const int n = left < 32 ? left : 32;
+#pragma unroll 4
+            for (int i = 0; i < n; ++i) {
+                const int q = p0 + i * WPR;
+                const float f = __shfl_sync(0xffffffffu, mine, i);
+                const float* sl = ws.slot(cta + q, q == 0, M, DP) + 4 * row + 2 * (lane & 1);
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const float2 x =
+                        *reinterpret_cast<const float2*>(sl + (v * 16 + (lane >> 1)) * 4 * M);
+                    o[v].x = fmaf(f, x.x, o[v].x);
+                    o[v].y = fmaf(f, x.y, o[v].y);
+                }
+            }
+        }
+    }
+    if constexpr (WPR > 1) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) part[warp][v][lane] = o[v];
+        if (lane == 0) {
+            part_m[warp] = top;
+            part_l[warp] = l;
+        }
+        __syncthreads();
+        if (sub) return;
+        float high = top;
+        for (int w = 1; w < WPR; ++w) high = fmaxf(high, part_m[warp + w]);
+        l = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] = make_float2(0.f, 0.f);
+        for (int w = 0; w < WPR; ++w) {
+            const float pm = part_m[warp + w];
+            const float f = pm == -INFINITY ? 0.f : exp2f(pm - high);
+            l = fmaf(f, part_l[warp + w], l);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float2 x = part[warp + w][v][lane];
+                o[v].x = fmaf(f, x.x, o[v].x);
+                o[v].y = fmaf(f, x.y, o[v].y);
+            }
+        }
+        top = high;
+    }
+    if (!valid) return;
+    const int tok = a.by_group.div(r), h = rec.kvh * a.group + r - tok * a.group;
+    int lo, hi;
+    attend_range(s.first + tok, s.len, a.causal, a.window, lo, hi);
+    const bool none = lo >= hi;
+    const float inv = 1.f / l;
+    TO* out = static_cast<TO*>(a.out) + (int64_t)(s.q0 + tok) * a.o_ts + (int64_t)h * a.o_hs;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int d = v * 64 + lane * 2;
+        if (d < a.c.dim) {
+            TO y[2] = {kv_from_f<TO>(none ? 0.f : o[v].x * inv), kv_from_f<TO>(none ? 0.f : o[v].y * inv)};
+            *reinterpret_cast<uint32_t*>(out + d) = *reinterpret_cast<uint32_t*>(y);
+        }
+    }
+    if (a.lse && lane == 0)
+        a.lse[(int64_t)(s.q0 + tok) * a.q_heads + h] =
+            none ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
 }
 
-template <typename TO, int DP>
-cudaError_t join(const AttendArgs& a, void* ws, int ctas, int M, cudaStream_t s) {
-    const int rows = M <= 16 ? 4 : 8;
+template <typename TO, int DP, int WPR>
+cudaError_t join_as(const AttendArgs& a, void* ws, int ctas, int M, cudaStream_t s) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ctas, (M + rows - 1) / rows);
-    cfg.blockDim = dim3(kJoinThreads);
+    cfg.gridDim = dim3(ctas, M * WPR / kJoinWarps);
+    cfg.blockDim = dim3(kJoinWarps * 32);
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_attend_join<TO, DP>, a, ws, ctas, M, rows);
+    return cudaLaunchKernelEx(&cfg, k_attend_join<TO, DP, WPR>, a, ws, ctas, M);
+}
+
+// Few rows: up to all CTAs' pieces in a row, four warps share them.  Many
+// rows: a few pieces, a warp per row.
+template <typename TO, int DP>
+cudaError_t join(const AttendArgs& a, void* ws, int ctas, int M, cudaStream_t s) {
+    return M == kFewRows ? join_as<TO, DP, 4>(a, ws, ctas, M, s)
+                         : join_as<TO, DP, 1>(a, ws, ctas, M, s);
 }
 
 }  // namespace

@@ -16,6 +16,23 @@
 
 namespace moeb200 {
 
+// Quotients by a divisor d set on the host: with s = ceil(log2 d) and
+// m = floor(2^32 (2^s - d) / d) + 1, n / d = (mulhi(n, m) + n) >> s for
+// 0 <= n < 2^31.
+struct FastDiv {
+    uint32_t d, m, s;
+    FastDiv() = default;
+    explicit FastDiv(int by) : d((uint32_t)by), m(0), s(0) {
+        while ((1ull << s) < d) ++s;
+        m = (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1);
+    }
+#ifdef __CUDACC__
+    __device__ __forceinline__ int div(int n) const {
+        return (int)((__umulhi((uint32_t)n, m) + (uint32_t)n) >> s);
+    }
+#endif
+};
+
 struct AttendArgs {
     KvBatch b;
     KvCache c;
@@ -25,6 +42,7 @@ struct AttendArgs {
     int64_t q_ts, q_hs, o_ts, o_hs;
     int type;         // of q and out
     int q_heads, group;
+    FastDiv by_group;
     float scale;
     int causal, window;
     unsigned* status;
@@ -39,7 +57,9 @@ struct AttendRecord {
 };
 
 // Workspace: one record per CTA, then two slots per CTA (head, tail) of M rows
-// of DP sums with each row's maximum (in units of log 2) and softmax sum.
+// of DP sums with each row's maximum (in units of log 2) and softmax sum.  Sum
+// d of a row is at (d / 4 * M + row) * 4 + d % 4: threads that own a row each
+// write whole lines.
 struct AttendWs {
     AttendRecord* rec;
     float* slots;
@@ -120,22 +140,32 @@ __device__ __forceinline__ AttendSeq attend_seq(const AttendArgs& a, int b, unsi
     return s;
 }
 
-// Units [lo, hi) of KT keys of a tile of rows r0 .. r0 + M - 1; a tile whose
-// rows attend nothing still has one unit, in which its zeros are written.
+// First and last row of a tile of rows r0 .. r0 + M - 1 attend keys from t_lo
+// and up to t_hi; every row attends [all_lo, all_hi).
+struct AttendTile {
+    int t_lo, t_hi, all_lo, all_hi;
+};
+
+__device__ __forceinline__ AttendTile attend_tile(const AttendArgs& a, const AttendSeq& s, int r0,
+                                                  int M) {
+    const int last = s.n * a.group - 1;
+    const int r1 = r0 + M - 1 < last ? r0 + M - 1 : last;
+    AttendTile t;
+    attend_range(s.first + a.by_group.div(r0), s.len, a.causal, a.window, t.t_lo, t.all_hi);
+    attend_range(s.first + a.by_group.div(r1), s.len, a.causal, a.window, t.all_lo, t.t_hi);
+    return t;
+}
+
+// Units [lo, hi) of KT keys of a tile; one whose rows attend nothing still has
+// a unit, in which its zeros are written.
 template <int M, int KT>
 __device__ __forceinline__ void attend_units(const AttendArgs& a, const AttendSeq& s, int tile,
                                              int& lo, int& hi) {
-    const int r0 = tile * M;
-    int r1 = r0 + M - 1;
-    const int last = s.n * a.group - 1;
-    r1 = r1 < last ? r1 : last;
-    int l0, h0, l1, h1;
-    attend_range(s.first + r0 / a.group, s.len, a.causal, a.window, l0, h0);
-    attend_range(s.first + r1 / a.group, s.len, a.causal, a.window, l1, h1);
+    const AttendTile t = attend_tile(a, s, tile * M, M);
     lo = hi = 0;
-    if (h1 > l0) {
-        lo = l0 / KT;
-        hi = (h1 + KT - 1) / KT;
+    if (t.t_hi > t.t_lo) {
+        lo = t.t_lo / KT;
+        hi = (t.t_hi + KT - 1) / KT;
     }
     if (hi <= lo) hi = lo + 1;
 }
@@ -148,38 +178,61 @@ __device__ __forceinline__ int attend_tiles(const AttendArgs& a, const AttendSeq
 // A CTA's place on the line of units.
 struct AttendCursor {
     int seq, tile, kvh;
-    int unit;         // units of the tile already behind
-    int64_t left;     // units this CTA still has to do
+    int unit;         // length of the tile already behind
+    int64_t left;     // length of line this CTA still has to do
 };
 
-// Finds the stretch of CTA `cta` of `ctas`: every thread sums the units of its
-// share of the sequences, a block scan places the shares, and the thread whose
-// share holds the stretch's first unit walks to it.  At least `least` units go
-// to a CTA.  Returns in every thread; left = 0: nothing to do.  The scratch is
-// shared memory that the caller may use for something else afterwards.
 struct AttendScratch {
     int64_t warp_total[16];
     AttendCursor found;
 };
 
-template <int M, int KT, int THREADS>
+// Finds the stretch of CTA `cta` of `ctas`.  A tile is COST + units long (COST:
+// what starting and ending it takes, in units; a cut inside that part gives
+// the whole tile to the later CTA), once per key/value head.  A thread sums
+// its share of the sequences, the tiles of a long one being spread over its
+// warp; a block scan places the shares, and the warp whose share holds the
+// stretch's start walks to it.  Returns in every thread; left = 0: nothing to
+// do.  The scratch is shared memory that the caller may use for something else
+// afterwards.
+template <int M, int KT, int COST, int THREADS>
 __device__ AttendCursor attend_place(const AttendArgs& a, AttendScratch& scratch, int cta,
-                                     int ctas, int least, unsigned* status) {
-    int64_t* warp_total = scratch.warp_total;
-    AttendCursor& found = scratch.found;
+                                     int ctas, unsigned* status) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int share = (a.b.B + THREADS - 1) / THREADS;
-    const int b0 = tid * share;
-    const int b1 = b0 + share < a.b.B ? b0 + share : a.b.B;
     int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) {
-        const AttendSeq s = attend_seq(a, b, cta == 0 ? status : nullptr);
-        const int tiles = attend_tiles<M>(a, s);
+    for (int i = 0; i < share; ++i) {
+        const int b = tid * share + i;
+        AttendSeq s{};
+        int tiles = 0;
+        if (b < a.b.B) {
+            s = attend_seq(a, b, cta == 0 ? status : nullptr);
+            tiles = attend_tiles<M>(a, s);
+        }
         int64_t sum = 0;
-        for (int t = 0; t < tiles; ++t) {
-            int lo, hi;
-            attend_units<M, KT>(a, s, t, lo, hi);
-            sum += hi - lo;
+        if (tiles <= 4)
+            for (int t = 0; t < tiles; ++t) {
+                int lo, hi;
+                attend_units<M, KT>(a, s, t, lo, hi);
+                sum += hi - lo + COST;
+            }
+        for (unsigned many = __ballot_sync(0xffffffffu, tiles > 4); many; many &= many - 1) {
+            const int from = __ffs(many) - 1;
+            AttendSeq q;
+            q.q0 = 0;
+            q.n = __shfl_sync(0xffffffffu, s.n, from);
+            q.len = __shfl_sync(0xffffffffu, s.len, from);
+            q.first = __shfl_sync(0xffffffffu, s.first, from);
+            const int n = __shfl_sync(0xffffffffu, tiles, from);
+            int part = 0;
+            for (int t = lane; t < n; t += 32) {
+                int lo, hi;
+                attend_units<M, KT>(a, q, t, lo, hi);
+                part += hi - lo + COST;
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+            if (lane == from) sum = part;
         }
         mine += sum * a.c.heads;
     }
@@ -189,48 +242,90 @@ __device__ AttendCursor attend_place(const AttendArgs& a, AttendScratch& scratch
         const int64_t up = __shfl_up_sync(0xffffffffu, before, o);
         if (lane >= o) before += up;
     }
-    if (lane == 31) warp_total[warp] = before;
-    if (tid == 0) found.left = 0;
+    if (lane == 31) scratch.warp_total[warp] = before;
+    if (tid == 0) scratch.found.left = 0;
     __syncthreads();
     before -= mine;
     int64_t total = 0;
 #pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) {
-        if (w < warp) before += warp_total[w];
-        total += warp_total[w];
+        if (w < warp) before += scratch.warp_total[w];
+        total += scratch.warp_total[w];
     }
+    const int64_t least = COST + 1;
     int64_t active = (total + least - 1) / least;
     active = active < ctas ? active : ctas;
+    int64_t start = -1, end = -1;
     if (cta < active) {
-        const int64_t start = total * cta / active, end = total * (cta + 1) / active;
-        if (start >= before && start < before + mine) {
-            int64_t skip = start - before;
-            for (int b = b0; b < b1; ++b) {
-                const AttendSeq s = attend_seq(a, b, nullptr);
-                const int tiles = attend_tiles<M>(a, s);
-                int t = 0;
-                for (; t < tiles; ++t) {
-                    int lo, hi;
-                    attend_units<M, KT>(a, s, t, lo, hi);
-                    const int64_t n = (int64_t)(hi - lo) * a.c.heads;
-                    if (skip < n) {
-                        found.seq = b;
-                        found.tile = t;
-                        found.kvh = (int)(skip / (hi - lo));
-                        found.unit = (int)(skip % (hi - lo));
-                        found.left = end - start;
-                        break;
-                    }
-                    skip -= n;
+        start = total * cta / active;
+        end = total * (cta + 1) / active;
+    }
+    const unsigned owner = __ballot_sync(0xffffffffu, start >= before && start < before + mine);
+    if (owner) {
+        const int from = __ffs(owner) - 1;
+        int64_t skip = start - __shfl_sync(0xffffffffu, before, from);
+        const int b0 = (warp * 32 + from) * share;
+        bool done = false;
+        for (int b = b0; b < b0 + share && b < a.b.B && !done; ++b) {
+            const AttendSeq s = attend_seq(a, b, nullptr);
+            const int tiles = attend_tiles<M>(a, s);
+            for (int t0 = 0; t0 < tiles && !done; t0 += 32) {
+                int64_t n = 0;
+                int lo = 0, hi = 0;
+                if (t0 + lane < tiles) {
+                    attend_units<M, KT>(a, s, t0 + lane, lo, hi);
+                    n = (int64_t)(hi - lo + COST) * a.c.heads;
                 }
-                if (t < tiles) break;
+                int64_t upto = n;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int64_t up = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += up;
+                }
+                if (skip >= upto - n && skip < upto) {
+                    const int at = (int)(skip - (upto - n)), size = hi - lo + COST;
+                    scratch.found.seq = b;
+                    scratch.found.tile = t0 + lane;
+                    scratch.found.kvh = at / size;
+                    scratch.found.unit = at % size;
+                    scratch.found.left = end - start;
+                }
+                const int64_t all = __shfl_sync(0xffffffffu, upto, 31);
+                done = skip < all;
+                skip -= all;
             }
         }
     }
     __syncthreads();
-    const AttendCursor c = found;
+    const AttendCursor c = scratch.found;
     __syncthreads();   // the scratch may be overwritten
     return c;
+}
+
+// The part of the cursor's tile that falls to this CTA: units u0 ..
+// u0 + take - 1 (take may be 0), `begins` / `ends` when these include the
+// tile's first and last.  Advance the cursor's `left` by `used`.
+struct AttendPart {
+    int u0, take;
+    int64_t used;
+    bool begins, ends;
+};
+
+template <int M, int KT, int COST>
+__device__ __forceinline__ AttendPart attend_part(const AttendArgs& a, const AttendCursor& c,
+                                                  const AttendSeq& s) {
+    int lo, hi;
+    attend_units<M, KT>(a, s, c.tile, lo, hi);
+    const int size = hi - lo + COST;
+    const int end = c.left < size - c.unit ? c.unit + (int)c.left : size;
+    const int u0 = c.unit > COST ? c.unit - COST : 0, u1 = end > COST ? end - COST : 0;
+    AttendPart p;
+    p.u0 = lo + u0;
+    p.take = u1 - u0;
+    p.used = end - c.unit;
+    p.begins = u0 == 0;
+    p.ends = end == size;
+    return p;
 }
 
 // Moves to the next tile that has rows (head, then tile, then sequence); `s`

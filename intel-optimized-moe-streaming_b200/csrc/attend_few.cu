@@ -33,6 +33,7 @@ constexpr int kFewWarps = 4;
 constexpr int kFewThreads = kFewWarps * 32;
 constexpr int kFewKeys = 16;                     // keys of a subtile
 constexpr int kFewUnit = kFewKeys * kFewWarps;   // keys of a unit
+constexpr int kFewCost = 0;                      // of a tile, in units
 constexpr uint32_t kFewPolls = 1u << 21;
 
 template <int DP, int KIND>
@@ -141,8 +142,8 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
 
     const int ctas = gridDim.x;
     AttendWs ws(wsp, ctas);
-    AttendCursor cur = attend_place<kFewRows, kFewUnit, kFewThreads>(
-        a, *reinterpret_cast<AttendScratch*>(sm), blockIdx.x, ctas, 1, a.status);
+    AttendCursor cur = attend_place<kFewRows, kFewUnit, kFewCost, kFewThreads>(
+        a, *reinterpret_cast<AttendScratch*>(sm), blockIdx.x, ctas, a.status);
     fence_async_smem();   // the scratch lies in the ring
     AttendRecord rec{};
     int in_slot = 0, out_slot = 0;        // ring positions to fill and to read next
@@ -152,12 +153,8 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
     if (cur.left > 0) s = attend_seq(a, cur.seq, nullptr);
 
     while (cur.left > 0) {
-        int u_lo, u_hi;
-        attend_units<kFewRows, kFewUnit>(a, s, cur.tile, u_lo, u_hi);
-        const int units = u_hi - u_lo;
-        const int64_t room = units - cur.unit;
-        const int take = (int)(room < cur.left ? room : cur.left);
-        const int u0 = u_lo + cur.unit;
+        const AttendPart part = attend_part<kFewRows, kFewUnit, kFewCost>(a, cur, s);
+        const int u0 = part.u0, take = part.take;
         const int rows = s.n * a.group - cur.tile * kFewRows;   // valid rows: the first `rows`
 
         // queries as A fragments; bf16 ones over a Q8_0 cache become binary16
@@ -169,9 +166,9 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
                     float top = 0.f;
                     if (r < rows) {
                         const int rr = cur.tile * kFewRows + r;
-                        const TQ* q = static_cast<const TQ*>(a.q) +
-                                      (int64_t)(s.q0 + rr / a.group) * a.q_ts +
-                                      (int64_t)(cur.kvh * a.group + rr % a.group) * a.q_hs;
+                        const int tok = a.by_group.div(rr);
+                        const TQ* q = static_cast<const TQ*>(a.q) + (int64_t)(s.q0 + tok) * a.q_ts +
+                                      (int64_t)(cur.kvh * a.group + rr - tok * a.group) * a.q_hs;
                         for (int d = lane; d < a.c.dim; d += 32) top = fmaxf(top, fabsf(kv_to_f<TQ>(q[d])));
                     }
                     top = warp_max(top);
@@ -192,9 +189,9 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
                 w[j] = 0;
                 if (r < rows && d < a.c.dim) {
                     const int rr = cur.tile * kFewRows + r;
-                    const TQ* q = static_cast<const TQ*>(a.q) +
-                                  (int64_t)(s.q0 + rr / a.group) * a.q_ts +
-                                  (int64_t)(cur.kvh * a.group + rr % a.group) * a.q_hs + d;
+                    const int tok = a.by_group.div(rr);
+                    const TQ* q = static_cast<const TQ*>(a.q) + (int64_t)(s.q0 + tok) * a.q_ts +
+                                  (int64_t)(cur.kvh * a.group + rr - tok * a.group) * a.q_hs + d;
                     w[j] = *reinterpret_cast<const uint32_t*>(q);
                     if constexpr (F::Q8 && std::is_same<TQ, __nv_bfloat16>::value)
                         w[j] = pack16<KIND_F16>(kv_to_f<TQ>(q[0]) * sm_rs[r],
@@ -212,16 +209,11 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
             const int r = n8 + 8 * i;
             lo[i] = hi[i] = 0;
             if (r < rows)
-                attend_range(s.first + (cur.tile * kFewRows + r) / a.group, s.len, a.causal,
+                attend_range(s.first + a.by_group.div(cur.tile * kFewRows + r), s.len, a.causal,
                              a.window, lo[i], hi[i]);
         }
-        // keys that any row of the tile attends, and those that all attend
-        int t_lo, t_hi, all_lo, all_hi;
-        {
-            const int r0 = cur.tile * kFewRows, r1 = r0 + (rows < 16 ? rows : 16) - 1;
-            attend_range(s.first + r0 / a.group, s.len, a.causal, a.window, t_lo, all_hi);
-            attend_range(s.first + r1 / a.group, s.len, a.causal, a.window, all_lo, t_hi);
-        }
+        const AttendTile tile = attend_tile(a, s, cur.tile * kFewRows, kFewRows);
+        const int t_lo = tile.t_lo, t_hi = tile.t_hi, all_lo = tile.all_lo, all_hi = tile.all_hi;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -575,8 +567,8 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
             keep[i] = m[i] == -INFINITY ? 0.f : ex2(m[i] - mm);
             if (lost) keep[i] = 0.f;
         }
-        const bool full = cur.unit == 0 && take == units;
-        const int which = cur.unit == 0;   // 1: tail slot, 0: head slot
+        const bool full = part.begins && part.ends;
+        const int which = part.begins;   // 1: tail slot, 0: head slot
         float* slot = ws.slot(blockIdx.x, which, kFewRows, DP);
         if (!full) {
             if (which) {
@@ -585,7 +577,7 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
                 rec.tile = cur.tile;
                 rec.kvh = cur.kvh;
             } else {
-                rec.head = cur.unit + take == units ? 2 : 1;
+                rec.head = part.ends ? 2 : 1;
             }
         }
 #pragma unroll
@@ -622,14 +614,14 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
                     ll += sm_l[w * 16 + r] *
                           (sm_m[w * 16 + r] == -INFINITY ? 0.f : ex2(sm_m[w * 16 + r] - mm));
                 if (!full) {
-                    *reinterpret_cast<float4*>(slot + r * DP + d) = v;
+                    *reinterpret_cast<float4*>(slot + (d / 4 * kFewRows + r) * 4) = v;
                     if (d == 0) {
                         slot[kFewRows * DP + 2 * r] = mm;
                         slot[kFewRows * DP + 2 * r + 1] = ll;
                     }
                 } else if (r < rows) {
                     const int rr = cur.tile * kFewRows + r;
-                    const int tok = rr / a.group, h = cur.kvh * a.group + rr % a.group;
+                    const int tok = a.by_group.div(rr), h = cur.kvh * a.group + rr - tok * a.group;
                     int l0, h0;
                     attend_range(s.first + tok, s.len, a.causal, a.window, l0, h0);
                     const bool none = l0 >= h0;
@@ -649,7 +641,7 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
             fence_async_smem();   // the ring's next copies come after these writes
             __syncthreads();
         }
-        cur.left -= take;
+        cur.left -= part.used;
         if (cur.left > 0) attend_next<kFewRows>(a, cur, s);
     }
     if (lost) kv_flag(a.status, KV_TIMEOUT);

@@ -34,6 +34,7 @@ namespace moeb200 {
 namespace {
 
 constexpr int kManyKeys = 128;               // keys of a unit
+constexpr int kManyCost = 2;                 // starting and ending a tile, in units
 constexpr uint32_t kManyPolls = 1u << 21;
 constexpr float kManyGrow = 8.f;             // log 2 of the growth that replaces the maximum
 
@@ -56,7 +57,7 @@ struct Many {
     static constexpr float SHIFT = KIND == KIND_BF16 ? 0.f : 7.f;
     static constexpr int o_stage = QB;
     static constexpr int o_bar = QB + NST * STAGEB;
-    static constexpr int o_fac = o_bar + 256;            // row factors
+    static constexpr int o_fac = o_bar + 512;            // row factors
     static constexpr int o_max = o_fac + M * 4;          // maxima and sums of half rows
     static constexpr int smem = o_max + (NQ == 1 ? 2048 : 0);
     static_assert(smem <= 232448, "shared memory of a CTA");
@@ -69,9 +70,11 @@ struct Many {
 struct ManyBars {
     uint64_t full[8], empty[8], s_full[2], p_full[2], pv_done[2], q_full[2];
     uint32_t tmem, lost;
-    uint32_t odd[4];   // keys of the unit whose values are not all finite
+    uint32_t products;     // units whose value products have been issued
+    uint32_t checked[2];   // partly attended units that each checking warp is done with
+    uint32_t odd[8][4];    // such units in turn: keys whose values are not all finite
 };
-static_assert(sizeof(ManyBars) <= 256, "");
+static_assert(sizeof(ManyBars) <= 512, "");
 
 // D (+)= A . B with A in tensor memory.
 __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
@@ -108,6 +111,26 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
+__device__ __forceinline__ void shfl_swap(uint4& keep, uint4& give, int mask, bool upper) {
+    // the lane with the bit clear gives `give` and takes the partner's `keep`
+    uint32_t* k = reinterpret_cast<uint32_t*>(&keep);
+    uint32_t* g = reinterpret_cast<uint32_t*>(&give);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t out = upper ? k[e] : g[e];
+        const uint32_t in = __shfl_xor_sync(0xffffffffu, out, mask);
+        if (upper) k[e] = in; else g[e] = in;
+    }
+}
+
+// y[i] of lane q of a quad becomes y[q] of lane i.
+__device__ __forceinline__ void quad_transpose(uint4 (&y)[4], int lane) {
+    shfl_swap(y[0], y[2], 2, lane & 2);
+    shfl_swap(y[1], y[3], 2, lane & 2);
+    shfl_swap(y[0], y[1], 1, lane & 1);
+    shfl_swap(y[2], y[3], 1, lane & 1);
+}
+
 template <int ID, int N>
 __device__ __forceinline__ void bar_sync() {
     asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory");
@@ -124,19 +147,21 @@ template <int DP, int KIND>
 struct Walk {
     AttendCursor cur;
     AttendSeq s;
-    int u0, take, units;
+    int u0, take;
+    int64_t used;
+    bool begins, ends;
     __device__ bool open(const AttendArgs& a) {   // the current segment's units
         if (cur.left <= 0) return false;
-        int lo, hi;
-        attend_units<Many<DP, KIND>::M, kManyKeys>(a, s, cur.tile, lo, hi);
-        units = hi - lo;
-        u0 = lo + cur.unit;
-        const int room = units - cur.unit;
-        take = room < cur.left ? room : (int)cur.left;
-        return true;
+        const AttendPart p = attend_part<Many<DP, KIND>::M, kManyKeys, kManyCost>(a, cur, s);
+        u0 = p.u0;
+        take = p.take;
+        used = p.used;
+        begins = p.begins;
+        ends = p.ends;
+        return take > 0;   // 0: the stretch ends before the tile's first unit
     }
     __device__ void next(const AttendArgs& a) {
-        cur.left -= take;
+        cur.left -= used;
         if (cur.left > 0) attend_next<Many<DP, KIND>::M>(a, cur, s);
     }
 };
@@ -178,9 +203,9 @@ struct QueryRows {
                 const int r = row0 + i0 + b * RPI + sub;
                 const bool ok = in_dim && r < valid;
                 const int rr = w.cur.tile * F::M + (ok ? r : 0);
-                const TQ* q = static_cast<const TQ*>(a.q) +
-                              (int64_t)(w.s.q0 + rr / a.group) * a.q_ts +
-                              (int64_t)(w.cur.kvh * a.group + rr % a.group) * a.q_hs +
+                const int tok = a.by_group.div(rr);
+                const TQ* q = static_cast<const TQ*>(a.q) + (int64_t)(w.s.q0 + tok) * a.q_ts +
+                              (int64_t)(w.cur.kvh * a.group + rr - tok * a.group) * a.q_hs +
                               (ok ? ch * 8 : 0);
                 if (copy) {
                     const int t = r & 127;
@@ -245,15 +270,16 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             mbar_init(&bars->q_full[i], F::NQ == 2 ? 4 : 8);
         }
         bars->lost = 0;
-        for (int i = 0; i < 4; ++i) bars->odd[i] = 0;
+        bars->products = bars->checked[0] = bars->checked[1] = 0;
+        for (int i = 0; i < 32; ++i) bars->odd[i / 4][i % 4] = 0;
         mbar_fence_init();
     }
     if (warp == 9) tmem_alloc(&bars->tmem, 512);
     const int ctas = gridDim.x;
     AttendWs ws(wsp, ctas);
     Walk<DP, KIND> w;
-    w.cur = attend_place<F::M, kManyKeys, F::THREADS>(
-        a, *reinterpret_cast<AttendScratch*>(sm), blockIdx.x, ctas, 1, a.status);
+    w.cur = attend_place<F::M, kManyKeys, kManyCost, F::THREADS>(
+        a, *reinterpret_cast<AttendScratch*>(sm), blockIdx.x, ctas, a.status);
     fence_async_smem();   // the scratch lies where the queries go
     tc_fence_before();
     __syncthreads();
@@ -267,6 +293,17 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             lost = true;
             *reinterpret_cast<volatile uint32_t*>(&bars->lost) = 1;
         }
+    };
+
+    // waits until a counter in shared memory reaches `upto`
+    auto spin = [&](const uint32_t* word, uint32_t upto) {
+        for (uint32_t i = 0; (int)(*reinterpret_cast<const volatile uint32_t*>(word) - upto) < 0; ++i)
+            if (i >= (lost ? 64u : kManyPolls * 8)) {
+                lost = true;
+                *reinterpret_cast<volatile uint32_t*>(&bars->lost) = 1;
+                break;
+            }
+        __threadfence_block();
     };
 
     if (warp < 8) {
@@ -286,6 +323,7 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         float* xmax = reinterpret_cast<float*>(sm + F::o_max);     // [2][2][128]
         AttendRecord rec{};
         uint32_t it = 0;       // units done by the CTA
+        uint32_t partial = 0;  // of them, those that not all rows attend
         int stage0 = 0;        // ring stages before this segment
 
         auto load_queries = [&](int n_valid) {
@@ -297,6 +335,67 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars->q_full[F::NQ == 2 ? wg : 0]);
         };
+        // The unit's odd values: all eight warps meet here.
+        auto poisoned = [&](volatile uint32_t* odd, int j, uint32_t t_s, int key0, int lo, int hi) {
+            const unsigned char* st[F::KPARTS];
+#pragma unroll
+            for (int h = 0; h < F::KPARTS; ++h)
+            {
+                const int n = stage0 + stage_v<F::NQ>(j, w.take) + h;
+                st[h] = sm + F::o_stage + (n % F::NST) * F::STAGEB;
+                await(&bars->full[n % F::NST], (uint32_t)(n / F::NST));
+            }
+            tc_fence_before();
+            bar_sync<2, 256>();   // with one tile, O takes both halves' probabilities
+            tc_fence_after();
+            if (j > 0) {
+                await(&bars->pv_done[F::NQ == 2 ? wg : 0], it - 1);
+                tc_fence_after();
+            }
+#pragma unroll 1
+            for (int k = 0; k < kManyKeys; ++k) {
+                if (!((odd[k >> 5] >> (k & 31)) & 1)) continue;
+                const uint32_t pw = tmem_ld1(t_s + k / 2);
+                tmem_wait_ld();
+                const uint16_t p16 = (uint16_t)(k & 1 ? pw >> 16 : pw);
+                const float p = KIND == KIND_BF16 ? __bfloat162float(__ushort_as_bfloat16(p16))
+                                                  : __half2float(__ushort_as_half(p16));
+                const bool at = key0 + k >= lo && key0 + k < hi;
+                const unsigned char* vt = st[k / F::VKEYS];
+                const int kr = k % F::VKEYS;
+#pragma unroll 1
+                for (int c = 0; c < F::OC / 16; ++c) {
+                    uint32_t o[16];
+                    tmem_ld16(t_o + c * 16, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int d = (F::NQ == 1 ? wg * 128 : 0) + c * 16 + i;
+                        const uint16_t v16 = *reinterpret_cast<const uint16_t*>(
+                            vt + (d >> 6) * (F::VKEYS * 128) + sw128_offset(kr, (d >> 3) & 7) +
+                            (d & 7) * 2);
+                        if (at && odd16<KIND>(v16))
+                            o[i] = __float_as_uint(
+                                __uint_as_float(o[i]) +
+                                p * (KIND == KIND_BF16 ? __bfloat162float(__ushort_as_bfloat16(v16))
+                                                       : __half2float(__ushort_as_half(v16))));
+                    }
+                    __syncwarp();
+                    tmem_st16(t_o + c * 16, o);
+                }
+                tmem_wait_st();
+            }
+            bar_sync<2, 256>();
+#pragma unroll
+            for (int h = 0; h < F::KPARTS; ++h)
+                for (int i = tid; i < F::STAGEB / 2; i += 256) {
+                    uint16_t* v = reinterpret_cast<uint16_t*>(const_cast<unsigned char*>(st[h])) + i;
+                    if (odd16<KIND>(*v)) *v = 0;
+                }
+            if (tid < 4) odd[tid] = 0;
+            fence_async_smem();
+            bar_sync<2, 256>();
+        };
         bool more = w.open(a);
         if (more) {
             load_queries(w.s.n * a.group - w.cur.tile * F::M);
@@ -305,16 +404,20 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         while (more) {
             const AttendSeq s = w.s;
             const AttendCursor cur = w.cur;
-            const int u0 = w.u0, take = w.take, units = w.units;
+            const int u0 = w.u0, take = w.take;
+            const bool begins = w.begins, ends = w.ends;
             const int rows = s.n * a.group - cur.tile * F::M;   // valid rows: the first `rows`
-            // keys that every row attends, and those of this thread's row
-            int all_lo, all_hi, lo = 0, hi = 0, x;
-            {
-                const int r0 = cur.tile * F::M, r1 = r0 + (rows < F::M ? rows : F::M) - 1;
-                attend_range(s.first + r0 / a.group, s.len, a.causal, a.window, x, all_hi);
-                attend_range(s.first + r1 / a.group, s.len, a.causal, a.window, all_lo, x);
-                if (trow < rows)
-                    attend_range(s.first + (r0 + trow) / a.group, s.len, a.causal, a.window, lo, hi);
+            // keys that all rows of the CTA attend, all rows of this warp, and this row
+            const AttendTile tile = attend_tile(a, s, cur.tile * F::M, F::M);
+            int lo = 0, hi = 0;
+            if (trow < rows)
+                attend_range(s.first + a.by_group.div(cur.tile * F::M + trow), s.len, a.causal,
+                             a.window, lo, hi);
+            int warp_lo = trow < rows ? lo : 0, warp_hi = trow < rows ? hi : 0x7fffffff;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                warp_lo = max(warp_lo, __shfl_xor_sync(0xffffffffu, warp_lo, o));
+                warp_hi = min(warp_hi, __shfl_xor_sync(0xffffffffu, warp_hi, o));
             }
             float m = -INFINITY, l = 0.f;
             float mul = 0.f;
@@ -342,12 +445,18 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                 for (int c = 0; c < F::NC / 32; ++c) tmem_ld32(t_s + col0 + c * 32, sv + c * 32);
                 tmem_wait_ld();
                 const int key0 = (u0 + j) * kManyKeys;
-                const bool whole = key0 >= all_lo && key0 + kManyKeys <= all_hi;
-                if (!whole) {
+                const bool whole = key0 >= tile.all_lo && key0 + kManyKeys <= tile.all_hi;
+                if (key0 < warp_lo || key0 + kManyKeys > warp_hi) {
                     const int from = lo - key0 - col0, to = hi - key0 - col0;
 #pragma unroll
-                    for (int i = 0; i < F::NC; ++i)
-                        if (i < from || i >= to) sv[i] = 0xff800000u;   // -infinity
+                    for (int c = 0; c < F::NC / 32; ++c) {   // bits of the attended columns
+                        const int f = min(max(from - c * 32, 0), 32), t = min(max(to - c * 32, 0), 32);
+                        const uint32_t keep =
+                            (uint32_t)(((1ull << t) - 1) & ~((1ull << f) - 1));
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (!(keep >> i & 1)) sv[c * 32 + i] = 0xff800000u;   // -infinity
+                    }
                 }
                 float t0 = __uint_as_float(sv[0]), t1 = __uint_as_float(sv[1]);
                 float t2 = __uint_as_float(sv[2]), t3 = __uint_as_float(sv[3]);
@@ -408,86 +517,21 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                 tmem_wait_st();
                 if (!whole) {
                     // A key that only some rows attend, or none: 0 * NaN would
-                    // reach the others.  Values that are not finite are added to
-                    // the rows that attend them one by one and leave the stage.
-                    unsigned char* st[F::KPARTS];
-                    bool odd = false;
-#pragma unroll
-                    for (int h = 0; h < F::KPARTS; ++h) {
-                        const int n = stage0 + stage_v<F::NQ>(j, take) + h;
-                        st[h] = sm + F::o_stage + (n % F::NST) * F::STAGEB;
-                        await(&bars->full[n % F::NST], (uint32_t)(n / F::NST));
-                        for (int i = tid; i < F::STAGEB / 16; i += 256) {
-                            const uint4 v = reinterpret_cast<const uint4*>(st[h])[i];
-                            if (odd16<KIND>(v.x) || odd16<KIND>(v.y) || odd16<KIND>(v.z) ||
-                                odd16<KIND>(v.w)) {
-                                odd = true;
-                                const int k = h * F::VKEYS + (i >> 3) % F::VKEYS;
-                                atomicOr(&bars->odd[k >> 5], 1u << (k & 31));
-                            }
-                        }
-                    }
-                    tc_fence_before();
-                    int any;
-                    asm volatile(
-                        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
-                        "bar.red.or.pred q, 2, 256, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
-                        : "=r"(any)
-                        : "r"((int)odd)
-                        : "memory");
-                    if (any) {
-                        tc_fence_after();
-                        if (j > 0) {
-                            await(&bars->pv_done[F::NQ == 2 ? wg : 0], it - 1);
-                            tc_fence_after();
-                        }
-#pragma unroll 1
-                        for (int k = 0; k < kManyKeys; ++k) {
-                            if (!((bars->odd[k >> 5] >> (k & 31)) & 1)) continue;
-                            const uint32_t pw = tmem_ld1(t_s + k / 2);
-                            tmem_wait_ld();
-                            const uint16_t ph16 = (uint16_t)(k & 1 ? pw >> 16 : pw);
-                            const float p = KIND == KIND_BF16
-                                                ? __bfloat162float(__ushort_as_bfloat16(ph16))
-                                                : __half2float(__ushort_as_half(ph16));
-                            const bool at = key0 + k >= lo && key0 + k < hi;
-                            const unsigned char* vt = st[k / F::VKEYS];
-                            const int kr = k % F::VKEYS;
-#pragma unroll 1
-                            for (int c = 0; c < F::OC / 16; ++c) {
-                                uint32_t o[16];
-                                tmem_ld16(t_o + c * 16, o);
-                                tmem_wait_ld();
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) {
-                                    const int d = (F::NQ == 1 ? wg * 128 : 0) + c * 16 + i;
-                                    const uint16_t v16 = *reinterpret_cast<const uint16_t*>(
-                                        vt + (d >> 6) * (F::VKEYS * 128) +
-                                        sw128_offset(kr, (d >> 3) & 7) + (d & 7) * 2);
-                                    if (at && odd16<KIND>(v16))
-                                        o[i] = __float_as_uint(
-                                            __uint_as_float(o[i]) +
-                                            p * (KIND == KIND_BF16
-                                                     ? __bfloat162float(__ushort_as_bfloat16(v16))
-                                                     : __half2float(__ushort_as_half(v16))));
-                                }
-                                __syncwarp();
-                                tmem_st16(t_o + c * 16, o);
-                            }
-                            tmem_wait_st();
-                        }
-                        bar_sync<2, 256>();
-#pragma unroll
-                        for (int h = 0; h < F::KPARTS; ++h)
-                            for (int i = tid; i < F::STAGEB / 2; i += 256) {
-                                uint16_t* v = reinterpret_cast<uint16_t*>(st[h]) + i;
-                                if (odd16<KIND>(*v)) *v = 0;
-                            }
-                        if (tid < 4) bars->odd[tid] = 0;
-                        fence_async_smem();
-                        bar_sync<2, 256>();
-                    }
+                    // reach the others.  Two warps look through the values of
+                    // such a unit; those that are not finite are added to the
+                    // rows that attend them one by one and leave the stage.
+                    ++partial;
+                    spin(&bars->checked[0], partial);
+                    spin(&bars->checked[1], partial);
+                    volatile uint32_t* odd = bars->odd[partial & 7];
+                    if (odd[0] | odd[1] | odd[2] | odd[3])
+                        poisoned(odd, j, t_s, key0, lo, hi);
                 }
+                // One tile: S(j) comes before the value product of j - 1, so a
+                // fast warp could be two phases of pv_done ahead and mistake
+                // the last one it saw for the one it needs; products run in
+                // order, so waiting here costs nothing.
+                if (F::NQ == 1 && j > 0) await(&bars->pv_done[0], it - 1);
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars->p_full[buf]);
@@ -505,8 +549,8 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                 l = xl[row] + xl[128 + row];
                 bar_sync<1, 256>();
             }
-            const bool full = cur.unit == 0 && take == units;
-            const int which = cur.unit == 0;   // 1: tail slot, 0: head slot
+            const bool full = begins && ends;
+            const int which = begins;   // 1: tail slot, 0: head slot
             if (!full) {
                 if (which) {
                     rec.tail = 1;
@@ -514,7 +558,7 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                     rec.tile = cur.tile;
                     rec.kvh = cur.kvh;
                 } else {
-                    rec.head = cur.unit + take == units ? 2 : 1;
+                    rec.head = ends ? 2 : 1;
                 }
             }
             m -= F::SHIFT;
@@ -522,9 +566,21 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             const bool none = lo >= hi;
             const float inv = none ? 0.f : 1.f / l;
             const int rr = cur.tile * F::M + (valid ? trow : 0);
-            const int tok = s.q0 + rr / a.group, h = cur.kvh * a.group + rr % a.group;
+            const int tk = a.by_group.div(rr);
+            const int tok = s.q0 + tk, h = cur.kvh * a.group + rr - tk * a.group;
             float* slot = ws.slot(blockIdx.x, which, F::M, DP);
+            TQ* orow = static_cast<TQ*>(a.out) + (int64_t)tok * a.o_ts + (int64_t)h * a.o_hs;
             const int d0 = F::NQ == 1 ? wg * 128 : 0;
+            // rows of the lanes of this quad (lane q of four stores 16 bytes of each)
+            TQ* qrow[4];
+            bool qvalid[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int from = (lane & ~3) + i;
+                qrow[i] = reinterpret_cast<TQ*>(
+                    __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(orow), from));
+                qvalid[i] = __shfl_sync(0xffffffffu, (int)valid, from);
+            }
 #pragma unroll 1
             for (int c = 0; c < F::OC / 32; ++c) {
                 uint32_t o[32];
@@ -532,26 +588,33 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                 tmem_ld32(t_o + c * 32, o);
                 tmem_wait_ld();
                 const int d = d0 + c * 32;
-                if (!valid) {
-                } else if (!full) {
-                    float* dst = slot + (size_t)trow * DP + d;
+                if (!full) {
+                    if (valid) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        reinterpret_cast<uint4*>(dst)[i] =
-                            make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-                } else if (d < a.c.dim) {
-                    TQ* dst = static_cast<TQ*>(a.out) + (int64_t)tok * a.o_ts + (int64_t)h * a.o_hs + d;
+                        for (int i = 0; i < 8; ++i)
+                            *reinterpret_cast<uint4*>(slot + ((size_t)(d / 4 + i) * F::M + trow) * 4) =
+                                make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    }
+                } else {
                     constexpr int OK = std::is_same<TQ, __nv_bfloat16>::value ? KIND_BF16 : KIND_F16;
+                    uint4 y[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        uint32_t y[4];
+                        uint32_t* yw = reinterpret_cast<uint32_t*>(&y[i]);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float v0 = __uint_as_float(o[8 * i + 2 * e]) * inv;
-                            const float v1 = __uint_as_float(o[8 * i + 2 * e + 1]) * inv;
-                            y[e] = none ? 0u : pack16<OK>(v0, v1);
-                        }
-                        reinterpret_cast<uint4*>(dst)[i] = make_uint4(y[0], y[1], y[2], y[3]);
+                        for (int e = 0; e < 4; ++e)
+                            yw[e] = none ? 0u
+                                         : pack16<OK>(__uint_as_float(o[8 * i + 2 * e]) * inv,
+                                                      __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
+                    }
+                    // 4 x 4 transposition within the quad, so that a store
+                    // covers 64 bytes of a row: swap across lane bit 1, then 0
+                    quad_transpose(y, lane);
+                    if (d + (lane & 3) * 8 < a.c.dim) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (qvalid[i])
+                                *reinterpret_cast<uint4*>(qrow[i] + d + (lane & 3) * 8) = y[i];
                     }
                 }
             }
@@ -666,13 +729,55 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                         }
                         umma_commit(&bars->pv_done[0]);
                     }
-                    ++it;
+                    *reinterpret_cast<volatile uint32_t*>(&bars->products) = ++it;
                 }
                 stage0 += 2 * F::KPARTS * take;
                 ++seg;
                 w.next(a);
             }
             // every product has been waited for by the softmax warps
+        } else if (warp >= 10) {
+            // --------------------------- values of partly attended units
+            // Units are skipped, so a stage's barrier may be phases behind: a unit
+            // is looked at once the value products of those before it were
+            // issued (their stages, the previous uses of its own, were full),
+            // and its own cannot be issued before it has been.
+            int stage0 = 0;
+            uint32_t partial = 0, it = 0;
+            while (w.open(a)) {
+                const AttendTile tile = attend_tile(a, w.s, w.cur.tile * F::M, F::M);
+                for (int j = 0; j < w.take; ++j, ++it) {
+                    const int key0 = (w.u0 + j) * kManyKeys;
+                    if (key0 >= tile.all_lo && key0 + kManyKeys <= tile.all_hi) continue;
+                    ++partial;
+                    spin(&bars->products, it);
+                    uint32_t* odd = bars->odd[partial & 7];
+                    for (int h = 0; h < F::KPARTS; ++h) {
+                        const int n = stage0 + stage_v<F::NQ>(j, w.take) + h;
+                        const uint4* st = reinterpret_cast<const uint4*>(
+                            sm + F::o_stage + (n % F::NST) * F::STAGEB);
+                        await(&bars->full[n % F::NST], (uint32_t)(n / F::NST));
+#pragma unroll 4
+                        for (int i = tid - 320; i < F::STAGEB / 16; i += 64) {
+                            const uint4 v = st[i];
+                            // an exponent of ones carries into the sign bit
+                            constexpr uint32_t e = KIND == KIND_BF16 ? 0x7f807f80u : 0x7c007c00u;
+                            constexpr uint32_t one = KIND == KIND_BF16 ? 0x00800080u : 0x04000400u;
+                            const uint32_t x = ((v.x & e) + one) | ((v.y & e) + one) |
+                                               ((v.z & e) + one) | ((v.w & e) + one);
+                            if (x & 0x80008000u) {
+                                const int k = h * F::VKEYS + (i >> 3) % F::VKEYS;
+                                atomicOr(&odd[k >> 5], 1u << (k & 31));
+                            }
+                        }
+                    }
+                    __threadfence_block();
+                    __syncwarp();
+                    if (lane == 0) *reinterpret_cast<volatile uint32_t*>(&bars->checked[warp - 10]) = partial;
+                }
+                stage0 += 2 * F::KPARTS * w.take;
+                w.next(a);
+            }
         } else if (!F::Q8 && warp == 8) {
             // --------------------------------------------------------- copies
             int stage0 = 0;
@@ -738,6 +843,17 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             const int total = 2 * F::KPARTS * take;
             uint4 code[2][CH];
             uint32_t scl[2][(CH + 1) / 2];
+            // page ids of a unit's pieces, one per lane; one unit's (with two
+            // stages per unit two units') are kept
+            const int piece_shift = a.c.page_shift < 7 ? a.c.page_shift : 7;
+            auto page_ids = [&](int j) {
+                const int key = (w.u0 + j) * kManyKeys + (lane << piece_shift);
+                if (j >= take || lane >= (kManyKeys >> piece_shift) || key >= w.s.len) return -1;
+                return kv_page(a.b, a.c, w.cur.seq, key >> a.c.page_shift, a.status);
+            };
+            int ids[F::KPARTS];
+#pragma unroll
+            for (int h = 0; h < F::KPARTS; ++h) ids[h] = page_ids(h);
             // loads the codes of the segment's n-th stage
             auto load = [&](int n, uint4 (&cd)[CH], uint32_t (&sc)[(CH + 1) / 2], bool& is_v) {
                 if (n >= total) return;
@@ -755,23 +871,29 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                 const int key0 = (w.u0 + j) * kManyKeys + (is_v ? h * F::VKEYS : 0);
                 const int x0 = is_v ? 0 : h * 128;
                 const int per = is_v ? VC : KC;
+                const int pid = F::KPARTS == 2 && (j & 1) ? ids[F::KPARTS - 1] : ids[0];
+                const int8_t* codes = static_cast<const int8_t*>(is_v ? a.c.v : a.c.k);
+                const __half* scales = is_v ? a.c.vs : a.c.ks;
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
                     const int idx = c * 128 + t;
                     const int key = key0 + idx / per, d = x0 + idx % per * 16;
+                    const int page = __shfl_sync(0xffffffffu, pid,
+                                                 (key & (kManyKeys - 1)) >> piece_shift);
+                    const bool ok = page >= 0 && key < w.s.len && d < a.c.dim;
+                    const int64_t r = (((int64_t)page * a.c.heads + w.cur.kvh) << a.c.page_shift) +
+                                      (key & (a.c.page_size - 1));
                     cd[c] = make_uint4(0, 0, 0, 0);
                     uint32_t sc16 = 0;
-                    if (key < w.s.len && d < a.c.dim) {
-                        const int page = kv_page(a.b, a.c, w.cur.seq, key >> a.c.page_shift, a.status);
-                        if (page >= 0) {
-                            const int64_t r = (((int64_t)page * a.c.heads + w.cur.kvh) << a.c.page_shift) +
-                                              (key & (a.c.page_size - 1));
-                            cd[c] = __ldg(reinterpret_cast<const uint4*>(
-                                static_cast<const int8_t*>(is_v ? a.c.v : a.c.k) + r * a.c.dim + d));
-                            sc16 = __half_as_ushort((is_v ? a.c.vs : a.c.ks)[r * nb + (d >> 5)]);
-                        }
+                    if (ok) {
+                        cd[c] = __ldg(reinterpret_cast<const uint4*>(codes + r * a.c.dim + d));
+                        sc16 = __ldg(reinterpret_cast<const unsigned short*>(scales) + r * nb + (d >> 5));
                     }
                     if (c & 1) sc[c / 2] |= sc16 << 16; else sc[c / 2] = sc16;
+                }
+                if (is_v && h == F::KPARTS - 1) {
+                    const int next = page_ids(j + F::KPARTS);
+                    if (F::KPARTS == 2 && (j & 1)) ids[F::KPARTS - 1] = next; else ids[0] = next;
                 }
             };
             auto store = [&](int n, uint4 (&cd)[CH], uint32_t (&sc)[(CH + 1) / 2], bool is_v) {

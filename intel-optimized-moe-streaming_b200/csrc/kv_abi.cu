@@ -148,6 +148,7 @@ int moe_b200_attend(const moe_b200_kv_cache* cache, const moe_b200_kv_batch* bat
     a.type = type;
     a.q_heads = q_heads;
     a.group = q_heads / a.c.heads;
+    a.by_group = FastDiv(a.group);
     a.scale = scale;
     a.causal = causal;
     a.window = window;
