@@ -309,7 +309,7 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
     if (warp < 8) {
         // ------------------------------------------------------------ softmax
         if constexpr (F::Q8)
-            asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
         else
             asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int wg = warp >> 2, quarter = warp & 3;
@@ -642,28 +642,33 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             // ------------------------------------------------------- products
             uint32_t it = 0, seg = 0;
             int stage0 = 0;
-            auto stage_at = [&](int n) { return smem_u32(sm + F::o_stage + (n % F::NST) * F::STAGEB); };
             auto wait_stage = [&](int n) {
                 await(&bars->full[n % F::NST], (uint32_t)(n / F::NST));
             };
             auto free_stage = [&](int n) { umma_commit(&bars->empty[n % F::NST]); };
+            // A descriptor's address field counts 16 bytes and no operand ends
+            // beyond it, so the steps are additions to its low word.
+            const uint64_t q_desc = umma_desc_sw128(smem_u32(sm));
+            const uint64_t k_desc = umma_desc_sw128(smem_u32(sm + F::o_stage));
+            const uint64_t v_desc = umma_desc_nmajor(smem_u32(sm + F::o_stage), F::VKEYS * 128);
+            auto slot_of = [&](int n) { return (uint64_t)((n % F::NST) * (F::STAGEB >> 4)); };
             // S = Q K^T of one query tile with one stage of keys
-            auto score = [&](int tile, int part, uint32_t d, uint32_t kst) {
-                const uint32_t q = smem_u32(sm) + (tile * F::SLABS + part * F::KSLABS) * 16384;
+            auto score = [&](int tile, int part, uint32_t d, int n) {
+                const uint64_t q = q_desc + (tile * F::SLABS + part * F::KSLABS) * 1024;
+                const uint64_t k0 = k_desc + slot_of(n);
 #pragma unroll
                 for (int sl = 0; sl < F::KSLABS; ++sl)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        umma_f16(d, umma_desc_sw128(q + sl * 16384 + k * 32),
-                                 umma_desc_sw128(kst + sl * 16384 + k * 32), F::IDESC_S,
+                        umma_f16(d, q + (sl * 1024 + k * 2), k0 + (sl * 1024 + k * 2), F::IDESC_S,
                                  part > 0 || sl > 0 || k > 0);
             };
             // O += P V with one stage of values
-            auto value = [&](uint32_t d, uint32_t p, uint32_t vst) {
+            auto value = [&](uint32_t d, uint32_t p, int n) {
+                const uint64_t v0 = v_desc + slot_of(n);
 #pragma unroll
                 for (int k = 0; k < F::VKEYS / 16; ++k)
-                    umma_f16_ts(d, p + k * 8, umma_desc_nmajor(vst + k * 2048, F::VKEYS * 128),
-                                F::IDESC_O);
+                    umma_f16_ts(d, p + k * 8, v0 + k * 128, F::IDESC_O);
             };
             while (w.open(a)) {
                 const int take = w.take;
@@ -677,7 +682,7 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                         const int n = stage0 + stage_k<F::NQ>(j) + h;
                         wait_stage(n);
                         tc_fence_after();
-                        score(0, h, tmem + b * 128, stage_at(n));
+                        score(0, h, tmem + b * 128, n);
                         free_stage(n);
                     }
                     umma_commit(&bars->s_full[b]);
@@ -687,7 +692,7 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                     wait_stage(n);
                     tc_fence_after();
                     for (int t = 0; t < 2; ++t) {
-                        score(t, 0, tmem + t * 128, stage_at(n));
+                        score(t, 0, tmem + t * 128, n);
                         umma_commit(&bars->s_full[t]);
                     }
                     free_stage(n);
@@ -701,7 +706,7 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                         for (int t = 0; t < 2; ++t) {
                             await(&bars->p_full[t], it);
                             tc_fence_after();
-                            value(tmem + 256 + t * DP, tmem + t * 128, stage_at(nv));
+                            value(tmem + 256 + t * DP, tmem + t * 128, nv);
                             umma_commit(&bars->pv_done[t]);
                             if (t == 1) free_stage(nv);
                             if (j + 1 < take) {
@@ -709,7 +714,7 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                                     wait_stage(nk);
                                     tc_fence_after();
                                 }
-                                score(t, 0, tmem + t * 128, stage_at(nk));
+                                score(t, 0, tmem + t * 128, nk);
                                 umma_commit(&bars->s_full[t]);
                                 if (t == 1) free_stage(nk);
                             }
@@ -724,7 +729,7 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                             const int n = stage0 + stage_v<1>(j, take) + h;
                             wait_stage(n);
                             tc_fence_after();
-                            value(tmem + 256, tmem + b * 128 + h * (F::VKEYS / 2), stage_at(n));
+                            value(tmem + 256, tmem + b * 128 + h * (F::VKEYS / 2), n);
                             free_stage(n);
                         }
                         umma_commit(&bars->pv_done[0]);
@@ -832,7 +837,7 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         }
     } else if constexpr (F::Q8) {
         // ------------------------------------------------------ Q8_0 decoding
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         const int t = tid - 384, nb = a.c.dim >> 5;
         constexpr int CH = F::STAGEB / 32 / 128;   // 16-code chunks of a thread and stage
         constexpr int KC = F::KSLABS * 4;          // chunks of a row in a stage of keys
@@ -841,8 +846,6 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         while (w.open(a)) {
             const int take = w.take;
             const int total = 2 * F::KPARTS * take;
-            uint4 code[2][CH];
-            uint32_t scl[2][(CH + 1) / 2];
             // page ids of a unit's pieces, one per lane; one unit's (with two
             // stages per unit two units') are kept
             const int piece_shift = a.c.page_shift < 7 ? a.c.page_shift : 7;
@@ -854,84 +857,81 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             int ids[F::KPARTS];
 #pragma unroll
             for (int h = 0; h < F::KPARTS; ++h) ids[h] = page_ids(h);
-            // loads the codes of the segment's n-th stage
-            auto load = [&](int n, uint4 (&cd)[CH], uint32_t (&sc)[(CH + 1) / 2], bool& is_v) {
-                if (n >= total) return;
+            // the segment's n-th stage: unit j, part h, keys or values
+            struct Stage {
                 int j, h;
-                if (F::NQ == 2) {
-                    j = n >> 1;
-                    is_v = n & 1;
-                    h = 0;
-                } else {
-                    const int g = n >> 1;   // K0 | K1 V0 | K2 V1 | ... | V(take-1)
-                    h = n & 1;
-                    is_v = g > 0 && (!(g & 1) || g == 2 * take - 1);
-                    j = g == 0 ? 0 : g == 2 * take - 1 ? take - 1 : is_v ? g / 2 - 1 : (g + 1) / 2;
-                }
-                const int key0 = (w.u0 + j) * kManyKeys + (is_v ? h * F::VKEYS : 0);
-                const int x0 = is_v ? 0 : h * 128;
-                const int per = is_v ? VC : KC;
-                const int pid = F::KPARTS == 2 && (j & 1) ? ids[F::KPARTS - 1] : ids[0];
-                const int8_t* codes = static_cast<const int8_t*>(is_v ? a.c.v : a.c.k);
-                const __half* scales = is_v ? a.c.vs : a.c.ks;
-#pragma unroll
-                for (int c = 0; c < CH; ++c) {
-                    const int idx = c * 128 + t;
-                    const int key = key0 + idx / per, d = x0 + idx % per * 16;
-                    const int page = __shfl_sync(0xffffffffu, pid,
-                                                 (key & (kManyKeys - 1)) >> piece_shift);
-                    const bool ok = page >= 0 && key < w.s.len && d < a.c.dim;
-                    const int64_t r = (((int64_t)page * a.c.heads + w.cur.kvh) << a.c.page_shift) +
-                                      (key & (a.c.page_size - 1));
-                    cd[c] = make_uint4(0, 0, 0, 0);
-                    uint32_t sc16 = 0;
-                    if (ok) {
-                        cd[c] = __ldg(reinterpret_cast<const uint4*>(codes + r * a.c.dim + d));
-                        sc16 = __ldg(reinterpret_cast<const unsigned short*>(scales) + r * nb + (d >> 5));
-                    }
-                    if (c & 1) sc[c / 2] |= sc16 << 16; else sc[c / 2] = sc16;
-                }
-                if (is_v && h == F::KPARTS - 1) {
-                    const int next = page_ids(j + F::KPARTS);
-                    if (F::KPARTS == 2 && (j & 1)) ids[F::KPARTS - 1] = next; else ids[0] = next;
+                bool v;
+            };
+            auto stage_of = [&](int n) {
+                if (F::NQ == 2) return Stage{n >> 1, 0, (n & 1) != 0};
+                const int g = n >> 1;   // K0 | K1 V0 | K2 V1 | ... | V(take-1)
+                const bool last = g == 2 * take - 1;
+                const bool v = last || (g > 0 && !(g & 1));
+                return Stage{last ? take - 1 : v ? g / 2 - 1 : (g + 1) / 2, n & 1, v};
+            };
+            uint4 code[CH];
+            uint32_t scl[CH];
+            auto load = [&](const Stage& g, int pid, int c) {
+                const int per = KC == VC ? KC : g.v ? VC : KC;
+                const int key = (w.u0 + g.j) * kManyKeys + (g.v ? g.h * F::VKEYS : 0) + (c * 128 + t) / per;
+                const int d = (g.v ? 0 : g.h * 128) + t % per * 16;
+                const int page = __shfl_sync(0xffffffffu, pid, (key & (kManyKeys - 1)) >> piece_shift);
+                const bool ok = page >= 0 && key < w.s.len && d < a.c.dim;
+                const int64_t r = (((int64_t)page * a.c.heads + w.cur.kvh) << a.c.page_shift) +
+                                  (key & (a.c.page_size - 1));
+                code[c] = make_uint4(0, 0, 0, 0);
+                scl[c] = 0;
+                if (ok) {
+                    code[c] = __ldg(reinterpret_cast<const uint4*>(
+                        static_cast<const int8_t*>(g.v ? a.c.v : a.c.k) + r * a.c.dim + d));
+                    scl[c] = __ldg(reinterpret_cast<const unsigned short*>(g.v ? a.c.vs : a.c.ks) +
+                                   r * nb + (d >> 5));
                 }
             };
-            auto store = [&](int n, uint4 (&cd)[CH], uint32_t (&sc)[(CH + 1) / 2], bool is_v) {
+            auto ids_of = [&](const Stage& g) {
+                return F::KPARTS == 2 && (g.j & 1) ? ids[F::KPARTS - 1] : ids[0];
+            };
+            {
+                const Stage g = stage_of(0);
+                const int pid = ids_of(g);
+#pragma unroll
+                for (int c = 0; c < CH; ++c) load(g, pid, c);
+            }
+            for (int n = 0; n < total; ++n) {
+                const Stage g = stage_of(n);
+                if (g.v && g.h == F::KPARTS - 1) {   // this unit's page ids have been used
+                    const int next = page_ids(g.j + F::KPARTS);
+                    if (F::KPARTS == 2 && (g.j & 1)) ids[F::KPARTS - 1] = next; else ids[0] = next;
+                }
+                const Stage gn = stage_of(n + 1 < total ? n + 1 : n);
+                const int pid = ids_of(gn);
                 const int slot = (stage0 + n) % F::NST;
                 if (stage0 + n >= F::NST) await(&bars->empty[slot], (uint32_t)((stage0 + n) / F::NST) + 1);
-                unsigned char* st = sm + F::o_stage + slot * F::STAGEB;
-                const int per = is_v ? VC : KC, keys = is_v ? F::VKEYS : kManyKeys;
+                const int per = KC == VC ? KC : g.v ? VC : KC, keys = g.v ? F::VKEYS : kManyKeys;
+                const int q = t % per, c0 = (q & 3) * 2;
+                // lanes of the odd slabs store their second half first, so
+                // that eight lanes cover eight different 16-byte columns
+                const int first = (q >> 2) & 1;
+                unsigned char* slab = sm + F::o_stage + slot * F::STAGEB + (q >> 2) * keys * 128;
+                unsigned char* at0 = slab + sw128_offset(t / per, c0 + first);
+                unsigned char* at1 = slab + sw128_offset(t / per, c0 + 1 - first);
 #pragma unroll
-                for (int c = 0; c < CH; ++c) {
-                    const int idx = c * 128 + t;
-                    const int r = idx / per, q = idx % per;
-                    const __half2 d = __half2half2(
-                        __ushort_as_half((unsigned short)(c & 1 ? sc[c / 2] >> 16 : sc[c / 2])));
+                for (int c = 0; c < CH; ++c) {   // 128 / per rows on: whole 8-row atoms
+                    const __half2 d = __half2half2(__ushort_as_half((unsigned short)scl[c]));
                     uint32_t x[8];
-                    const uint32_t* cw = reinterpret_cast<const uint32_t*>(&cd[c]);
+                    const uint32_t* cw = reinterpret_cast<const uint32_t*>(&code[c]);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) codes4(cw[i], d, x[2 * i], x[2 * i + 1]);
-                    unsigned char* slab = st + (q >> 2) * keys * 128;
-                    const int c0 = (q & 3) * 2;
-                    // lanes of the odd slabs store their second half first, so
-                    // that eight lanes cover eight different 16-byte columns
-                    const int first = (q >> 2) & 1;
                     const uint4 lo4 = make_uint4(x[0], x[1], x[2], x[3]);
                     const uint4 hi4 = make_uint4(x[4], x[5], x[6], x[7]);
-                    *reinterpret_cast<uint4*>(slab + sw128_offset(r, c0 + first)) = first ? hi4 : lo4;
-                    *reinterpret_cast<uint4*>(slab + sw128_offset(r, c0 + 1 - first)) = first ? lo4 : hi4;
+                    const int step = c * (128 / per) * 128;
+                    *reinterpret_cast<uint4*>(at0 + step) = first ? hi4 : lo4;
+                    *reinterpret_cast<uint4*>(at1 + step) = first ? lo4 : hi4;
+                    if (n + 1 < total) load(gn, pid, c);   // this chunk of the next stage
                 }
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars->full[slot]);
-            };
-            bool v0 = false, v1 = false;
-            load(0, code[0], scl[0], v0);
-            for (int n = 0; n < total; n += 2) {
-                load(n + 1, code[1], scl[1], v1);
-                store(n, code[0], scl[0], v0);
-                load(n + 2, code[0], scl[0], v0);
-                if (n + 1 < total) store(n + 1, code[1], scl[1], v1);
             }
             stage0 += total;
             w.next(a);
