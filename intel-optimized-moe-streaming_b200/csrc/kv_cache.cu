@@ -69,10 +69,16 @@ __device__ __forceinline__ __half quantise16(const float (&x)[16], Vec16<int8_t>
         return __ushort_as_half(0x7fff);
     }
     const float step = fminf(__half2float(__float2half_ru(__fdiv_rn(top, 127.f))), kKvScaleMax);
+    const float inv = step > 0.f ? __frcp_rn(step) : 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        const float c = step > 0.f ? rintf(__fdiv_rn(x[i], step)) : 0.f;
-        q.v[i] = (int8_t)__float2int_rn(fminf(fmaxf(c, -127.f), 127.f));
+        // x / step, correctly rounded: one step of Newton's correction to
+        // x * (1 / step), whose remainder the fused multiply-add gives exactly
+        const float y = x[i] * inv;
+        const float c = fmaf(fmaf(-y, step, x[i]), inv, y);
+        // nearest integer, ties to even: 1.5 * 2^23 leaves no fraction bits
+        const float n = fminf(fmaxf(c, -127.f), 127.f) + 12582912.f;
+        q.v[i] = (int8_t)__float_as_int(n);
     }
     return __float2half_rn(step);
 }

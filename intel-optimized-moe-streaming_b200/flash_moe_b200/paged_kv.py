@@ -27,6 +27,7 @@ from . import _lib
 from .formats import BF16, F16, F32, Q8_0
 
 TYPE_IDS = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+_BYTES = {torch.float32: 4, torch.float16: 2, torch.bfloat16: 2}
 BLOCK_VALUES = 32   # values that share one scale of a Q8_0 cache
 
 
@@ -52,6 +53,7 @@ class KVBatch:
             raise ValueError("KVBatch page table rows must not overlap")
         self.q_start, self.kv_lens, self.page_table = q_start, kv_lens, page_table
         self.device = q_start.device
+        self.index = q_start.get_device()
         self.sequences = n
         self.max_pages = page_table.shape[1]
         self._structs: dict[int, _lib.KVBatchStruct] = {}
@@ -68,24 +70,13 @@ class KVBatch:
         return s
 
 
-def _strides(t: torch.Tensor) -> tuple[int, int]:
-    """Token and head strides of `t` [tokens, heads, dim]; 0 along an axis of
-    one entry, whose stride torch leaves arbitrary."""
-    ts, hs, _ = t.stride()
-    return (ts if t.shape[0] > 1 else 0), (hs if t.shape[1] > 1 else 0)
+def _raw_stream(index: int) -> int:
+    """Handle of torch's current stream of a device."""
+    return torch.cuda.current_stream(index).cuda_stream
 
 
-def _aligned(t: torch.Tensor) -> bool:
-    """Whether `t` [tokens, heads, dim] has contiguous, 16-byte aligned head
-    rows."""
-    step = 16 // t.element_size()
-    ts, hs = _strides(t)
-    return not (t.stride(2) != 1 or ts % step or hs % step or t.data_ptr() % 16)
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """`t`, or a contiguous copy when its head rows are not aligned."""
-    return t if _aligned(t) else t.clone(memory_format=torch.contiguous_format)
+# the same without building a Stream object (about 2 us of a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 
 
 class PagedKVCache:
@@ -134,6 +125,8 @@ class PagedKVCache:
                                           ptr(v), ptr(k_scales), ptr(v_scales))
         self._ref = C.byref(self._struct)
         self._ws_bytes: dict[tuple, int] = {}
+        self._index = k.get_device()
+        self._q_dtypes = ((torch.float16, torch.bfloat16) if self.type == Q8_0 else (k.dtype,))
 
     @classmethod
     def empty(cls, num_pages: int, page_size: int, kv_heads: int, head_dim: int, type_id: int,
@@ -157,27 +150,42 @@ class PagedKVCache:
         """A context that makes `stream` current (and the cache's device), or
         None when the call can run as it is."""
         if stream is None:
-            if torch.cuda.current_device() == self.device.index:
+            if torch.cuda.current_device() == self._index:
                 return None
             return torch.cuda.device(self.device)
         if stream.device != self.device:
             raise ValueError("the stream must belong to the cache's device")
         return torch.cuda.stream(stream)
 
-    def _check_rows(self, t, heads, dtypes, what):
-        if (t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.head_dim
-                or t.dtype not in dtypes or t.device != self.device):
+    def _rows(self, t, heads, dtypes, what, output=False):
+        """Address and token / head strides of `t` [tokens, heads, head_dim]
+        with contiguous, 16-byte aligned head rows, and the tensor that holds
+        them: `t`, or a contiguous copy of an input that is not aligned.  The
+        stride along an axis of one entry, which torch leaves arbitrary, is
+        0."""
+        shape = t.shape
+        if (len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim
+                or t.dtype not in dtypes or t.get_device() != self._index):
             raise ValueError(f"{what} must be a [tokens, {heads}, {self.head_dim}] CUDA tensor on "
                              f"the cache's device, dtype one of {[str(d) for d in dtypes]}")
-
-    def _check_output(self, t, what):
-        if not _aligned(t):
-            raise ValueError(f"{what} must have contiguous, 16-byte aligned head rows")
+        ts, hs, ds = t.stride()
+        if shape[0] <= 1:
+            ts = 0
+        if heads == 1:
+            hs = 0
+        ptr = t.data_ptr()
+        if ds != 1 or (ptr | ts * _BYTES[t.dtype] | hs * _BYTES[t.dtype]) & 15:
+            if output:
+                raise ValueError(f"{what} must have contiguous, 16-byte aligned head rows")
+            t = t.clone(memory_format=torch.contiguous_format)
+            return t.data_ptr(), heads * self.head_dim, self.head_dim, t
+        return ptr, ts, hs, t
 
     def _status(self, status):
         if status is None:
             return None
-        if status.dtype != torch.int32 or status.numel() < 1 or status.device != self.device:
+        if (status.dtype != torch.int32 or status.numel() < 1
+                or status.get_device() != self._index):
             raise ValueError("status must be an int32 tensor on the cache's device")
         return status.data_ptr()
 
@@ -193,15 +201,16 @@ class PagedKVCache:
         if other is not None:
             with other:
                 return self.write(batch, k, v, status)
-        self._check_rows(k, self.kv_heads, TYPE_IDS, "k")
-        self._check_rows(v, self.kv_heads, (k.dtype,), "v")
-        if k.shape != v.shape or batch.device != self.device:
+        kp, kts, khs, k = self._rows(k, self.kv_heads, TYPE_IDS, "k")
+        vp, vts, vhs, v = self._rows(v, self.kv_heads, (k.dtype,), "v")
+        tokens = k.shape[0]
+        if tokens != v.shape[0] or batch.index != self._index:
             raise ValueError("k, v and the batch must agree in tokens and device")
-        k, v = _rows(k), _rows(v)
-        _lib.check(self.lib.moe_b200_kv_write(
-            self._ref, batch.struct(k.shape[0]), TYPE_IDS[k.dtype], k.data_ptr(), *_strides(k),
-            v.data_ptr(), *_strides(v), self._status(status),
-            torch.cuda.current_stream(self.device).cuda_stream), "moe_b200_kv_write")
+        st = self.lib.moe_b200_kv_write(
+            self._ref, batch.struct(tokens), TYPE_IDS[k.dtype], kp, kts, khs, vp, vts, vhs,
+            self._status(status), _raw_stream(self._index))
+        if st:
+            _lib.check(st, "moe_b200_kv_write")
 
     def read(self, batch: KVBatch, tokens: int | None = None, dtype: torch.dtype | None = None,
              out: tuple[torch.Tensor, torch.Tensor] | None = None, status=None, stream=None):
@@ -220,19 +229,20 @@ class PagedKVCache:
                 raise ValueError("read needs out, or the number of tokens")
             if dtype is None:
                 dtype = torch.float16 if self.type == Q8_0 else self.k.dtype
-            shape = (tokens, self.kv_heads, self.head_dim)
-            out = tuple(torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
-        k, v = out
-        self._check_rows(k, self.kv_heads, TYPE_IDS, "out k")
-        self._check_rows(v, self.kv_heads, (k.dtype,), "out v")
-        if k.shape != v.shape or batch.device != self.device:
+            shape = (2, tokens, self.kv_heads, self.head_dim)
+            k, v = torch.empty(shape, dtype=dtype, device=self.device).unbind(0)
+        else:
+            k, v = out
+        kp, kts, khs, _ = self._rows(k, self.kv_heads, TYPE_IDS, "out k", output=True)
+        vp, vts, vhs, _ = self._rows(v, self.kv_heads, (k.dtype,), "out v", output=True)
+        tokens = k.shape[0]
+        if tokens != v.shape[0] or batch.index != self._index:
             raise ValueError("out and the batch must agree in tokens and device")
-        self._check_output(k, "out k")
-        self._check_output(v, "out v")
-        _lib.check(self.lib.moe_b200_kv_read(
-            self._ref, batch.struct(k.shape[0]), TYPE_IDS[k.dtype], k.data_ptr(), *_strides(k),
-            v.data_ptr(), *_strides(v), self._status(status),
-            torch.cuda.current_stream(self.device).cuda_stream), "moe_b200_kv_read")
+        st = self.lib.moe_b200_kv_read(
+            self._ref, batch.struct(tokens), TYPE_IDS[k.dtype], kp, kts, khs, vp, vts, vhs,
+            self._status(status), _raw_stream(self._index))
+        if st:
+            _lib.check(st, "moe_b200_kv_read")
         return k, v
 
     def attend(self, batch: KVBatch, q: torch.Tensor, out: torch.Tensor | None = None,
@@ -250,24 +260,24 @@ class PagedKVCache:
         if other is not None:
             with other:
                 return self.attend(batch, q, out, lse, scale, causal, window, status)
-        dtypes = (torch.float16, torch.bfloat16) if self.type == Q8_0 else (self.k.dtype,)
-        if q.dim() != 3 or q.shape[1] < 1 or q.shape[1] % self.kv_heads:
+        shape = q.shape
+        heads = shape[1] if len(shape) == 3 else 0
+        if heads < 1 or heads % self.kv_heads:
             raise ValueError("q must be [tokens, q_heads, head_dim], q_heads a multiple of "
                              "kv_heads")
-        tokens, heads = q.shape[0], q.shape[1]
-        self._check_rows(q, heads, dtypes, "q")
-        if batch.device != self.device:
+        qp, qts, qhs, q = self._rows(q, heads, self._q_dtypes, "q")
+        if batch.index != self._index:
             raise ValueError("q and the batch must be on the cache's device")
         if window < 0 or (window and not causal):
             raise ValueError("window must be positive, and needs causal")
-        q = _rows(q)
+        tokens = shape[0]
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+            out = torch.empty(shape, dtype=q.dtype, device=self.device)
+            op, ots, ohs = out.data_ptr(), heads * self.head_dim, self.head_dim
         else:
-            self._check_rows(out, heads, (q.dtype,), "out")
+            op, ots, ohs, _ = self._rows(out, heads, (q.dtype,), "out", output=True)
             if out.shape[0] != tokens:
                 raise ValueError("out must have q's shape")
-            self._check_output(out, "out")
         if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (tokens, heads)
                                 or not lse.is_contiguous() or lse.device != self.device):
             raise ValueError("lse must be a contiguous fp32 [tokens, q_heads] tensor on the "
@@ -285,10 +295,11 @@ class PagedKVCache:
         # a workspace of the call's own: torch's allocator hands it to the next
         # call on this stream, or keeps it with the graph that captured it
         ws = torch.empty(max(need, 256), dtype=torch.uint8, device=self.device)
-        _lib.check(self.lib.moe_b200_attend(
-            self._ref, bs, TYPE_IDS[q.dtype], q.data_ptr(), *_strides(q), heads,
-            out.data_ptr(), *_strides(out), lse.data_ptr() if lse is not None else None,
+        st = self.lib.moe_b200_attend(
+            self._ref, bs, TYPE_IDS[q.dtype], qp, qts, qhs, heads, op, ots, ohs,
+            lse.data_ptr() if lse is not None else None,
             self.head_dim ** -0.5 if scale is None else scale, 1 if causal else 0, window,
-            ws.data_ptr(), ws.numel(), self._status(status),
-            torch.cuda.current_stream(self.device).cuda_stream), "moe_b200_attend")
+            ws.data_ptr(), max(need, 256), self._status(status), _raw_stream(self._index))
+        if st:
+            _lib.check(st, "moe_b200_attend")
         return out
