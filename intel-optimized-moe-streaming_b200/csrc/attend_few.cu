@@ -8,10 +8,12 @@
 // the CUDA cores would need all of theirs.  tcgen05's smallest M is 64 and its
 // operands go through shared and tensor memory, which 16 rows do not repay.
 //
-// A warp walks subtiles of 16 keys on its own: a ring of NS shared-memory
-// entries per warp (a subtile's keys, then its values) filled by tensor copies
-// with a 128-byte swizzle, one lane issuing, no block barrier in the loop.
-// The scores of 16 rows x 16 keys stay in registers as the accumulator, become
+// A warp walks subtiles of 16 to 64 keys (8 KB) on its own: a ring of NS
+// shared-memory entries per warp (a subtile's keys, then its values) filled by
+// tensor copies with a 128-byte swizzle, no block barrier in the loop.  A
+// subtile is one chain of products, maximum, exponentials and products, about
+// 1900 cycles long however few keys it has, so it has as many as fit.
+// The scores of 16 rows x 16 G keys stay in registers as the accumulator, become
 // the A operand of the value product in place, and the running maximum, sum
 // and 16 x DP output are the warp's own until the tile ends; then the four
 // warps' sums are added through shared memory.  Two CTAs per SM, so that one
@@ -31,8 +33,6 @@ namespace {
 
 constexpr int kFewWarps = 4;
 constexpr int kFewThreads = kFewWarps * 32;
-constexpr int kFewKeys = 16;                     // keys of a subtile
-constexpr int kFewUnit = kFewKeys * kFewWarps;   // keys of a unit
 constexpr int kFewCost = 0;                      // of a tile, in units
 constexpr uint32_t kFewPolls = 1u << 21;
 
@@ -43,10 +43,15 @@ struct Few {
     static constexpr int ROWB = DP * EB;                       // bytes of a cached row
     static constexpr int SLABB = ROWB < 128 ? ROWB : 128;      // bytes of a row in one copy
     static constexpr int SLABS = ROWB / SLABB;
-    static constexpr int TILEB = kFewKeys * ROWB;
-    static constexpr int SCALEB = Q8 ? DP : 0;                 // 16 rows x DP / 32 scales
-    // ring entries: at most 96 KB per CTA, and 8
-    static constexpr int FIT = 96 * 1024 / (kFewWarps * (TILEB + SCALEB));
+    // G groups of 16 keys at a time, as many as make an entry of 8 KB (at most 4)
+    static constexpr int G = 8192 / (16 * ROWB) > 4 ? 4 : 8192 / (16 * ROWB);
+    static constexpr int KEYS = 16 * G;                        // keys of a subtile
+    static constexpr int UNIT = KEYS * kFewWarps;              // keys of a unit
+    static constexpr int TILEB = KEYS * ROWB;
+    static constexpr int SLAB = KEYS * SLABB;
+    static constexpr int SCALEB = Q8 ? KEYS * DP / 16 : 0;     // KEYS rows of DP / 32 scales
+    // ring entries: at most 102 KB per CTA (two CTAs share an SM), and 8
+    static constexpr int FIT = 104448 / (kFewWarps * (TILEB + SCALEB));
     static constexpr int NS = FIT > 8 ? 8 : FIT;
     static constexpr int VB = Q8 ? (DP >= 128 ? 16 : 8) : 8;   // codes a thread takes of a value row
     static constexpr int TILES = DP / 8;
@@ -62,6 +67,7 @@ struct Few {
     static constexpr int o_rs = o_l + kFewWarps * 16 * 4;
     static constexpr int smem = o_rs + 16 * 4 + 1024;          // 1024: base alignment
     static_assert(NS >= 3, "");
+    static_assert(2 * (smem + 1024) <= 233472, "two CTAs per SM");
     static_assert(kFewWarps * 16 * (PD + 4) * 4 <= o_q, "join buffer inside the ring");
 };
 
@@ -69,13 +75,13 @@ template <int KIND>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                          uint32_t b1) {
     if constexpr (KIND == KIND_BF16)
-        asm volatile(
+        asm(
             "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
             "{%8,%9}, {%0,%1,%2,%3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
-        asm volatile(
+        asm(
             "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
             "{%8,%9}, {%0,%1,%2,%3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -94,6 +100,12 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
                      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                      : "r"(addr)
                      : "memory");
+}
+
+// A NaN, an infinity, or a scale that takes code -128 out of binary16 (512 and
+// above): where nothing was copied, scales and codes are any bits.
+__device__ __forceinline__ bool odd_scale(__half s) {
+    return (__half_as_ushort(s) & 0x7fffu) >= 0x6000u;
 }
 
 // Key of column n of an 8-key score tile.  Q8_0 swaps odd keys n and n ^ 4:
@@ -142,7 +154,7 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
 
     const int ctas = gridDim.x;
     AttendWs ws(wsp, ctas);
-    AttendCursor cur = attend_place<kFewRows, kFewUnit, kFewCost, kFewThreads>(
+    AttendCursor cur = attend_place<kFewRows, F::UNIT, kFewCost, kFewThreads>(
         a, *reinterpret_cast<AttendScratch*>(sm), blockIdx.x, ctas, a.status);
     fence_async_smem();   // the scratch lies in the ring
     AttendRecord rec{};
@@ -153,7 +165,7 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
     if (cur.left > 0) s = attend_seq(a, cur.seq, nullptr);
 
     while (cur.left > 0) {
-        const AttendPart part = attend_part<kFewRows, kFewUnit, kFewCost>(a, cur, s);
+        const AttendPart part = attend_part<kFewRows, F::UNIT, kFewCost>(a, cur, s);
         const int u0 = part.u0, take = part.take;
         const int rows = s.n * a.group - cur.tile * kFewRows;   // valid rows: the first `rows`
 
@@ -198,7 +210,8 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
                                                 kv_to_f<TQ>(q[1]) * sm_rs[r]);
                 }
             }
-            qf[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+            qf[i] = make_uint4(w[0] ^ flip, w[1] ^ flip, w[2] ^ flip, w[3] ^ flip);
         }
         // the two rows of this thread: the keys they attend, the factor that
         // takes a score to units of log 2
@@ -217,7 +230,7 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            mul[i] = a.scale * kLog2e;
+            mul[i] = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);   // 0: equal weights
             if constexpr (F::Q8 && std::is_same<TQ, __nv_bfloat16>::value)
                 mul[i] /= sm_rs[n8 + 8 * i];
         }
@@ -233,6 +246,18 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
             }
         }
 
+        auto q_at = [&](int st, uint32_t (&qa)[4]) {
+            if constexpr (DP <= 128) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) qa[i] = qreg[st][i];
+            } else {
+                const uint4 w = qf[st * 32 + lane];
+                qa[0] = w.x;
+                qa[1] = w.y;
+                qa[2] = w.z;
+                qa[3] = w.w;
+            }
+        };
         float o[F::TILES][4];
 #pragma unroll
         for (int i = 0; i < F::TILES; ++i)
@@ -240,39 +265,48 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
             for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-        // Page ids of 32 subtiles at a time, one per lane (-1: nothing there).
+        // A subtile is fetched in boxes of whole pages or parts of one; the
+        // page ids of 32 boxes at a time are held one per lane (-1: nothing
+        // there).
+        const int box = a.c.page_size < F::KEYS ? a.c.page_size : F::KEYS;
+        const int boxes = F::KEYS / box;
         int page_of = -1, win = 0;
-        uint32_t there = 0;   // bit j % 32: subtile j was fetched
-        auto look_up = [&](int j0) {
-            win = j0;
+        uint32_t there = 0;   // bit j % 32: a part of subtile j was fetched
+        auto look_up = [&](int b0) {
+            win = b0;
             page_of = -1;
-            const int key = ((u0 + j0 + lane) * kFewWarps + warp) * kFewKeys;
-            if (j0 + lane < take && key < t_hi && key + kFewKeys > t_lo)
+            const int j = (b0 + lane) / boxes;
+            const int key = ((u0 + j) * kFewWarps + warp) * F::KEYS + (b0 + lane) % boxes * box;
+            if (j < take && key < t_hi && key + box > t_lo)
                 page_of = kv_page(a.b, a.c, cur.seq, key >> a.c.page_shift, a.status);
         };
         // entry e: the keys (even) or values (odd) of subtile e / 2
         auto fetch = [&](int e) {
             const int j = e >> 1, w = e & 1;
             if (j >= take) return;
-            if (j - win >= 32) look_up(j);
-            const int page = __shfl_sync(0xffffffffu, page_of, j - win);
-            if (!w) there = (there & ~(1u << (j & 31))) | ((page >= 0 ? 1u : 0u) << (j & 31));
-            if (page < 0) return;
-            const int key = ((u0 + j) * kFewWarps + warp) * kFewKeys;
-            const int row = key & (a.c.page_size - 1);
-            const int z = page * a.c.heads + cur.kvh;
-            if (lane == 0) {
-                uint64_t* bar = &bars[in_slot];
-                unsigned char* dst = ring + in_slot * F::TILEB;
-                mbar_arrive_expect_tx(bar, F::TILEB + (F::Q8 ? a.c.dim : 0));
+            if (j * boxes - win >= 32) look_up(j * boxes);
+            const int page = __shfl_sync(0xffffffffu, page_of, (j * boxes - win + lane % boxes) & 31);
+            const bool go = lane < boxes && page >= 0;
+            const int n = __popc(__ballot_sync(0xffffffffu, go));
+            if (!w) there = (there & ~(1u << (j & 31))) | ((n ? 1u : 0u) << (j & 31));
+            if (!n) return;
+            uint64_t* bar = &bars[in_slot];
+            if (lane == 0)
+                mbar_arrive_expect_tx(bar, (uint32_t)(n * box * (F::ROWB + (F::Q8 ? nb * 2 : 0))));
+            __syncwarp();
+            if (go) {
+                const int key = ((u0 + j) * kFewWarps + warp) * F::KEYS + lane * box;
+                const int row = key & (a.c.page_size - 1);
+                const int z = page * a.c.heads + cur.kvh;
+                unsigned char* dst = ring + in_slot * F::TILEB + lane * box * F::SLABB;
 #pragma unroll
                 for (int sl = 0; sl < F::SLABS; ++sl)
-                    tma_load_3d(dst + sl * kFewKeys * F::SLABB, w ? &vmap : &kmap,
-                                sl * (F::SLABB / F::EB), row, z, bar);
+                    tma_load_3d(dst + sl * F::SLAB, w ? &vmap : &kmap, sl * (F::SLABB / F::EB), row,
+                                z, bar);
                 if constexpr (F::Q8)
-                    bulk_g2s(sring + in_slot * F::SCALEB,
+                    bulk_g2s(sring + in_slot * F::SCALEB + lane * box * nb * 2,
                              (w ? a.c.vs : a.c.ks) + (((int64_t)z << a.c.page_shift) + row) * nb,
-                             a.c.dim, bar);
+                             (uint32_t)(box * nb * 2), bar);
             }
             in_slot = in_slot + 1 == F::NS ? 0 : in_slot + 1;
         };
@@ -294,69 +328,57 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
                 fetch(2 * j + 1 + F::NS);
                 continue;
             }
-            const int key0 = ((u0 + j) * kFewWarps + warp) * kFewKeys;
-            // ---- scores
-            float sc[2][4] = {}, sx[2][4] = {};
+            const int key0 = ((u0 + j) * kFewWarps + warp) * F::KEYS;
+            // ---- scores: 8-key column tiles
+            float p[2 * F::G][4] = {};
             await();
             {
                 const unsigned char* kt = ring + out_slot * F::TILEB;
-                const uint32_t kaddr = smem_u32(kt);
                 if constexpr (!F::Q8) {
+                    const uint32_t kaddr = smem_u32(kt);
                     const int key = (lane >> 4) * 8 + (lane & 7), half = (lane >> 3) & 1;
 #pragma unroll
                     for (int st = 0; st < DP / 16; ++st) {
-                        uint32_t b[4], qa[4];
-                        const int slab = st >> 2, ch = (st & 3) * 2 + half;
-                        ldsm4<false>(b, kaddr + slab * 2048 + key * 128 + ((ch ^ (key & 7)) << 4));
-                        if constexpr (DP <= 128) {
+                        uint32_t b[F::G][4], qa[4];
+                        const int ch = (st & 3) * 2 + half;
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) qa[i] = qreg[st][i];
-                        } else {
-                            const uint4 w = qf[st * 32 + lane];
-                            qa[0] = w.x; qa[1] = w.y; qa[2] = w.z; qa[3] = w.w;
-                        }
-                        if (st & 1) {
-                            mma16816<KIND>(sx[0], qa, b[0], b[1]);
-                            mma16816<KIND>(sx[1], qa, b[2], b[3]);
-                        } else {
-                            mma16816<KIND>(sc[0], qa, b[0], b[1]);
-                            mma16816<KIND>(sc[1], qa, b[2], b[3]);
+                        for (int g = 0; g < F::G; ++g)
+                            ldsm4<false>(b[g], kaddr + (st >> 2) * F::SLAB + (g * 16 + key) * 128 +
+                                                   ((ch ^ (key & 7)) << 4));
+                        q_at(st, qa);
+#pragma unroll
+                        for (int g = 0; g < F::G; ++g) {
+                            mma16816<KIND>(p[2 * g], qa, b[g][0], b[g][1]);
+                            mma16816<KIND>(p[2 * g + 1], qa, b[g][2], b[g][3]);
                         }
                     }
                 } else {
                     const __half* ks = reinterpret_cast<const __half*>(sring + out_slot * F::SCALEB);
 #pragma unroll
                     for (int sp = 0; sp < DP / 64; ++sp) {
+                        const int blk = sp * 2 + (c4 >> 1);
+                        uint32_t qa[4][4];
 #pragma unroll
-                        for (int t = 0; t < 2; ++t) {
+                        for (int st = 0; st < 4; ++st) q_at(sp * 4 + st, qa[st]);
+#pragma unroll
+                        for (int t = 0; t < 2 * F::G; ++t) {
                             const int key = t * 8 + column_key<KIND>(n8);
-                            uint32_t addr;
-                            if constexpr (F::SLABB == 128)
-                                addr = kaddr + (sp >> 1) * 2048 + key * 128 +
-                                       ((((sp & 1) * 4 + c4) ^ (key & 7)) << 4);
-                            else
-                                addr = kaddr + key * 64 + c4 * 16;
-                            uint32_t w[4];
-                            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                                         : "r"(addr)
-                                         : "memory");
-                            const int blk = sp * 2 + (c4 >> 1);
+                            const int at = F::SLABB == 128
+                                               ? (sp >> 1) * F::SLAB + key * 128 +
+                                                     ((((sp & 1) * 4 + c4) ^ (key & 7)) << 4)
+                                               : key * 64 + c4 * 16;
+                            const uint4 w = *reinterpret_cast<const uint4*>(kt + at);
                             const __half2 d = __half2half2(blk < nb ? ks[key * nb + blk]
                                                                     : __ushort_as_half(0));
-#pragma unroll
-                            for (int st = 0; st < 4; ++st) {
-                                uint32_t b0, b1, qa[4];
-                                codes4(w[st], d, b0, b1);
-                                if constexpr (DP <= 128) {
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i) qa[i] = qreg[sp * 4 + st][i];
-                                } else {
-                                    const uint4 x = qf[(sp * 4 + st) * 32 + lane];
-                                    qa[0] = x.x; qa[1] = x.y; qa[2] = x.z; qa[3] = x.w;
-                                }
-                                mma16816<KIND>(st & 1 ? sx[t] : sc[t], qa, b0, b1);
-                            }
+                            uint32_t b0, b1;
+                            codes4(w.x, d, b0, b1);
+                            mma16816<KIND>(p[t], qa[0], b0, b1);
+                            codes4(w.y, d, b0, b1);
+                            mma16816<KIND>(p[t], qa[1], b0, b1);
+                            codes4(w.z, d, b0, b1);
+                            mma16816<KIND>(p[t], qa[2], b0, b1);
+                            codes4(w.w, d, b0, b1);
+                            mma16816<KIND>(p[t], qa[3], b0, b1);
                         }
                     }
                 }
@@ -365,35 +387,33 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
             release();
             fetch(2 * j + F::NS);
             // ---- softmax of this subtile
-            const bool whole = key0 >= all_lo && key0 + kFewKeys <= all_hi;
-            float p[2][4];
+            const bool whole = key0 >= all_lo && key0 + F::KEYS <= all_hi;
+            if (!whole) {
+#pragma unroll
+                for (int t = 0; t < 2 * F::G; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = key0 + t * 8 + column_key<KIND>(c4 * 2 + (e & 1));
+                        if (key < lo[e >> 1] || key >= hi[e >> 1]) p[t][e] = -INFINITY;
+                    }
+            }
             float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < 2 * F::G; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float v = (sc[t][e] + sx[t][e]) * mul[e >> 1];
-                    const int key = key0 + t * 8 + column_key<KIND>(c4 * 2 + (e & 1));
-                    if (!whole && (key < lo[e >> 1] || key >= hi[e >> 1])) v = -INFINITY;
-                    p[t][e] = v;
-                    top[e >> 1] = fmaxf(top[e >> 1], v);
-                }
+                for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], p[t][e]);
             bool grew = false;
             float keep[2], base[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
                 top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-                const float mn = fmaxf(m[i], top[i]);
+                const float mn = fmaxf(m[i], top[i] * mul[i]);
                 base[i] = mn == -INFINITY ? 0.f : mn - F::SHIFT;
                 keep[i] = ex2(m[i] - (mn == -INFINITY ? 0.f : mn));
                 grew = grew || mn > m[i];
                 m[i] = mn;
             }
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) p[t][e] = ex2(p[t][e] - base[e >> 1]);
             if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) l[i] *= keep[i];
@@ -406,13 +426,17 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                l[i] += p[0][2 * i] + p[0][2 * i + 1] + p[1][2 * i] + p[1][2 * i + 1];
-            uint32_t pa[4];
+            for (int t = 0; t < 2 * F::G; ++t)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                pa[2 * t] = pack16<KIND>(p[t][0], p[t][1]);
-                pa[2 * t + 1] = pack16<KIND>(p[t][2], p[t][3]);
+                for (int e = 0; e < 4; ++e) {
+                    p[t][e] = ex2(fmaf(p[t][e], mul[e >> 1], -base[e >> 1]));
+                    l[e >> 1] += p[t][e];
+                }
+            uint32_t pa[F::G][4];
+#pragma unroll
+            for (int t = 0; t < 2 * F::G; ++t) {
+                pa[t / 2][2 * (t & 1)] = pack16<KIND>(p[t][0], p[t][1]);
+                pa[t / 2][2 * (t & 1) + 1] = pack16<KIND>(p[t][2], p[t][3]);
             }
             // ---- values
             await();
@@ -424,8 +448,8 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
                 // the rows that attend them one by one and leave the tile.
                 bool odd = false;
                 if constexpr (F::Q8) {
-                    for (int i = lane; i < kFewKeys * nb; i += 32)
-                        odd = odd || odd16<KIND_F16>(__half_as_ushort(vs[i]));
+                    for (int i = lane; i < F::KEYS * nb; i += 32)
+                        odd = odd || odd_scale(vs[i]);
                 } else {
                     const uint4* v4 = reinterpret_cast<const uint4*>(vt);
                     for (int i = lane; i < F::TILEB / 16; i += 32) {
@@ -435,55 +459,58 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
                     }
                 }
                 if (__any_sync(0xffffffffu, odd)) {
-#pragma unroll 1
-                    for (int k = 0; k < kFewKeys; ++k) {
-                        const int col = column_key<KIND>(k & 7);   // its own inverse
-                        const int from = (lane & ~3) | (col >> 1);
-                        const bool t1 = k >= 8, e1 = col & 1;
-                        float pk[2];
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const float a0 = __shfl_sync(0xffffffffu, p[0][2 * i], from);
-                            const float a1 = __shfl_sync(0xffffffffu, p[0][2 * i + 1], from);
-                            const float b0 = __shfl_sync(0xffffffffu, p[1][2 * i], from);
-                            const float b1 = __shfl_sync(0xffffffffu, p[1][2 * i + 1], from);
-                            pk[i] = t1 ? (e1 ? b1 : b0) : (e1 ? a1 : a0);
+                    // value of key k, dimension d when it is not finite, else 0
+                    auto odd_value = [&](int k, int d) {
+                        if constexpr (F::Q8) {
+                            if (d >= a.c.dim) return 0.f;
+                            const __half s = vs[k * nb + (d >> 5)];
+                            if (!odd_scale(s)) return 0.f;
+                            const int at = F::SLABB == 128
+                                               ? (d >> 7) * F::SLAB + k * 128 +
+                                                     ((((d >> 4) & 7) ^ (k & 7)) << 4) + (d & 15)
+                                               : k * 64 + d;
+                            return __half2float(s) * (float)reinterpret_cast<const int8_t*>(vt)[at];
+                        } else {
+                            const int at = (d >> 6) * F::SLAB + k * 128 +
+                                           ((((d >> 3) & 7) ^ (k & 7)) << 4) + (d & 7) * 2;
+                            const uint16_t w = *reinterpret_cast<const uint16_t*>(vt + at);
+                            if (!odd16<KIND>(w)) return 0.f;
+                            return KIND == KIND_BF16 ? __bfloat162float(__ushort_as_bfloat16(w))
+                                                     : __half2float(__ushort_as_half(w));
                         }
-                        const bool at0 = key0 + k >= lo[0] && key0 + k < hi[0];
-                        const bool at1 = key0 + k >= lo[1] && key0 + k < hi[1];
+                    };
 #pragma unroll
-                        for (int i = 0; i < F::TILES; ++i)
+                    for (int t = 0; t < 2 * F::G; ++t) {
+#pragma unroll 1
+                        for (int k8 = 0; k8 < 8; ++k8) {
+                            const int col = column_key<KIND>(k8);   // its own inverse
+                            const int from = (lane & ~3) | (col >> 1);
+                            float pk[2];
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const int d = out_dim<DP, KIND>(i, c4 * 2 + e);
-                                float v = 0.f;
-                                if constexpr (F::Q8) {
-                                    if (d < a.c.dim && odd16<KIND_F16>(__half_as_ushort(vs[k * nb + (d >> 5)]))) {
-                                        const int byte = F::SLABB == 128
-                                            ? (d >> 7) * 2048 + k * 128 + ((((d >> 4) & 7) ^ (k & 7)) << 4) + (d & 15)
-                                            : k * 64 + d;
-                                        v = __half2float(vs[k * nb + (d >> 5)]) *
-                                            (float)reinterpret_cast<const int8_t*>(vt)[byte];
-                                    }
-                                } else {
-                                    const int byte = (d >> 6) * 2048 + k * 128 +
-                                                     ((((d >> 3) & 7) ^ (k & 7)) << 4) + (d & 7) * 2;
-                                    const uint16_t w = *reinterpret_cast<const uint16_t*>(vt + byte);
-                                    if (odd16<KIND>(w))
-                                        v = KIND == KIND_BF16
-                                                ? __bfloat162float(__ushort_as_bfloat16(w))
-                                                : __half2float(__ushort_as_half(w));
-                                }
-                                if (v != 0.f) {   // NaN or infinite
-                                    if (at0) o[i][e] += pk[0] * v;
-                                    if (at1) o[i][2 + e] += pk[1] * v;
-                                }
+                            for (int i = 0; i < 2; ++i) {
+                                const float x = __shfl_sync(0xffffffffu, p[t][2 * i], from);
+                                const float y = __shfl_sync(0xffffffffu, p[t][2 * i + 1], from);
+                                pk[i] = col & 1 ? y : x;
                             }
+                            const int k = t * 8 + k8;
+                            const bool at0 = key0 + k >= lo[0] && key0 + k < hi[0];
+                            const bool at1 = key0 + k >= lo[1] && key0 + k < hi[1];
+#pragma unroll
+                            for (int i = 0; i < F::TILES; ++i)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const float v = odd_value(k, out_dim<DP, KIND>(i, c4 * 2 + e));
+                                    if (v != 0.f) {   // NaN or infinite
+                                        if (at0) o[i][e] += pk[0] * v;
+                                        if (at1) o[i][2 + e] += pk[1] * v;
+                                    }
+                                }
+                        }
                     }
                     __syncwarp();
                     if constexpr (F::Q8) {
-                        for (int i = lane; i < kFewKeys * nb; i += 32)
-                            if (odd16<KIND_F16>(__half_as_ushort(vs[i]))) vs[i] = __ushort_as_half(0);
+                        for (int i = lane; i < F::KEYS * nb; i += 32)
+                            if (odd_scale(vs[i])) vs[i] = __ushort_as_half(0);
                     } else {
                         uint16_t* v2 = reinterpret_cast<uint16_t*>(vt);
                         for (int i = lane; i < F::TILEB / 2; i += 32)
@@ -493,50 +520,53 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
                     __syncwarp();
                 }
             }
-            const uint32_t vaddr = smem_u32(vt);
             if constexpr (!F::Q8) {
+                const uint32_t vaddr = smem_u32(vt);
                 const int key = ((lane >> 3) & 1) * 8 + (lane & 7), half = lane >> 4;
 #pragma unroll
                 for (int d = 0; d < DP / 16; ++d) {
-                    uint32_t b[4];
                     const int ch = (d & 3) * 2 + half;
-                    ldsm4<true>(b, vaddr + (d >> 2) * 2048 + key * 128 + ((ch ^ (key & 7)) << 4));
-                    mma16816<KIND>(o[2 * d], pa, b[0], b[1]);
-                    mma16816<KIND>(o[2 * d + 1], pa, b[2], b[3]);
+#pragma unroll
+                    for (int g = 0; g < F::G; ++g) {
+                        uint32_t b[4];
+                        ldsm4<true>(b, vaddr + (d >> 2) * F::SLAB + (g * 16 + key) * 128 +
+                                           ((ch ^ (key & 7)) << 4));
+                        mma16816<KIND>(o[2 * d], pa[g], b[0], b[1]);
+                        mma16816<KIND>(o[2 * d + 1], pa[g], b[2], b[3]);
+                    }
                 }
             } else {
                 constexpr int W = F::VB / 4;   // 32-bit words of codes per key
 #pragma unroll
                 for (int sl = 0; sl < DP / (F::VB * 8); ++sl) {
-                    uint32_t w[4][W];
-                    __half2 d[4];
                     const int blk = (sl * F::VB * 8 + n8 * F::VB) >> 5;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int key = column_key<KIND>(c4 * 2 + (i & 1)) + (i >> 1) * 8;
-                        d[i] = __half2half2(blk < nb ? vs[key * nb + blk] : __ushort_as_half(0));
-                        if constexpr (F::VB == 16)
-                            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                                         : "=r"(w[i][0]), "=r"(w[i][1]), "=r"(w[i][2]), "=r"(w[i][3])
-                                         : "r"(vaddr + sl * 2048 + key * 128 + ((n8 ^ (key & 7)) << 4))
-                                         : "memory");
-                        else
-                            asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];"
-                                         : "=r"(w[i][0]), "=r"(w[i][1])
-                                         : "r"(vaddr + key * 64 + n8 * 8)
-                                         : "memory");
-                    }
+                    for (int g = 0; g < F::G; ++g) {
+                        uint32_t w[4][W];
+                        __half2 d[4];
 #pragma unroll
-                    for (int g = 0; g < W; ++g) {
-                        uint32_t x[4][2];
+                        for (int i = 0; i < 4; ++i) {
+                            const int key = g * 16 + column_key<KIND>(c4 * 2 + (i & 1)) + (i >> 1) * 8;
+                            d[i] = __half2half2(blk < nb ? vs[key * nb + blk] : __ushort_as_half(0));
+                            if constexpr (F::VB == 16)
+                                *reinterpret_cast<uint4*>(w[i]) = *reinterpret_cast<const uint4*>(
+                                    vt + sl * F::SLAB + key * 128 + ((n8 ^ (key & 7)) << 4));
+                            else
+                                *reinterpret_cast<uint2*>(w[i]) =
+                                    *reinterpret_cast<const uint2*>(vt + key * 64 + n8 * 8);
+                        }
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) codes4(w[i][g], d[i], x[i][0], x[i][1]);
+                        for (int q = 0; q < W; ++q) {
+                            uint32_t x[4][2];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const unsigned sel = e & 1 ? 0x7632u : 0x5410u;
-                            mma16816<KIND>(o[sl * F::VB + g * 4 + e], pa,
-                                           __byte_perm(x[0][e >> 1], x[1][e >> 1], sel),
-                                           __byte_perm(x[2][e >> 1], x[3][e >> 1], sel));
+                            for (int i = 0; i < 4; ++i) codes4(w[i][q], d[i], x[i][0], x[i][1]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const unsigned sel = e & 1 ? 0x7632u : 0x5410u;
+                                mma16816<KIND>(o[sl * F::VB + q * 4 + e], pa[g],
+                                               __byte_perm(x[0][e >> 1], x[1][e >> 1], sel),
+                                               __byte_perm(x[2][e >> 1], x[3][e >> 1], sel));
+                            }
                         }
                     }
                 }
@@ -652,8 +682,9 @@ template <int DP, int KIND, typename TQ>
 cudaError_t launch_few(const AttendArgs& a, void* ws, cudaStream_t s) {
     using F = Few<DP, KIND>;
     CUtensorMap kmap, vmap;
-    if (!attend_map(&kmap, a.c, a.c.k, F::SLABB / F::EB, kFewKeys) ||
-        !attend_map(&vmap, a.c, a.c.v, F::SLABB / F::EB, kFewKeys))
+    const int box = a.c.page_size < F::KEYS ? a.c.page_size : F::KEYS;
+    if (!attend_map(&kmap, a.c, a.c.k, F::SLABB / F::EB, box) ||
+        !attend_map(&vmap, a.c, a.c.v, F::SLABB / F::EB, box))
         return cudaErrorInvalidValue;
     cudaError_t e = cudaFuncSetAttribute(k_attend_few<DP, KIND, TQ>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, F::smem);
