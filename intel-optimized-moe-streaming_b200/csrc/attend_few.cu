@@ -444,20 +444,35 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
             __half* vs = reinterpret_cast<__half*>(sring + out_slot * F::SCALEB);
             if (!whole) {
                 // A key that only some rows attend, or none: 0 * NaN would
-                // reach the others.  Values that are not finite are added to
-                // the rows that attend them one by one and leave the tile.
+                // reach the others.  Keys that no row attends (they may lie
+                // behind the sequence, or not have been copied) become zeros.
+                // Of the others, values that are not finite are added to the
+                // rows that attend them one by one and leave the tile.
+                const int r_lo = t_lo - key0, r_hi = t_hi - key0;
                 bool odd = false;
                 if constexpr (F::Q8) {
-                    for (int i = lane; i < F::KEYS * nb; i += 32)
-                        odd = odd || odd_scale(vs[i]);
+                    for (int i = lane; i < F::KEYS; i += 32)
+                        for (int b = 0; b < nb; ++b) {
+                            if (i < r_lo || i >= r_hi)
+                                vs[i * nb + b] = __ushort_as_half(0);
+                            else
+                                odd = odd || odd_scale(vs[i * nb + b]);
+                        }
                 } else {
-                    const uint4* v4 = reinterpret_cast<const uint4*>(vt);
+                    uint4* v4 = reinterpret_cast<uint4*>(vt);
+#pragma unroll 4
                     for (int i = lane; i < F::TILEB / 16; i += 32) {
-                        const uint4 w = v4[i];
-                        odd = odd || odd16<KIND>(w.x) || odd16<KIND>(w.y) || odd16<KIND>(w.z) ||
-                              odd16<KIND>(w.w);
+                        const int r = (i >> 3) % F::KEYS;
+                        if (r < r_lo || r >= r_hi) {
+                            v4[i] = make_uint4(0, 0, 0, 0);
+                        } else {
+                            const uint4 w = v4[i];
+                            odd = odd || odd16x8<KIND>(w);
+                        }
                     }
                 }
+                fence_async_smem();
+                __syncwarp();
                 if (__any_sync(0xffffffffu, odd)) {
                     // value of key k, dimension d when it is not finite, else 0
                     auto odd_value = [&](int k, int d) {

@@ -518,8 +518,9 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                 if (!whole) {
                     // A key that only some rows attend, or none: 0 * NaN would
                     // reach the others.  Two warps look through the values of
-                    // such a unit; those that are not finite are added to the
-                    // rows that attend them one by one and leave the stage.
+                    // such a unit and clear those that no row attends; if any
+                    // that are left are not finite, they are added to the rows
+                    // that attend them one by one and leave the stage.
                     ++partial;
                     spin(&bars->checked[0], partial);
                     spin(&bars->checked[1], partial);
@@ -759,23 +760,19 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                     uint32_t* odd = bars->odd[partial & 7];
                     for (int h = 0; h < F::KPARTS; ++h) {
                         const int n = stage0 + stage_v<F::NQ>(j, w.take) + h;
-                        const uint4* st = reinterpret_cast<const uint4*>(
-                            sm + F::o_stage + (n % F::NST) * F::STAGEB);
+                        uint4* st = reinterpret_cast<uint4*>(sm + F::o_stage +
+                                                             (n % F::NST) * F::STAGEB);
                         await(&bars->full[n % F::NST], (uint32_t)(n / F::NST));
 #pragma unroll 4
                         for (int i = tid - 320; i < F::STAGEB / 16; i += 64) {
-                            const uint4 v = st[i];
-                            // an exponent of ones carries into the sign bit
-                            constexpr uint32_t e = KIND == KIND_BF16 ? 0x7f807f80u : 0x7c007c00u;
-                            constexpr uint32_t one = KIND == KIND_BF16 ? 0x00800080u : 0x04000400u;
-                            const uint32_t x = ((v.x & e) + one) | ((v.y & e) + one) |
-                                               ((v.z & e) + one) | ((v.w & e) + one);
-                            if (x & 0x80008000u) {
-                                const int k = h * F::VKEYS + (i >> 3) % F::VKEYS;
+                            const int k = h * F::VKEYS + (i >> 3) % F::VKEYS;
+                            if (key0 + k < tile.t_lo || key0 + k >= tile.t_hi)
+                                st[i] = make_uint4(0, 0, 0, 0);
+                            else if (odd16x8<KIND>(st[i]))
                                 atomicOr(&odd[k >> 5], 1u << (k & 31));
-                            }
                         }
                     }
+                    fence_async_smem();
                     __threadfence_block();
                     __syncwarp();
                     if (lane == 0) *reinterpret_cast<volatile uint32_t*>(&bars->checked[warp - 10]) = partial;

@@ -58,6 +58,15 @@ __device__ __forceinline__ bool odd16(uint32_t pair) {   // a NaN or an infinity
     return (pair & e) == e || ((pair >> 16) & e) == e;
 }
 
+template <int KIND>
+__device__ __forceinline__ bool odd16x8(const uint4& v) {   // in eight values
+    // an exponent of ones carries into the sign bit
+    constexpr uint32_t e = KIND == KIND_BF16 ? 0x7f807f80u : 0x7c007c00u;
+    constexpr uint32_t one = KIND == KIND_BF16 ? 0x00800080u : 0x04000400u;
+    return ((((v.x & e) + one) | ((v.y & e) + one) | ((v.z & e) + one) | ((v.w & e) + one)) &
+            0x80008000u) != 0;
+}
+
 // Power of two that takes a row maximum of magnitude `top` to [1, 2) (1 for
 // zero, subnormal, infinite and NaN rows): a bfloat16 row times it is exact
 // in binary16 but for values 2^-14 times smaller than the maximum.
