@@ -50,7 +50,9 @@ struct Many {
     static constexpr int STAGEB = KSLABS * kManyKeys * 128;
     static constexpr int QB = NQ * SLABS * 128 * 128;
     static constexpr int NST = DP == 64 ? 8 : 5;
-    static constexpr int NC = NQ == 2 ? 128 : 64;        // score columns of a thread
+    static constexpr int STEP = NQ == 2 ? 64 : 128;      // keys of a score tile
+    static constexpr int HS = kManyKeys / STEP;          // score tiles of a unit
+    static constexpr int NC = 64;                        // score columns of a thread
     static constexpr int OC = NQ == 2 ? DP : DP / 2;     // output columns of a thread
     static constexpr int THREADS = Q8 ? 512 : 384;
     // binary16 probabilities: 2^7 of the maximum in use, at most 2^15
@@ -61,16 +63,16 @@ struct Many {
     static constexpr int o_max = o_fac + M * 4;          // maxima and sums of half rows
     static constexpr int smem = o_max + (NQ == 1 ? 2048 : 0);
     static_assert(smem <= 232448, "shared memory of a CTA");
-    static constexpr uint32_t IDESC_S = umma_idesc_f16(128, kManyKeys) |
+    static constexpr uint32_t IDESC_S = umma_idesc_f16(128, STEP) |
                                         (KIND == KIND_BF16 ? (1u << 7) | (1u << 10) : 0u);
     static constexpr uint32_t IDESC_O = umma_idesc_f16(128, DP) | (1u << 16) |   // B: N-major
                                         (KIND == KIND_BF16 ? (1u << 7) | (1u << 10) : 0u);
 };
 
 struct ManyBars {
-    uint64_t full[8], empty[8], s_full[2], p_full[2], pv_done[2], q_full[2];
+    uint64_t full[8], empty[8], s_full[2][2], p_full[2][2], pv_done[2], q_full[2];
     uint32_t tmem, lost;
-    uint32_t products;     // units whose value products have been issued
+    uint32_t products;     // score tiles whose value products have been issued
     uint32_t checked[2];   // partly attended units that each checking warp is done with
     uint32_t odd[8][4];    // such units in turn: keys whose values are not all finite
 };
@@ -141,6 +143,17 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool v
                  "r"(valid ? 16 : 0)
                  : "memory");
 }
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(e));
+    return e != 0;
+}
+
+// A value that all lanes hold, marked as such for the compiler.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 // One role's walk over the segments (stretch of one tile) of its CTA.
 template <int DP, int KIND>
@@ -264,8 +277,10 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             mbar_init(&bars->empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&bars->s_full[i], 1);
-            mbar_init(&bars->p_full[i], F::NQ == 2 ? 4 : 8);
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(&bars->s_full[i][b], 1);
+                mbar_init(&bars->p_full[i][b], F::NQ == 2 ? 4 : 8);
+            }
             mbar_init(&bars->pv_done[i], 1);
             mbar_init(&bars->q_full[i], F::NQ == 2 ? 4 : 8);
         }
@@ -308,10 +323,6 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
 
     if (warp < 8) {
         // ------------------------------------------------------------ softmax
-        if constexpr (F::Q8)
-            asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
-        else
-            asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int wg = warp >> 2, quarter = warp & 3;
         const int row = quarter * 32 + lane;                       // of the 128-row tile
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;     // TMEM lane offset
@@ -322,8 +333,8 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         constexpr int QN = F::NQ == 2 ? 32 : 16;                   // query rows the warp loads
         float* xmax = reinterpret_cast<float*>(sm + F::o_max);     // [2][2][128]
         AttendRecord rec{};
-        uint32_t it = 0;       // units done by the CTA
-        uint32_t partial = 0;  // of them, those that not all rows attend
+        uint32_t it = 0;       // score tiles done by the CTA
+        uint32_t partial = 0;  // units met that not all rows attend
         int stage0 = 0;        // ring stages before this segment
 
         auto load_queries = [&](int n_valid) {
@@ -336,11 +347,12 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             if (lane == 0) mbar_arrive(&bars->q_full[F::NQ == 2 ? wg : 0]);
         };
         // The unit's odd values: all eight warps meet here.
-        auto poisoned = [&](volatile uint32_t* odd, int j, uint32_t t_s, int key0, int lo, int hi) {
-            const unsigned char* st[F::KPARTS];
+        auto poisoned = [&](volatile uint32_t* odd, int i, uint32_t t_s, int key0, int lo, int hi) {
+            const int j = i / F::HS, half = i % F::HS;
+            const int tw = F::NQ == 2 ? wg : 0;
+            unsigned char* st[F::KPARTS];
 #pragma unroll
-            for (int h = 0; h < F::KPARTS; ++h)
-            {
+            for (int h = 0; h < F::KPARTS; ++h) {
                 const int n = stage0 + stage_v<F::NQ>(j, w.take) + h;
                 st[h] = sm + F::o_stage + (n % F::NST) * F::STAGEB;
                 await(&bars->full[n % F::NST], (uint32_t)(n / F::NST));
@@ -348,12 +360,12 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             tc_fence_before();
             bar_sync<2, 256>();   // with one tile, O takes both halves' probabilities
             tc_fence_after();
-            if (j > 0) {
-                await(&bars->pv_done[F::NQ == 2 ? wg : 0], it - 1);
+            if (i > 0) {
+                await(&bars->pv_done[tw], it - 1);
                 tc_fence_after();
             }
 #pragma unroll 1
-            for (int k = 0; k < kManyKeys; ++k) {
+            for (int k = 0; k < F::STEP; ++k) {
                 if (!((odd[k >> 5] >> (k & 31)) & 1)) continue;
                 const uint32_t pw = tmem_ld1(t_s + k / 2);
                 tmem_wait_ld();
@@ -361,22 +373,23 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                 const float p = KIND == KIND_BF16 ? __bfloat162float(__ushort_as_bfloat16(p16))
                                                   : __half2float(__ushort_as_half(p16));
                 const bool at = key0 + k >= lo && key0 + k < hi;
-                const unsigned char* vt = st[k / F::VKEYS];
-                const int kr = k % F::VKEYS;
+                const int uk = half * F::STEP + k;   // key of the unit
+                const unsigned char* vt = st[uk / F::VKEYS];
+                const int kr = uk % F::VKEYS;
 #pragma unroll 1
                 for (int c = 0; c < F::OC / 16; ++c) {
                     uint32_t o[16];
                     tmem_ld16(t_o + c * 16, o);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int d = (F::NQ == 1 ? wg * 128 : 0) + c * 16 + i;
+                    for (int e = 0; e < 16; ++e) {
+                        const int d = (F::NQ == 1 ? wg * 128 : 0) + c * 16 + e;
                         const uint16_t v16 = *reinterpret_cast<const uint16_t*>(
                             vt + (d >> 6) * (F::VKEYS * 128) + sw128_offset(kr, (d >> 3) & 7) +
                             (d & 7) * 2);
                         if (at && odd16<KIND>(v16))
-                            o[i] = __float_as_uint(
-                                __uint_as_float(o[i]) +
+                            o[e] = __float_as_uint(
+                                __uint_as_float(o[e]) +
                                 p * (KIND == KIND_BF16 ? __bfloat162float(__ushort_as_bfloat16(v16))
                                                        : __half2float(__ushort_as_half(v16))));
                     }
@@ -386,13 +399,18 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                 tmem_wait_st();
             }
             bar_sync<2, 256>();
+            // this step's keys: rows of each 64-value slab
+            constexpr int KEYS = F::STEP / F::KPARTS;
 #pragma unroll
             for (int h = 0; h < F::KPARTS; ++h)
-                for (int i = tid; i < F::STAGEB / 2; i += 256) {
-                    uint16_t* v = reinterpret_cast<uint16_t*>(const_cast<unsigned char*>(st[h])) + i;
+                for (int e = tid; e < F::SLABS * KEYS * 64; e += 256) {
+                    const int sl = e / (KEYS * 64), rest = e % (KEYS * 64);
+                    const int row = (F::KPARTS == 1 ? half * F::STEP : 0) + rest / 64;
+                    uint16_t* v = reinterpret_cast<uint16_t*>(st[h] + sl * (F::VKEYS * 128) + row * 128) +
+                                  rest % 64;
                     if (odd16<KIND>(*v)) *v = 0;
                 }
-            if (tid < 4) odd[tid] = 0;
+            if (tid < F::STEP / 32) odd[tid] = 0;
             fence_async_smem();
             bar_sync<2, 256>();
         };
@@ -429,14 +447,15 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                 for (int c = 0; c < F::OC / 32; ++c) tmem_st32(t_o + c * 32, z);
                 tmem_wait_st();
             }
+            const int tw = F::NQ == 2 ? wg : 0;
 #pragma unroll 1
-            for (int j = 0; j < take; ++j, ++it) {
-                const int buf = F::NQ == 2 ? wg : (int)(it & 1);
-                const uint32_t ph = F::NQ == 2 ? it : it >> 1;
-                const uint32_t t_s = tmem + lanes + buf * 128;
-                await(&bars->s_full[buf], ph);
+            for (int i = 0; i < take * F::HS; ++i, ++it) {
+                const int j = i / F::HS, half = i % F::HS;
+                const int buf = (int)(it & 1);
+                const uint32_t t_s = tmem + lanes + (F::NQ == 2 ? wg * 128 + buf * 64 : buf * 128);
+                await(&bars->s_full[tw][buf], it >> 1);
                 tc_fence_after();
-                if (j == 0) {
+                if (i == 0) {
                     mul = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);   // 0: equal weights
                     if constexpr (QueryRows<DP, KIND, TQ>::CONVERT) mul /= fac[trow];
                 }
@@ -444,9 +463,9 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
 #pragma unroll
                 for (int c = 0; c < F::NC / 32; ++c) tmem_ld32(t_s + col0 + c * 32, sv + c * 32);
                 tmem_wait_ld();
-                const int key0 = (u0 + j) * kManyKeys;
-                const bool whole = key0 >= tile.all_lo && key0 + kManyKeys <= tile.all_hi;
-                if (key0 < warp_lo || key0 + kManyKeys > warp_hi) {
+                const int unit0 = (u0 + j) * kManyKeys, key0 = unit0 + half * F::STEP;
+                const bool whole = unit0 >= tile.all_lo && unit0 + kManyKeys <= tile.all_hi;
+                if (key0 < warp_lo || key0 + F::STEP > warp_hi) {
                     const int from = lo - key0 - col0, to = hi - key0 - col0;
 #pragma unroll
                     for (int c = 0; c < F::NC / 32; ++c) {   // bits of the attended columns
@@ -461,13 +480,11 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                 float t0 = __uint_as_float(sv[0]), t1 = __uint_as_float(sv[1]);
                 float t2 = __uint_as_float(sv[2]), t3 = __uint_as_float(sv[3]);
 #pragma unroll
-                for (int i = 4; i < F::NC; i += 8) {
-                    t0 = fmaxf(fmaxf(t0, __uint_as_float(sv[i])), __uint_as_float(sv[i + 1]));
-                    t1 = fmaxf(fmaxf(t1, __uint_as_float(sv[i + 2])), __uint_as_float(sv[i + 3]));
-                    if (i + 4 < F::NC) {
-                        t2 = fmaxf(fmaxf(t2, __uint_as_float(sv[i + 4])), __uint_as_float(sv[i + 5]));
-                        t3 = fmaxf(fmaxf(t3, __uint_as_float(sv[i + 6])), __uint_as_float(sv[i + 7]));
-                    }
+                for (int e = 4; e < F::NC; e += 4) {
+                    t0 = fmaxf(t0, __uint_as_float(sv[e]));
+                    t1 = fmaxf(t1, __uint_as_float(sv[e + 1]));
+                    t2 = fmaxf(t2, __uint_as_float(sv[e + 2]));
+                    t3 = fmaxf(t3, __uint_as_float(sv[e + 3]));
                 }
                 float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * mul;
                 if constexpr (F::NQ == 1) {
@@ -477,10 +494,10 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                     top = fmaxf(top, xm[(wg ^ 1) * 128 + row]);
                 }
                 const bool grow = top > m + kManyGrow || (m == -INFINITY && top > m);
-                if (__any_sync(0xffffffffu, grow && j > 0)) {
+                if (__any_sync(0xffffffffu, grow && i > 0)) {
                     const float f = grow ? ex2(m - top) : 1.f;
                     l *= f;
-                    await(&bars->pv_done[F::NQ == 2 ? wg : 0], it - 1);
+                    await(&bars->pv_done[tw], it - 1);
                     tc_fence_after();
 #pragma unroll 1
                     for (int c = 0; c < F::OC / 32; ++c) {
@@ -521,27 +538,29 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                     // such a unit and clear those that no row attends; if any
                     // that are left are not finite, they are added to the rows
                     // that attend them one by one and leave the stage.
-                    ++partial;
+                    if (half == 0) ++partial;
                     spin(&bars->checked[0], partial);
                     spin(&bars->checked[1], partial);
-                    volatile uint32_t* odd = bars->odd[partial & 7];
-                    if (odd[0] | odd[1] | odd[2] | odd[3])
-                        poisoned(odd, j, t_s, key0, lo, hi);
+                    volatile uint32_t* odd = bars->odd[partial & 7] + half * (F::STEP / 32);
+                    uint32_t any = 0;
+#pragma unroll
+                    for (int k = 0; k < F::STEP / 32; ++k) any |= odd[k];
+                    if (any) poisoned(odd, i, t_s, key0, lo, hi);
                 }
-                // One tile: S(j) comes before the value product of j - 1, so a
-                // fast warp could be two phases of pv_done ahead and mistake
-                // the last one it saw for the one it needs; products run in
-                // order, so waiting here costs nothing.
-                if (F::NQ == 1 && j > 0) await(&bars->pv_done[0], it - 1);
+                // The end waits for the last value product by its phase's
+                // parity.  S(i) only tells that product i - 2 is done: were
+                // i - 1 still running then, its phase would be taken for that
+                // of the last.
+                if (i > 0 && i == take * F::HS - 1) await(&bars->pv_done[tw], it - 1);
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bars->p_full[buf]);
+                if (lane == 0) mbar_arrive(&bars->p_full[tw][buf]);
             }
             // the next segment's queries are on their way while this one ends
             w.next(a);
             more = w.open(a);
             if (more) load_queries(w.s.n * a.group - w.cur.tile * F::M);
-            await(&bars->pv_done[F::NQ == 2 ? wg : 0], it - 1);
+            await(&bars->pv_done[tw], it - 1);
             tc_fence_after();
             if constexpr (F::NQ == 1) {   // both halves' sums
                 float* xl = xmax + (it & 1) * 256;
@@ -635,107 +654,92 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         }
         if (tid == 0) ws.rec[blockIdx.x] = rec;
     } else if (warp < 12) {
-        if constexpr (F::Q8)
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-        else
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        if (warp == 9 && lane == 0) {
+        if (warp == 9) {
             // ------------------------------------------------------- products
+            // The whole warp walks along and one elected lane issues: the
+            // products' operands are then known to be uniform and stay in
+            // uniform registers.  Issued by a lane that branched off alone,
+            // each took about 120 cycles, twice what a 128 x 128 x 16 product
+            // needs (256-row tiles of 128 values: 940 -> TF TFLOP/s).
             uint32_t it = 0, seg = 0;
             int stage0 = 0;
             auto wait_stage = [&](int n) {
                 await(&bars->full[n % F::NST], (uint32_t)(n / F::NST));
             };
-            auto free_stage = [&](int n) { umma_commit(&bars->empty[n % F::NST]); };
             // A descriptor's address field counts 16 bytes and no operand ends
             // beyond it, so the steps are additions to its low word.
+            const uint32_t t_mem = uniform(tmem);
             const uint64_t q_desc = umma_desc_sw128(smem_u32(sm));
             const uint64_t k_desc = umma_desc_sw128(smem_u32(sm + F::o_stage));
             const uint64_t v_desc = umma_desc_nmajor(smem_u32(sm + F::o_stage), F::VKEYS * 128);
-            auto slot_of = [&](int n) { return (uint64_t)((n % F::NST) * (F::STAGEB >> 4)); };
-            // S = Q K^T of one query tile with one stage of keys
-            auto score = [&](int tile, int part, uint32_t d, int n) {
-                const uint64_t q = q_desc + (tile * F::SLABS + part * F::KSLABS) * 1024;
-                const uint64_t k0 = k_desc + slot_of(n);
+            auto slot_of = [&](int n) { return uniform((n % F::NST) * (F::STAGEB >> 4)); };
+            auto free_at = [&](int n) { return &bars->empty[uniform(n % F::NST)]; };
+            // S = Q K^T of one query tile with `half` of a unit's keys, from
+            // their stages (parts by head dimension)
+            auto score = [&](int tile, int j, int half, uint32_t b) {
+                const uint32_t d = t_mem + uniform(F::NQ == 2 ? tile * 128 + b * 64 : b * 128);
 #pragma unroll
-                for (int sl = 0; sl < F::KSLABS; ++sl)
+                for (int h = 0; h < F::KPARTS; ++h) {
+                    const int n = stage0 + stage_k<F::NQ>(j) + h;
+                    if (tile == 0 && half == 0) wait_stage(n);
+                    const uint64_t q = q_desc + uniform((tile * F::SLABS + h * F::KSLABS) * 1024);
+                    const uint64_t k0 = k_desc + (slot_of(n) + uniform(half * (F::STEP * 8)));
+                    uint64_t* empty = free_at(n);
+                    uint64_t* ready = &bars->s_full[uniform(tile)][uniform(b)];
+                    tc_fence_after();
+                    if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        umma_f16(d, q + (sl * 1024 + k * 2), k0 + (sl * 1024 + k * 2), F::IDESC_S,
-                                 part > 0 || sl > 0 || k > 0);
+                        for (int sl = 0; sl < F::KSLABS; ++sl)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                umma_f16(d, q + (sl * 1024 + k * 2), k0 + (sl * 1024 + k * 2),
+                                         F::IDESC_S, h > 0 || sl > 0 || k > 0);
+                        if (tile == F::NQ - 1 && half == F::HS - 1) umma_commit(empty);
+                        if (h == F::KPARTS - 1) umma_commit(ready);
+                    }
+                    __syncwarp();
+                }
             };
-            // O += P V with one stage of values
-            auto value = [&](uint32_t d, uint32_t p, int n) {
-                const uint64_t v0 = v_desc + slot_of(n);
+            // O += P V with those keys' values, from their stages (parts by key)
+            auto value = [&](int tile, int j, int half, uint32_t b) {
+                const uint32_t p = t_mem + uniform(F::NQ == 2 ? tile * 128 + b * 64 : b * 128);
+                const uint32_t d = t_mem + 256 + uniform(tile * DP);
 #pragma unroll
-                for (int k = 0; k < F::VKEYS / 16; ++k)
-                    umma_f16_ts(d, p + k * 8, v0 + k * 128, F::IDESC_O);
+                for (int h = 0; h < F::KPARTS; ++h) {
+                    const int n = stage0 + stage_v<F::NQ>(j, w.take) + h;
+                    if (tile == 0 && half == 0) wait_stage(n);
+                    const uint64_t v0 = v_desc + (slot_of(n) + uniform(half * (F::STEP * 8)));
+                    uint64_t* empty = free_at(n);
+                    uint64_t* done = &bars->pv_done[uniform(tile)];
+                    tc_fence_after();
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < F::STEP / F::KPARTS / 16; ++k)
+                            umma_f16_ts(d, p + h * (F::VKEYS / 2) + k * 8, v0 + k * 128, F::IDESC_O);
+                        if (tile == F::NQ - 1 && half == F::HS - 1) umma_commit(empty);
+                        if (h == F::KPARTS - 1) umma_commit(done);
+                    }
+                    __syncwarp();
+                }
             };
             while (w.open(a)) {
                 const int take = w.take;
                 await(&bars->q_full[0], seg);
                 if constexpr (F::NQ == 2) await(&bars->q_full[1], seg);
                 tc_fence_after();
-                auto scores_of = [&](int j) {   // one tile: S(j) from its stages of keys
-                    const uint32_t b = (it + (j > 0)) & 1;
-#pragma unroll
-                    for (int h = 0; h < F::KPARTS; ++h) {
-                        const int n = stage0 + stage_k<F::NQ>(j) + h;
-                        wait_stage(n);
+                for (int t = 0; t < F::NQ; ++t) score(t, 0, 0, it & 1);
+                for (int i = 0; i < take * F::HS; ++i) {
+                    const uint32_t b = it & 1;
+                    if (i + 1 < take * F::HS)
+                        for (int t = 0; t < F::NQ; ++t)
+                            score(t, (i + 1) / F::HS, (i + 1) % F::HS, b ^ 1);
+                    for (int t = 0; t < F::NQ; ++t) {
+                        await(&bars->p_full[t][b], it >> 1);
                         tc_fence_after();
-                        score(0, h, tmem + b * 128, n);
-                        free_stage(n);
+                        value(t, i / F::HS, i % F::HS, b);
                     }
-                    umma_commit(&bars->s_full[b]);
-                };
-                if constexpr (F::NQ == 2) {
-                    const int n = stage0;
-                    wait_stage(n);
-                    tc_fence_after();
-                    for (int t = 0; t < 2; ++t) {
-                        score(t, 0, tmem + t * 128, n);
-                        umma_commit(&bars->s_full[t]);
-                    }
-                    free_stage(n);
-                } else {
-                    scores_of(0);
-                }
-                for (int j = 0; j < take; ++j) {
-                    if constexpr (F::NQ == 2) {
-                        const int nv = stage0 + stage_v<2>(j, take), nk = stage0 + stage_k<2>(j + 1);
-                        wait_stage(nv);
-                        for (int t = 0; t < 2; ++t) {
-                            await(&bars->p_full[t], it);
-                            tc_fence_after();
-                            value(tmem + 256 + t * DP, tmem + t * 128, nv);
-                            umma_commit(&bars->pv_done[t]);
-                            if (t == 1) free_stage(nv);
-                            if (j + 1 < take) {
-                                if (t == 0) {
-                                    wait_stage(nk);
-                                    tc_fence_after();
-                                }
-                                score(t, 0, tmem + t * 128, nk);
-                                umma_commit(&bars->s_full[t]);
-                                if (t == 1) free_stage(nk);
-                            }
-                        }
-                    } else {
-                        if (j + 1 < take) scores_of(j + 1);
-                        const uint32_t b = it & 1;
-                        await(&bars->p_full[b], it >> 1);
-                        tc_fence_after();
-#pragma unroll
-                        for (int h = 0; h < F::KPARTS; ++h) {
-                            const int n = stage0 + stage_v<1>(j, take) + h;
-                            wait_stage(n);
-                            tc_fence_after();
-                            value(tmem + 256, tmem + b * 128 + h * (F::VKEYS / 2), n);
-                            free_stage(n);
-                        }
-                        umma_commit(&bars->pv_done[0]);
-                    }
-                    *reinterpret_cast<volatile uint32_t*>(&bars->products) = ++it;
+                    ++it;
+                    if (lane == 0) *reinterpret_cast<volatile uint32_t*>(&bars->products) = it;
                 }
                 stage0 += 2 * F::KPARTS * take;
                 ++seg;
@@ -752,7 +756,7 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             uint32_t partial = 0, it = 0;
             while (w.open(a)) {
                 const AttendTile tile = attend_tile(a, w.s, w.cur.tile * F::M, F::M);
-                for (int j = 0; j < w.take; ++j, ++it) {
+                for (int j = 0; j < w.take; ++j, it += F::HS) {
                     const int key0 = (w.u0 + j) * kManyKeys;
                     if (key0 >= tile.all_lo && key0 + kManyKeys <= tile.all_hi) continue;
                     ++partial;
@@ -763,13 +767,24 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                         uint4* st = reinterpret_cast<uint4*>(sm + F::o_stage +
                                                              (n % F::NST) * F::STAGEB);
                         await(&bars->full[n % F::NST], (uint32_t)(n / F::NST));
-#pragma unroll 4
-                        for (int i = tid - 320; i < F::STAGEB / 16; i += 64) {
-                            const int k = h * F::VKEYS + (i >> 3) % F::VKEYS;
-                            if (key0 + k < tile.t_lo || key0 + k >= tile.t_hi)
-                                st[i] = make_uint4(0, 0, 0, 0);
-                            else if (odd16x8<KIND>(st[i]))
-                                atomicOr(&odd[k >> 5], 1u << (k & 31));
+                        // keys that every row attends are left alone: what
+                        // they hold belongs to all rows
+                        const int k0 = h * F::VKEYS;
+                        const int cut0 = min(max(tile.all_lo - key0 - k0, 0), F::VKEYS);
+                        const int cut1 = min(max(tile.all_hi - key0 - k0, cut0), F::VKEYS);
+                        const int n_keys = cut0 + F::VKEYS - cut1;
+                        constexpr int CPK = DP / 8;   // 16-byte chunks of a key
+#pragma unroll 8
+                        for (int i = tid - 320; i < n_keys * CPK; i += 64) {
+                            const int q = i / CPK, c = i % CPK;
+                            const int k = q < cut0 ? q : q - cut0 + cut1;
+                            uint4* at = st + (c >> 3) * (F::VKEYS * 8) + k * 8 + (c & 7);
+                            const int key = key0 + k0 + k;
+                            const uint4 v = *at;
+                            if (key < tile.t_lo || key >= tile.t_hi)
+                                *at = make_uint4(0, 0, 0, 0);
+                            else if (odd16x8<KIND>(v))
+                                atomicOr(&odd[(k0 + k) >> 5], 1u << ((k0 + k) & 31));
                         }
                     }
                     fence_async_smem();
@@ -834,7 +849,6 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         }
     } else if constexpr (F::Q8) {
         // ------------------------------------------------------ Q8_0 decoding
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         const int t = tid - 384, nb = a.c.dim >> 5;
         constexpr int CH = F::STAGEB / 32 / 128;   // 16-code chunks of a thread and stage
         constexpr int KC = F::KSLABS * 4;          // chunks of a row in a stage of keys
