@@ -5,9 +5,8 @@
 
 #include <mutex>
 
-#include "attend.h"
+#include "attend_mma.cuh"
 #include "launch.h"
-#include "sm100.cuh"
 
 namespace moeb200 {
 
@@ -203,19 +202,93 @@ bool attend_map(void* map, const KvCache& c, const void* base, int cols, int row
 
 namespace {
 
-// Tiles of many rows from 33 rows per sequence on average.
-bool use_many(const KvBatch& b, int group) { return (int64_t)b.T * group > 32 * (int64_t)b.B; }
+// A Q8_0 cache's pages of the batch's sequences as binary16 (scale * code
+// rounded once, what the kernels take them for), laid out by sequence.  Moves
+// 3 bytes a value; one block per page, 16 codes a thread.
+__global__ void __launch_bounds__(256) k_attend_expand(KvBatch b, KvCache c, __half* k, __half* v,
+                                                       int window, unsigned* status) {
+    const int seq = blockIdx.y, page = blockIdx.x;
+    const int len = __ldg(b.kv_lens + seq);
+    const int n = __ldg(b.q_start + seq + 1) - __ldg(b.q_start + seq);
+    const int first = page << c.page_shift;
+    // pages behind the sequence, or before the first row's window
+    if (first >= len || n <= 0) return;
+    if (window > 0 && first + c.page_size <= len - n - window + 1) return;
+    const int id = kv_page(b, c, seq, page, status);
+    if (id < 0) return;
+    const int units = (c.heads << c.page_shift) * c.dim >> 4;
+    const int64_t from = ((int64_t)id * c.heads << c.page_shift) * c.dim;
+    const int64_t to = (((int64_t)seq * b.max_pages + page) * c.heads << c.page_shift) * c.dim;
+#pragma unroll 2
+    for (int i = threadIdx.x; i < units; i += 256) {
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            const int64_t at = from + (int64_t)i * 16;
+            const uint4 codes = __ldcs(reinterpret_cast<const uint4*>(
+                static_cast<const int8_t*>(w ? c.v : c.k) + at));
+            const __half2 d = __half2half2((w ? c.vs : c.ks)[at >> 5]);
+            uint32_t x[8];
+            codes4(codes.x, d, x[0], x[1]);
+            codes4(codes.y, d, x[2], x[3]);
+            codes4(codes.z, d, x[4], x[5]);
+            codes4(codes.w, d, x[6], x[7]);
+            uint4* out = reinterpret_cast<uint4*>((w ? v : k) + to + (int64_t)i * 16);
+            out[0] = make_uint4(x[0], x[1], x[2], x[3]);
+            out[1] = make_uint4(x[4], x[5], x[6], x[7]);
+        }
+    }
+}
+
+// How a call runs.  Tiles of 16 rows up to 32 rows per sequence on average (a
+// tile reads the keys again), tiles of 128 or 256 beyond.  Those decode a Q8_0
+// cache's values as often as a sequence has tiles, on warps that the softmax
+// needs (chunks of 2048 rows over 8k keys, 32/8 heads x 128: 444 us, expanded
+// first 260 us); from two tiles on the pages are expanded to binary16 in the
+// workspace, if the table's width bounds that by 1 GB.
+struct AttendPlan {
+    bool many;
+    size_t base, plane;   // workspace of the kernel; bytes of an expanded plane, or 0
+    size_t bytes() const { return base + 2 * plane; }
+};
+
+AttendPlan attend_plan(const KvBatch& b, const KvCache& c, int group) {
+    const int dp = attend_dim(c.dim);
+    const int64_t rows = (int64_t)b.T * group;
+    AttendPlan p{};
+    p.many = rows > 32 * (int64_t)b.B;
+    p.base = align_up(p.many ? AttendWs::bytes(sm_count(), many_rows(dp), dp)
+                             : AttendWs::bytes(attend_few_ctas(), kFewRows, dp));
+    if (p.many && c.type == Q8_0 && rows > many_rows(dp) * (int64_t)b.B && b.max_pages > 0 &&
+        b.B <= 65535) {
+        const uint64_t values =
+            ((uint64_t)b.B * b.max_pages * c.heads << c.page_shift) * (uint64_t)c.dim;
+        if ((uint64_t)b.B * b.max_pages * c.heads <= 0x7fffffffull && values * 4 <= (1ull << 30))
+            p.plane = align_up((size_t)values * 2);
+    }
+    return p;
+}
 
 }  // namespace
 
 size_t attend_workspace_bytes(const KvBatch& b, const KvCache& c, int q_heads) {
-    const int dp = attend_dim(c.dim);
-    return use_many(b, q_heads / c.heads) ? AttendWs::bytes(sm_count(), many_rows(dp), dp)
-                                          : AttendWs::bytes(attend_few_ctas(), kFewRows, dp);
+    return attend_plan(b, c, q_heads / c.heads).bytes();
 }
 
 cudaError_t launch_attend(const AttendArgs& a, void* ws, cudaStream_t s) {
-    return use_many(a.b, a.group) ? launch_attend_many(a, ws, s) : launch_attend_few(a, ws, s);
+    const AttendPlan p = attend_plan(a.b, a.c, a.group);
+    if (!p.many) return launch_attend_few(a, ws, s);
+    if (!p.plane) return launch_attend_many(a, ws, s);
+    AttendArgs x = a;
+    x.c.type = KV_F16;
+    x.c.k = static_cast<char*>(ws) + p.base;
+    x.c.v = static_cast<char*>(ws) + p.base + p.plane;
+    x.c.ks = x.c.vs = nullptr;
+    x.c.pages = a.b.B * a.b.max_pages;
+    x.b.table = nullptr;
+    k_attend_expand<<<dim3(a.b.max_pages, a.b.B), 256, 0, s>>>(
+        a.b, a.c, static_cast<__half*>(x.c.k), static_cast<__half*>(x.c.v), a.window, a.status);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? launch_attend_many(x, ws, s) : e;
 }
 
 }  // namespace moeb200

@@ -50,9 +50,6 @@ struct Many {
     static constexpr int STAGEB = KSLABS * kManyKeys * 128;
     static constexpr int QB = NQ * SLABS * 128 * 128;
     static constexpr int NST = DP == 64 ? 8 : 5;
-    static constexpr int STEP = NQ == 2 ? 64 : 128;      // keys of a score tile
-    static constexpr int HS = kManyKeys / STEP;          // score tiles of a unit
-    static constexpr int NC = 64;                        // score columns of a thread
     static constexpr int OC = NQ == 2 ? DP : DP / 2;     // output columns of a thread
     static constexpr int THREADS = Q8 ? 512 : 384;
     // binary16 probabilities: 2^7 of the maximum in use, at most 2^15
@@ -63,16 +60,16 @@ struct Many {
     static constexpr int o_max = o_fac + M * 4;          // maxima and sums of half rows
     static constexpr int smem = o_max + (NQ == 1 ? 2048 : 0);
     static_assert(smem <= 232448, "shared memory of a CTA");
-    static constexpr uint32_t IDESC_S = umma_idesc_f16(128, STEP) |
+    static constexpr uint32_t IDESC_S = umma_idesc_f16(128, kManyKeys) |
                                         (KIND == KIND_BF16 ? (1u << 7) | (1u << 10) : 0u);
     static constexpr uint32_t IDESC_O = umma_idesc_f16(128, DP) | (1u << 16) |   // B: N-major
                                         (KIND == KIND_BF16 ? (1u << 7) | (1u << 10) : 0u);
 };
 
 struct ManyBars {
-    uint64_t full[8], empty[8], s_full[2][2], p_full[2][2], pv_done[2], q_full[2];
+    uint64_t full[8], empty[8], s_full[2], p_full[2][2], pv_done[2], q_full[2];
     uint32_t tmem, lost;
-    uint32_t products;     // score tiles whose value products have been issued
+    uint32_t products;     // units whose value products have been issued
     uint32_t checked[2];   // partly attended units that each checking warp is done with
     uint32_t odd[8][4];    // such units in turn: keys whose values are not all finite
 };
@@ -96,6 +93,8 @@ __device__ __forceinline__ uint64_t umma_desc_nmajor(uint32_t saddr, uint32_t sl
            ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
+// Two multiply-adds, two additions in one issue slot (of the softmax warps,
+// that have no other to spare: 3% of a chunk's time against plain ones).
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     float2 d;
     asm("fma.rn.f32x2 %0, %1, %2, %3;"
@@ -191,12 +190,12 @@ __device__ __forceinline__ int stage_v(int j, int take) {
 }
 
 // Queries of this warp's rows of a tile into the swizzled operand layout.
-// TQ values are copied as they are (cp.async); or, for bfloat16 over Q8_0 and
+// TQ values are copied as they are (cp.async); or, for bfloat16 over Q8_0 values and
 // for negative scales, through registers: scaled to binary16, sign flipped.
 template <int DP, int KIND, typename TQ>
 struct QueryRows {
     using F = Many<DP, KIND>;
-    static constexpr bool CONVERT = F::Q8 && std::is_same<TQ, __nv_bfloat16>::value;
+    static constexpr bool CONVERT = KIND != KIND_BF16 && std::is_same<TQ, __nv_bfloat16>::value;
     static constexpr int LPR = DP / 8;        // lanes of a row, 16 bytes each
     static constexpr int RPI = 32 / LPR;      // rows of an iteration
     static constexpr int BATCH = 4;
@@ -277,10 +276,8 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             mbar_init(&bars->empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
-            for (int b = 0; b < 2; ++b) {
-                mbar_init(&bars->s_full[i][b], 1);
-                mbar_init(&bars->p_full[i][b], F::NQ == 2 ? 4 : 8);
-            }
+            mbar_init(&bars->s_full[i], 1);
+            for (int h = 0; h < 2; ++h) mbar_init(&bars->p_full[i][h], 4);
             mbar_init(&bars->pv_done[i], 1);
             mbar_init(&bars->q_full[i], F::NQ == 2 ? 4 : 8);
         }
@@ -327,14 +324,14 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         const int row = quarter * 32 + lane;                       // of the 128-row tile
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;     // TMEM lane offset
         const int trow = F::NQ == 2 ? wg * 128 + row : row;        // of the CTA's rows
-        const int col0 = F::NQ == 2 ? 0 : wg * 64;                 // first score column
         const uint32_t t_o = tmem + lanes + 256 + (F::NQ == 2 ? wg * DP : wg * 128);
         const int q0 = F::NQ == 2 ? wg * 128 + quarter * 32 : quarter * 32 + wg * 16;
         constexpr int QN = F::NQ == 2 ? 32 : 16;                   // query rows the warp loads
+        const int tw = F::NQ == 2 ? wg : 0;                        // query tile
         float* xmax = reinterpret_cast<float*>(sm + F::o_max);     // [2][2][128]
         AttendRecord rec{};
-        uint32_t it = 0;       // score tiles done by the CTA
-        uint32_t partial = 0;  // units met that not all rows attend
+        uint32_t it = 0;       // units done by the CTA
+        uint32_t partial = 0;  // of them, those that not all rows attend
         int stage0 = 0;        // ring stages before this segment
 
         auto load_queries = [&](int n_valid) {
@@ -347,9 +344,7 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             if (lane == 0) mbar_arrive(&bars->q_full[F::NQ == 2 ? wg : 0]);
         };
         // The unit's odd values: all eight warps meet here.
-        auto poisoned = [&](volatile uint32_t* odd, int i, uint32_t t_s, int key0, int lo, int hi) {
-            const int j = i / F::HS, half = i % F::HS;
-            const int tw = F::NQ == 2 ? wg : 0;
+        auto poisoned = [&](volatile uint32_t* odd, int j, uint32_t t_s, int key0, int lo, int hi) {
             unsigned char* st[F::KPARTS];
 #pragma unroll
             for (int h = 0; h < F::KPARTS; ++h) {
@@ -360,22 +355,21 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             tc_fence_before();
             bar_sync<2, 256>();   // with one tile, O takes both halves' probabilities
             tc_fence_after();
-            if (i > 0) {
+            if (j > 0) {
                 await(&bars->pv_done[tw], it - 1);
                 tc_fence_after();
             }
 #pragma unroll 1
-            for (int k = 0; k < F::STEP; ++k) {
+            for (int k = 0; k < kManyKeys; ++k) {
                 if (!((odd[k >> 5] >> (k & 31)) & 1)) continue;
-                const uint32_t pw = tmem_ld1(t_s + k / 2);
+                const uint32_t pw = tmem_ld1(t_s + (k >> 6) * 64 + (k & 63) / 2);
                 tmem_wait_ld();
                 const uint16_t p16 = (uint16_t)(k & 1 ? pw >> 16 : pw);
                 const float p = KIND == KIND_BF16 ? __bfloat162float(__ushort_as_bfloat16(p16))
                                                   : __half2float(__ushort_as_half(p16));
                 const bool at = key0 + k >= lo && key0 + k < hi;
-                const int uk = half * F::STEP + k;   // key of the unit
-                const unsigned char* vt = st[uk / F::VKEYS];
-                const int kr = uk % F::VKEYS;
+                const unsigned char* vt = st[k / F::VKEYS];
+                const int kr = k % F::VKEYS;
 #pragma unroll 1
                 for (int c = 0; c < F::OC / 16; ++c) {
                     uint32_t o[16];
@@ -399,18 +393,13 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                 tmem_wait_st();
             }
             bar_sync<2, 256>();
-            // this step's keys: rows of each 64-value slab
-            constexpr int KEYS = F::STEP / F::KPARTS;
 #pragma unroll
             for (int h = 0; h < F::KPARTS; ++h)
-                for (int e = tid; e < F::SLABS * KEYS * 64; e += 256) {
-                    const int sl = e / (KEYS * 64), rest = e % (KEYS * 64);
-                    const int row = (F::KPARTS == 1 ? half * F::STEP : 0) + rest / 64;
-                    uint16_t* v = reinterpret_cast<uint16_t*>(st[h] + sl * (F::VKEYS * 128) + row * 128) +
-                                  rest % 64;
+                for (int i = tid; i < F::STAGEB / 2; i += 256) {
+                    uint16_t* v = reinterpret_cast<uint16_t*>(st[h]) + i;
                     if (odd16<KIND>(*v)) *v = 0;
                 }
-            if (tid < F::STEP / 32) odd[tid] = 0;
+            if (tid < 4) odd[tid] = 0;
             fence_async_smem();
             bar_sync<2, 256>();
         };
@@ -447,45 +436,64 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                 for (int c = 0; c < F::OC / 32; ++c) tmem_st32(t_o + c * 32, z);
                 tmem_wait_st();
             }
-            const int tw = F::NQ == 2 ? wg : 0;
 #pragma unroll 1
-            for (int i = 0; i < take * F::HS; ++i, ++it) {
-                const int j = i / F::HS, half = i % F::HS;
-                const int buf = (int)(it & 1);
-                const uint32_t t_s = tmem + lanes + (F::NQ == 2 ? wg * 128 + buf * 64 : buf * 128);
-                await(&bars->s_full[tw][buf], it >> 1);
+            for (int j = 0; j < take; ++j, ++it) {
+                const int buf = F::NQ == 2 ? wg : (int)(it & 1);
+                const uint32_t ph = F::NQ == 2 ? it : it >> 1;
+                const uint32_t t_s = tmem + lanes + buf * 128;
+                await(&bars->s_full[buf], ph);
                 tc_fence_after();
-                if (i == 0) {
+                if (j == 0) {
                     mul = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);   // 0: equal weights
                     if constexpr (QueryRows<DP, KIND, TQ>::CONVERT) mul /= fac[trow];
                 }
-                uint32_t sv[F::NC];
+                const int key0 = (u0 + j) * kManyKeys;
+                const bool whole = key0 >= tile.all_lo && key0 + kManyKeys <= tile.all_hi;
+                const bool masked = key0 < warp_lo || key0 + kManyKeys > warp_hi;
+                // 32 score columns; those the row does not attend to -infinity
+                auto mask = [&](uint32_t* v, int col) {
+                    const int f = min(max(lo - key0 - col, 0), 32);
+                    const int t = min(max(hi - key0 - col, 0), 32);
+                    const uint32_t keep = (uint32_t)(((1ull << t) - 1) & ~((1ull << f) - 1));
 #pragma unroll
-                for (int c = 0; c < F::NC / 32; ++c) tmem_ld32(t_s + col0 + c * 32, sv + c * 32);
-                tmem_wait_ld();
-                const int unit0 = (u0 + j) * kManyKeys, key0 = unit0 + half * F::STEP;
-                const bool whole = unit0 >= tile.all_lo && unit0 + kManyKeys <= tile.all_hi;
-                if (key0 < warp_lo || key0 + F::STEP > warp_hi) {
-                    const int from = lo - key0 - col0, to = hi - key0 - col0;
+                    for (int i = 0; i < 32; ++i)
+                        if (!(keep >> i & 1)) v[i] = 0xff800000u;
+                };
+                float t0 = -INFINITY, t1 = t0, t2 = t0, t3 = t0;
+                auto highest = [&](const uint32_t* v) {
 #pragma unroll
-                    for (int c = 0; c < F::NC / 32; ++c) {   // bits of the attended columns
-                        const int f = min(max(from - c * 32, 0), 32), t = min(max(to - c * 32, 0), 32);
-                        const uint32_t keep =
-                            (uint32_t)(((1ull << t) - 1) & ~((1ull << f) - 1));
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (!(keep >> i & 1)) sv[c * 32 + i] = 0xff800000u;   // -infinity
+                    for (int i = 0; i < 32; i += 8) {
+                        t0 = fmaxf(fmaxf(t0, __uint_as_float(v[i])), __uint_as_float(v[i + 1]));
+                        t1 = fmaxf(fmaxf(t1, __uint_as_float(v[i + 2])), __uint_as_float(v[i + 3]));
+                        t2 = fmaxf(fmaxf(t2, __uint_as_float(v[i + 4])), __uint_as_float(v[i + 5]));
+                        t3 = fmaxf(fmaxf(t3, __uint_as_float(v[i + 6])), __uint_as_float(v[i + 7]));
                     }
+                };
+                // A thread of the two-tile form reads its 128 scores in two
+                // halves of 64 and, having the maximum, takes the second half
+                // from registers and the first one from tensor memory again.
+                uint32_t va[32], vb[32];
+                if constexpr (F::NQ == 2) {
+                    tmem_ld32(t_s, va);
+                    tmem_ld32(t_s + 32, vb);
+                    tmem_wait_ld();
+                    if (masked) {
+                        mask(va, 0);
+                        mask(vb, 32);
+                    }
+                    highest(va);
+                    highest(vb);
                 }
-                float t0 = __uint_as_float(sv[0]), t1 = __uint_as_float(sv[1]);
-                float t2 = __uint_as_float(sv[2]), t3 = __uint_as_float(sv[3]);
-#pragma unroll
-                for (int e = 4; e < F::NC; e += 4) {
-                    t0 = fmaxf(t0, __uint_as_float(sv[e]));
-                    t1 = fmaxf(t1, __uint_as_float(sv[e + 1]));
-                    t2 = fmaxf(t2, __uint_as_float(sv[e + 2]));
-                    t3 = fmaxf(t3, __uint_as_float(sv[e + 3]));
+                const int last = F::NQ == 2 ? 64 : wg * 64;
+                tmem_ld32(t_s + last, va);
+                tmem_ld32(t_s + last + 32, vb);
+                tmem_wait_ld();
+                if (masked) {
+                    mask(va, last);
+                    mask(vb, last + 32);
                 }
+                highest(va);
+                highest(vb);
                 float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * mul;
                 if constexpr (F::NQ == 1) {
                     float* xm = xmax + (it & 1) * 256;
@@ -494,67 +502,82 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                     top = fmaxf(top, xm[(wg ^ 1) * 128 + row]);
                 }
                 const bool grow = top > m + kManyGrow || (m == -INFINITY && top > m);
-                if (__any_sync(0xffffffffu, grow && i > 0)) {
+                if (__any_sync(0xffffffffu, grow && j > 0)) {
                     const float f = grow ? ex2(m - top) : 1.f;
                     l *= f;
                     await(&bars->pv_done[tw], it - 1);
                     tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < F::OC / 32; ++c) {
-                        uint32_t o[32];
-                        tmem_ld32(t_o + c * 32, o);
+                    for (int c = 0; c < F::OC / 16; ++c) {
+                        uint32_t o[16];
+                        tmem_ld16(t_o + c * 16, o);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                        tmem_st32(t_o + c * 32, o);
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tmem_st16(t_o + c * 16, o);
                     }
                     tmem_wait_st();
                 }
                 if (grow) m = top;
                 const float base = m == -INFINITY ? 0.f : m - F::SHIFT;
-                const float2 mul2 = make_float2(mul, mul), base2 = make_float2(-base, -base);
+                const float2 scale2 = make_float2(mul, mul), base2 = make_float2(-base, -base);
                 float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
-#pragma unroll
-                for (int c = 0; c < F::NC / 32; ++c) {
+                // 32 scores to probabilities, in 16 columns at `at`
+                auto weigh = [&](const uint32_t* v, uint32_t at) {
                     uint32_t pk[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        float2 v = make_float2(__uint_as_float(sv[c * 32 + 2 * i]),
-                                               __uint_as_float(sv[c * 32 + 2 * i + 1]));
-                        v = fma2(v, mul2, base2);
-                        v.x = ex2(v.x);
-                        v.y = ex2(v.y);
-                        if (i & 1) sum1 = add2(sum1, v); else sum0 = add2(sum0, v);
-                        pk[i] = pack16<KIND>(v.x, v.y);
+                        float2 x = fma2(make_float2(__uint_as_float(v[2 * i]),
+                                                    __uint_as_float(v[2 * i + 1])), scale2, base2);
+                        x.x = ex2(x.x);
+                        x.y = ex2(x.y);
+                        if (i & 1) sum1 = add2(sum1, x); else sum0 = add2(sum0, x);
+                        pk[i] = pack16<KIND>(x.x, x.y);
                     }
-                    tmem_st16(t_s + col0 / 2 + c * 16, pk);
+                    tmem_st16(at, pk);
+                };
+                auto hand_over = [&](int half) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars->p_full[buf][half]);
+                };
+                weigh(va, t_s + last);
+                if constexpr (F::NQ == 2) tmem_ld32(t_s, va);
+                weigh(vb, t_s + last + 16);
+                if constexpr (F::NQ == 2) tmem_ld32(t_s + 32, vb);
+                tmem_wait_st();
+                if constexpr (F::NQ == 2) {
+                    if (whole) hand_over(1);
+                    tmem_wait_ld();
+                    if (masked) {
+                        mask(va, 0);
+                        mask(vb, 32);
+                    }
+                    weigh(va, t_s);
+                    weigh(vb, t_s + 16);
+                    tmem_wait_st();
                 }
                 sum0 = add2(sum0, sum1);
                 l += sum0.x + sum0.y;
-                tmem_wait_st();
                 if (!whole) {
                     // A key that only some rows attend, or none: 0 * NaN would
                     // reach the others.  Two warps look through the values of
                     // such a unit and clear those that no row attends; if any
                     // that are left are not finite, they are added to the rows
                     // that attend them one by one and leave the stage.
-                    if (half == 0) ++partial;
+                    ++partial;
                     spin(&bars->checked[0], partial);
                     spin(&bars->checked[1], partial);
-                    volatile uint32_t* odd = bars->odd[partial & 7] + half * (F::STEP / 32);
-                    uint32_t any = 0;
-#pragma unroll
-                    for (int k = 0; k < F::STEP / 32; ++k) any |= odd[k];
-                    if (any) poisoned(odd, i, t_s, key0, lo, hi);
+                    volatile uint32_t* odd = bars->odd[partial & 7];
+                    if (odd[0] | odd[1] | odd[2] | odd[3]) poisoned(odd, j, t_s, key0, lo, hi);
+                    if (F::NQ == 2) hand_over(1);
                 }
-                // The end waits for the last value product by its phase's
-                // parity.  S(i) only tells that product i - 2 is done: were
-                // i - 1 still running then, its phase would be taken for that
-                // of the last.
-                if (i > 0 && i == take * F::HS - 1) await(&bars->pv_done[tw], it - 1);
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars->p_full[tw][buf]);
+                // One tile: the end waits for the last value product by its
+                // phase's parity.  S(j) only tells that product j - 2 is done:
+                // were j - 1 still running then, its phase would be taken for
+                // that of the last.
+                if (F::NQ == 1 && j > 0 && j == take - 1) await(&bars->pv_done[0], it - 1);
+                hand_over(F::NQ == 2 ? 0 : wg);
             }
             // the next segment's queries are on their way while this one ends
             w.next(a);
@@ -674,18 +697,18 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             const uint64_t v_desc = umma_desc_nmajor(smem_u32(sm + F::o_stage), F::VKEYS * 128);
             auto slot_of = [&](int n) { return uniform((n % F::NST) * (F::STAGEB >> 4)); };
             auto free_at = [&](int n) { return &bars->empty[uniform(n % F::NST)]; };
-            // S = Q K^T of one query tile with `half` of a unit's keys, from
-            // their stages (parts by head dimension)
-            auto score = [&](int tile, int j, int half, uint32_t b) {
-                const uint32_t d = t_mem + uniform(F::NQ == 2 ? tile * 128 + b * 64 : b * 128);
+            // S = Q K^T of one query tile with a unit's keys, from their stages
+            // (parts by head dimension), into score buffer b
+            auto score = [&](int tile, int j, uint32_t b) {
+                const uint32_t d = t_mem + uniform(b * 128);
 #pragma unroll
                 for (int h = 0; h < F::KPARTS; ++h) {
                     const int n = stage0 + stage_k<F::NQ>(j) + h;
-                    if (tile == 0 && half == 0) wait_stage(n);
+                    if (tile == 0) wait_stage(n);
                     const uint64_t q = q_desc + uniform((tile * F::SLABS + h * F::KSLABS) * 1024);
-                    const uint64_t k0 = k_desc + (slot_of(n) + uniform(half * (F::STEP * 8)));
+                    const uint64_t k0 = k_desc + slot_of(n);
                     uint64_t* empty = free_at(n);
-                    uint64_t* ready = &bars->s_full[uniform(tile)][uniform(b)];
+                    uint64_t* ready = &bars->s_full[uniform(b)];
                     tc_fence_after();
                     if (elect_one()) {
 #pragma unroll
@@ -694,30 +717,33 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                             for (int k = 0; k < 4; ++k)
                                 umma_f16(d, q + (sl * 1024 + k * 2), k0 + (sl * 1024 + k * 2),
                                          F::IDESC_S, h > 0 || sl > 0 || k > 0);
-                        if (tile == F::NQ - 1 && half == F::HS - 1) umma_commit(empty);
+                        if (tile == F::NQ - 1) umma_commit(empty);
                         if (h == F::KPARTS - 1) umma_commit(ready);
                     }
                     __syncwarp();
                 }
             };
-            // O += P V with those keys' values, from their stages (parts by key)
-            auto value = [&](int tile, int j, int half, uint32_t b) {
-                const uint32_t p = t_mem + uniform(F::NQ == 2 ? tile * 128 + b * 64 : b * 128);
+            // O += P V, half a unit's keys at a time as their probabilities come
+            // (two tiles: the second half first)
+            auto value = [&](int tile, int j, uint32_t b) {
+                const uint32_t p = t_mem + uniform(b * 128);
                 const uint32_t d = t_mem + 256 + uniform(tile * DP);
 #pragma unroll
-                for (int h = 0; h < F::KPARTS; ++h) {
-                    const int n = stage0 + stage_v<F::NQ>(j, w.take) + h;
-                    if (tile == 0 && half == 0) wait_stage(n);
-                    const uint64_t v0 = v_desc + (slot_of(n) + uniform(half * (F::STEP * 8)));
+                for (int i = 0; i < 2; ++i) {
+                    const int h = F::NQ == 2 ? 1 - i : i;
+                    const int n = stage0 + stage_v<F::NQ>(j, w.take) + (F::NQ == 2 ? 0 : h);
+                    if (F::NQ == 1 || (tile == 0 && i == 0)) wait_stage(n);
+                    const uint64_t v0 = v_desc + slot_of(n) + (F::NQ == 2 ? h * 512 : 0);
                     uint64_t* empty = free_at(n);
                     uint64_t* done = &bars->pv_done[uniform(tile)];
+                    await(&bars->p_full[b][h], F::NQ == 2 ? it : it >> 1);
                     tc_fence_after();
                     if (elect_one()) {
 #pragma unroll
-                        for (int k = 0; k < F::STEP / F::KPARTS / 16; ++k)
-                            umma_f16_ts(d, p + h * (F::VKEYS / 2) + k * 8, v0 + k * 128, F::IDESC_O);
-                        if (tile == F::NQ - 1 && half == F::HS - 1) umma_commit(empty);
-                        if (h == F::KPARTS - 1) umma_commit(done);
+                        for (int k = 0; k < 4; ++k)
+                            umma_f16_ts(d, p + h * 64 + k * 8, v0 + k * 128, F::IDESC_O);
+                        if (F::NQ == 1 || (tile == 1 && i == 1)) umma_commit(empty);
+                        if (i == 1) umma_commit(done);
                     }
                     __syncwarp();
                 }
@@ -725,18 +751,22 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             while (w.open(a)) {
                 const int take = w.take;
                 await(&bars->q_full[0], seg);
-                if constexpr (F::NQ == 2) await(&bars->q_full[1], seg);
-                tc_fence_after();
-                for (int t = 0; t < F::NQ; ++t) score(t, 0, 0, it & 1);
-                for (int i = 0; i < take * F::HS; ++i) {
-                    const uint32_t b = it & 1;
-                    if (i + 1 < take * F::HS)
-                        for (int t = 0; t < F::NQ; ++t)
-                            score(t, (i + 1) / F::HS, (i + 1) % F::HS, b ^ 1);
-                    for (int t = 0; t < F::NQ; ++t) {
-                        await(&bars->p_full[t][b], it >> 1);
-                        tc_fence_after();
-                        value(t, i / F::HS, i % F::HS, b);
+                if constexpr (F::NQ == 2) {
+                    score(0, 0, 0);
+                    await(&bars->q_full[1], seg);
+                    score(1, 0, 1);
+                } else {
+                    score(0, 0, it & 1);
+                }
+                for (int j = 0; j < take; ++j) {
+                    if constexpr (F::NQ == 2) {
+                        for (int t = 0; t < 2; ++t) {
+                            value(t, j, t);
+                            if (j + 1 < take) score(t, j + 1, t);
+                        }
+                    } else {
+                        if (j + 1 < take) score(0, j + 1, (it + 1) & 1);
+                        value(0, j, it & 1);
                     }
                     ++it;
                     if (lane == 0) *reinterpret_cast<volatile uint32_t*>(&bars->products) = it;
@@ -756,7 +786,7 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             uint32_t partial = 0, it = 0;
             while (w.open(a)) {
                 const AttendTile tile = attend_tile(a, w.s, w.cur.tile * F::M, F::M);
-                for (int j = 0; j < w.take; ++j, it += F::HS) {
+                for (int j = 0; j < w.take; ++j, ++it) {
                     const int key0 = (w.u0 + j) * kManyKeys;
                     if (key0 >= tile.all_lo && key0 + kManyKeys <= tile.all_hi) continue;
                     ++partial;
@@ -977,7 +1007,9 @@ cudaError_t launch_many(const AttendArgs& a, void* ws, cudaStream_t s) {
 
 template <int DP>
 cudaError_t launch_dim(const AttendArgs& a, void* ws, cudaStream_t s) {
-    if (a.c.type == KV_F16) return launch_many<DP, KIND_F16, __half>(a, ws, s);
+    if (a.c.type == KV_F16)   // bfloat16 queries: over the expanded form of a Q8_0 cache
+        return a.type == KV_F16 ? launch_many<DP, KIND_F16, __half>(a, ws, s)
+                                : launch_many<DP, KIND_F16, __nv_bfloat16>(a, ws, s);
     if (a.c.type == KV_BF16) return launch_many<DP, KIND_BF16, __nv_bfloat16>(a, ws, s);
     if (a.type == KV_F16) return launch_many<DP, KIND_Q8, __half>(a, ws, s);
     return launch_many<DP, KIND_Q8, __nv_bfloat16>(a, ws, s);

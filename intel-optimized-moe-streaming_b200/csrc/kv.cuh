@@ -28,7 +28,8 @@ constexpr int kKvBlock = 32;
 struct KvBatch {
     const int32_t* q_start;   // [B + 1] first row of each sequence
     const int32_t* kv_lens;   // [B] cached tokens, the new ones included
-    const int32_t* table;     // [B][max_pages], row stride table_stride
+    const int32_t* table;     // [B][max_pages], row stride table_stride; null: page p of
+                              // sequence b is b * max_pages + p
     int64_t table_stride;
     int B, T, max_pages;
 };
@@ -83,7 +84,8 @@ __device__ __forceinline__ int kv_page(const KvBatch& b, const KvCache& c, int s
         kv_flag(status, KV_BAD_LENGTH);
         return -1;
     }
-    const int id = __ldg(b.table + (int64_t)seq * b.table_stride + page);
+    const int id = b.table ? __ldg(b.table + (int64_t)seq * b.table_stride + page)
+                           : seq * b.max_pages + page;
     if (id < 0 || id >= c.pages) {
         kv_flag(status, KV_BAD_PAGE);
         return -1;
