@@ -208,17 +208,19 @@ struct QueryRows {
         const bool in_dim = ch * 8 < a.c.dim;
         const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
         const bool copy = !CONVERT && flip == 0;
+        // lane i: where row row0 + i of the tile starts
+        const int mine = w.cur.tile * F::M + row0 + lane;
+        const int tok = a.by_group.div(mine);
+        const int64_t start = (int64_t)(w.s.q0 + tok) * a.q_ts +
+                              (int64_t)(w.cur.kvh * a.group + mine - tok * a.group) * a.q_hs;
         for (int i0 = 0; i0 < n_rows; i0 += RPI * BATCH) {
             uint4 x[BATCH];
 #pragma unroll
             for (int b = 0; b < BATCH; ++b) {
-                const int r = row0 + i0 + b * RPI + sub;
+                const int i = i0 + b * RPI + sub, r = row0 + i;
                 const bool ok = in_dim && r < valid;
-                const int rr = w.cur.tile * F::M + (ok ? r : 0);
-                const int tok = a.by_group.div(rr);
-                const TQ* q = static_cast<const TQ*>(a.q) + (int64_t)(w.s.q0 + tok) * a.q_ts +
-                              (int64_t)(w.cur.kvh * a.group + rr - tok * a.group) * a.q_hs +
-                              (ok ? ch * 8 : 0);
+                const int64_t at = __shfl_sync(0xffffffffu, start, i);
+                const TQ* q = static_cast<const TQ*>(a.q) + (ok ? at + ch * 8 : 0);
                 if (copy) {
                     const int t = r & 127;
                     cp_async16(smem_u32(tile + (r >> 7) * (F::SLABS * 16384) + (ch >> 3) * 16384) +
@@ -624,7 +626,7 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                     __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(orow), from));
                 qvalid[i] = __shfl_sync(0xffffffffu, (int)valid, from);
             }
-#pragma unroll 1
+#pragma unroll 2
             for (int c = 0; c < F::OC / 32; ++c) {
                 uint32_t o[32];
                 __syncwarp();
@@ -779,9 +781,9 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
         } else if (warp >= 10) {
             // --------------------------- values of partly attended units
             // Units are skipped, so a stage's barrier may be phases behind: a unit
-            // is looked at once the value products of those before it were
-            // issued (their stages, the previous uses of its own, were full),
-            // and its own cannot be issued before it has been.
+            // is looked at once the value products were issued that come behind
+            // the previous use of its stage (which was full, then), and its own
+            // cannot be issued before it has been.
             int stage0 = 0;
             uint32_t partial = 0, it = 0;
             while (w.open(a)) {
@@ -790,7 +792,11 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                     const int key0 = (w.u0 + j) * kManyKeys;
                     if (key0 >= tile.all_lo && key0 + kManyKeys <= tile.all_hi) continue;
                     ++partial;
-                    spin(&bars->products, it);
+                    // two tiles: the stage's last use was as keys two units ago
+                    if (F::NQ == 1)
+                        spin(&bars->products, it);
+                    else if (it > 0)
+                        spin(&bars->products, it - 1);
                     uint32_t* odd = bars->odd[partial & 7];
                     for (int h = 0; h < F::KPARTS; ++h) {
                         const int n = stage0 + stage_v<F::NQ>(j, w.take) + h;
