@@ -701,8 +701,14 @@ cudaError_t launch_few(const AttendArgs& a, void* ws, cudaStream_t s) {
     if (!attend_map(&kmap, a.c, a.c.k, F::SLABB / F::EB, box) ||
         !attend_map(&vmap, a.c, a.c.v, F::SLABB / F::EB, box))
         return cudaErrorInvalidValue;
-    cudaError_t e = cudaFuncSetAttribute(k_attend_few<DP, KIND, TQ>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, F::smem);
+    static bool raised[64] = {};   // shared memory limit, per device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev < 0 || dev >= 64 || !raised[dev])) {
+        e = cudaFuncSetAttribute(k_attend_few<DP, KIND, TQ>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 F::smem);
+        if (e == cudaSuccess && dev >= 0 && dev < 64) raised[dev] = true;
+    }
     if (e != cudaSuccess) return e;
     k_attend_few<DP, KIND, TQ><<<attend_few_ctas(), kFewThreads, F::smem, s>>>(kmap, vmap, a, ws);
     e = cudaGetLastError();

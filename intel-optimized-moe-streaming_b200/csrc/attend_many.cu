@@ -1002,8 +1002,14 @@ cudaError_t launch_many(const AttendArgs& a, void* ws, cudaStream_t s) {
             !attend_map(&vmap, a.c, a.c.v, 64, piece < F::VKEYS ? piece : F::VKEYS))
             return cudaErrorInvalidValue;
     }
-    cudaError_t e = cudaFuncSetAttribute(k_attend_many<DP, KIND, TQ>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, F::smem);
+    static bool raised[64] = {};   // shared memory limit, per device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev < 0 || dev >= 64 || !raised[dev])) {
+        e = cudaFuncSetAttribute(k_attend_many<DP, KIND, TQ>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 F::smem);
+        if (e == cudaSuccess && dev >= 0 && dev < 64) raised[dev] = true;
+    }
     if (e != cudaSuccess) return e;
     k_attend_many<DP, KIND, TQ><<<sm_count(), F::THREADS, F::smem, s>>>(kmap, vmap, a, ws);
     e = cudaGetLastError();

@@ -14,6 +14,8 @@
 // tokens, one warp per token, then all its threads walk the units of those
 // tokens, keys and values in the same iteration so that both loads are in
 // flight.
+#include <type_traits>
+
 #include "kv.cuh"
 #include "launch.h"
 
@@ -50,35 +52,59 @@ __device__ __forceinline__ void store16(T* p, const Vec16<T>& d) {
     for (int i = 0; i < (int)sizeof(T); ++i) s[i] = r[i];
 }
 
-// One thread's half of a Q8_0 block: codes of x[0..15] and the block's scale
-// (the other half sits in the neighbouring lane; both lanes must call).
-__device__ __forceinline__ __half quantise16(const float (&x)[16], Vec16<int8_t>& q, unsigned mask) {
-    float top = 0.f;
-    bool finite = true;
+// Bits of the largest magnitude of 16 values, as an fp32 pattern: patterns of
+// magnitudes order like integers, infinities and NaN above all others.
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(const Vec16<T>& x) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(x.v);
+    if constexpr (sizeof(T) == 4) {
+        uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const float a = fabsf(x[i]);
-        finite = finite && a <= 3.402823466e38f;
-        top = fmaxf(top, a);
+        for (int i = 0; i < 16; ++i) top = max(top, w[i] & 0x7fffffffu);
+        return top;
+    } else {
+        uint32_t pair = w[0] & 0x7fff7fffu;
+#pragma unroll
+        for (int i = 1; i < 8; ++i) pair = __vmaxu2(pair, w[i] & 0x7fff7fffu);
+        const unsigned short h = (unsigned short)max(pair & 0xffffu, pair >> 16);
+        if constexpr (std::is_same<T, __half>::value)
+            return __float_as_uint(__half2float(__ushort_as_half(h))) & 0x7fffffffu;
+        return (uint32_t)h << 16;
     }
-    top = fmaxf(top, __shfl_xor_sync(mask, top, 1));
-    finite = __shfl_xor_sync(mask, (int)finite, 1) && finite;
-    if (!finite) {
+}
+
+// One thread's half of a Q8_0 block: codes of its 16 values and the block's
+// scale (the other half sits in the neighbouring lane; both lanes must call).
+template <typename T>
+__device__ __forceinline__ __half quantise16(const Vec16<T>& x, Vec16<int8_t>& q, unsigned mask) {
+    uint32_t top = top_bits(x);
+    top = max(top, __shfl_xor_sync(mask, top, 1));
+    if (top >= 0x7f800000u) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) q.v[i] = 0;
         return __ushort_as_half(0x7fff);
     }
-    const float step = fminf(__half2float(__float2half_ru(__fdiv_rn(top, 127.f))), kKvScaleMax);
+    const float want = __half2float(__float2half_ru(__fdiv_rn(__uint_as_float(top), 127.f)));
+    const float step = fminf(want, kKvScaleMax);
     const float inv = step > 0.f ? __frcp_rn(step) : 0.f;
+    const float limit = want > kKvScaleMax ? 127.f : INFINITY;   // |x / step| <= 127 otherwise
+    uint32_t* out = reinterpret_cast<uint32_t*>(q.v);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        // x / step, correctly rounded: one step of Newton's correction to
-        // x * (1 / step), whose remainder the fused multiply-add gives exactly
-        const float y = x[i] * inv;
-        const float c = fmaf(fmaf(-y, step, x[i]), inv, y);
-        // nearest integer, ties to even: 1.5 * 2^23 leaves no fraction bits
-        const float n = fminf(fmaxf(c, -127.f), 127.f) + 12582912.f;
-        q.v[i] = (int8_t)__float_as_int(n);
+    for (int w = 0; w < 4; ++w) {
+        uint32_t n[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            // x / step: x times the reciprocal, and one step of Newton's
+            // correction, whose remainder the fused multiply-add gives exactly:
+            // off by 2^-46 before its rounding, so ties stay ties
+            const float f = kv_to_f<T>(x.v[4 * w + i]);
+            const float y = f * inv;
+            float c = fmaf(fmaf(-y, step, f), inv, y);
+            if (limit == 127.f) c = fminf(fmaxf(c, -127.f), 127.f);
+            // nearest integer, ties to even: 1.5 * 2^23 leaves no fraction bits
+            n[i] = __float_as_uint(c + 12582912.f);
+        }
+        out[w] = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
     }
     return __float2half_rn(step);
 }
@@ -131,10 +157,7 @@ k_kv_write(KvBatch b, KvCache c, KvRows in, int tokens, unsigned* status) {
         for (int w = 0; w < 2; ++w) {
             Vec16<TC> y;
             if constexpr (sizeof(TC) == 1) {
-                float f[16];
-#pragma unroll
-                for (int j = 0; j < 16; ++j) f[j] = kv_to_f<TI>(x[w].v[j]);
-                const __half s = quantise16(f, y, mask);
+                const __half s = quantise16(x[w], y, mask);
                 if (!(d & 16)) (w ? c.vs : c.ks)[row * (c.dim >> 5) + (d >> 5)] = s;
             } else {
 #pragma unroll

@@ -230,7 +230,7 @@ class PagedKVCache:
             if dtype is None:
                 dtype = torch.float16 if self.type == Q8_0 else self.k.dtype
             shape = (2, tokens, self.kv_heads, self.head_dim)
-            k, v = torch.empty(shape, dtype=dtype, device=self.device).unbind(0)
+            k, v = self.k.new_empty(shape, dtype=dtype).unbind(0)
         else:
             k, v = out
         kp, kts, khs, _ = self._rows(k, self.kv_heads, TYPE_IDS, "out k", output=True)
@@ -272,7 +272,7 @@ class PagedKVCache:
             raise ValueError("window must be positive, and needs causal")
         tokens = shape[0]
         if out is None:
-            out = torch.empty(shape, dtype=q.dtype, device=self.device)
+            out = q.new_empty(shape)
             op, ots, ohs = out.data_ptr(), heads * self.head_dim, self.head_dim
         else:
             op, ots, ohs, _ = self._rows(out, heads, (q.dtype,), "out", output=True)
@@ -294,7 +294,7 @@ class PagedKVCache:
             need = self._ws_bytes[key] = n.value
         # a workspace of the call's own: torch's allocator hands it to the next
         # call on this stream, or keeps it with the graph that captured it
-        ws = torch.empty(max(need, 256), dtype=torch.uint8, device=self.device)
+        ws = q.new_empty(max(need, 256), dtype=torch.uint8)
         st = self.lib.moe_b200_attend(
             self._ref, bs, TYPE_IDS[q.dtype], qp, qts, qhs, heads, op, ots, ohs,
             lse.data_ptr() if lse is not None else None,
