@@ -10,8 +10,8 @@
 //
 // Both kernels move each value once: bound by HBM.  A thread owns 16 values
 // of a head (two 16-byte loads of a 16-bit row, one 16-byte store of codes),
-// two threads own a Q8_0 block.  A CTA first looks up the slots of its
-// tokens, one warp per token, then all its threads walk the units of those
+// two threads own a Q8_0 block.  A CTA looks up the slots of its up to 32
+// tokens, one lane per token, then all its threads walk the units of those
 // tokens, keys and values in the same iteration so that both loads are in
 // flight.
 #include <type_traits>
@@ -24,7 +24,7 @@ namespace moeb200 {
 namespace {
 
 constexpr int kKvThreads = 256;
-constexpr int kKvMaxTokens = 16;   // tokens per CTA at most
+constexpr int kKvMaxTokens = 32;   // tokens per CTA at most: one per lane
 
 struct KvRows {
     void* k;
@@ -109,26 +109,38 @@ __device__ __forceinline__ __half quantise16(const Vec16<T>& x, Vec16<int8_t>& q
     return __float2half_rn(step);
 }
 
-// Slot (page * heads * page_size + row, in rows of one head; -1: none) of
-// the CTA's tokens.
+// Slot (page * heads * page_size + row, in rows of one head; -1: none, -2:
+// behind the last sequence) of the CTA's tokens: the first warp searches the
+// first token's sequence, and each lane goes on from there for its own token.
+// The other threads wait at the caller's barrier.
 __device__ __forceinline__ void cta_slots(const KvBatch& b, const KvCache& c, int t0, int n,
                                           int64_t* slots, unsigned* status) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int i = warp; i < n; i += kKvThreads / 32) {
-        const int t = t0 + i;
-        const int s = kv_find_seq(b, t);
-        int64_t slot = -1;
-        if (s >= 0 && lane == 0) {
-            const int pos = __ldg(b.kv_lens + s) - __ldg(b.q_start + s + 1) + t;
-            if (pos >= 0) {
-                const int page = kv_page(b, c, s, pos >> c.page_shift, status);
-                if (page >= 0)
-                    slot = ((int64_t)page * c.heads << c.page_shift) + (pos & (c.page_size - 1));
-            }
+    const int lane = threadIdx.x & 31;
+    if (threadIdx.x >= 32) return;
+    int s = kv_find_seq(b, t0);
+    const int t = t0 + lane;
+    if (lane >= n) return;
+    // s = -1: before the first sequence (a malformed q_start), or behind the last
+    int lo = s < 0 ? 0 : s, hi = b.B;
+    if (s < 0 || t >= __ldg(b.q_start + s + 1)) {   // the last b with q_start[b] <= t
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (__ldg(b.q_start + mid) <= t) lo = mid; else hi = mid;
         }
-        if (lane == 0) slots[i] = s < 0 ? -2 : slot;
+        s = lo;
     }
-    __syncthreads();
+    const int q0 = __ldg(b.q_start + s), q1 = __ldg(b.q_start + s + 1);
+    int64_t slot = -2;
+    if (q0 <= t && t < q1) {
+        slot = -1;
+        const int pos = __ldg(b.kv_lens + s) - q1 + t;
+        if (pos >= 0) {
+            const int page = kv_page(b, c, s, pos >> c.page_shift, status);
+            if (page >= 0)
+                slot = ((int64_t)page * c.heads << c.page_shift) + (pos & (c.page_size - 1));
+        }
+    }
+    slots[lane] = slot;
 }
 
 // TI: type of the rows, TC: type of the cache (int8_t: Q8_0).
@@ -138,32 +150,46 @@ k_kv_write(KvBatch b, KvCache c, KvRows in, int tokens, unsigned* status) {
     __shared__ int64_t slots[kKvMaxTokens];
     const int t0 = blockIdx.x * tokens;
     const int n = b.T - t0 < tokens ? b.T - t0 : tokens;
-    cta_slots(b, c, t0, n, slots, status);
     const int per_head = c.dim >> 4;
     const int per_token = per_head * c.heads;
-    for (int u = threadIdx.x; u < n * per_token; u += kKvThreads) {
-        const int i = u / per_token;
-        const int64_t slot = slots[i];
-        if (slot < 0) continue;   // both lanes of a block share the token
+    // a unit's rows are loaded while the one before it is stored, the first
+    // while the slots are looked up
+    Vec16<TI> x[2];
+    int i = 0, h = 0, d = 0;
+    auto load = [&](int u) {
+        i = u / per_token;
         const int r = u - i * per_token;
-        const int h = r / per_head;
-        const int d = (r - h * per_head) << 4;
-        Vec16<TI> x[2];
+        h = r / per_head;
+        d = (r - h * per_head) << 4;
         load16(x[0], static_cast<const TI*>(in.k) + (t0 + i) * in.k_ts + h * in.k_hs + d);
         load16(x[1], static_cast<const TI*>(in.v) + (t0 + i) * in.v_ts + h * in.v_hs + d);
+    };
+    const int units = n * per_token;
+    int u = threadIdx.x;
+    if (u < units) load(u);
+    cta_slots(b, c, t0, n, slots, status);
+    __syncthreads();
+    while (u < units) {
+        const int64_t slot = slots[i];
         const int64_t row = slot + ((int64_t)h << c.page_shift);
+        const int at = d;
+        const Vec16<TI> y0 = x[0], y1 = x[1];
+        u += kKvThreads;
+        if (u < units) load(u);
+        if (slot < 0) continue;   // both lanes of a block share the token
         const unsigned mask = __activemask();
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
+            const Vec16<TI>& v = w ? y1 : y0;
             Vec16<TC> y;
             if constexpr (sizeof(TC) == 1) {
-                const __half s = quantise16(x[w], y, mask);
-                if (!(d & 16)) (w ? c.vs : c.ks)[row * (c.dim >> 5) + (d >> 5)] = s;
+                const __half s = quantise16(v, y, mask);
+                if (!(at & 16)) (w ? c.vs : c.ks)[row * (c.dim >> 5) + (at >> 5)] = s;
             } else {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) y.v[j] = kv_from_f<TC>(kv_to_f<TI>(x[w].v[j]));
+                for (int j = 0; j < 16; ++j) y.v[j] = kv_from_f<TC>(kv_to_f<TI>(v.v[j]));
             }
-            store16(static_cast<TC*>(w ? c.v : c.k) + row * c.dim + d, y);
+            store16(static_cast<TC*>(w ? c.v : c.k) + row * c.dim + at, y);
         }
     }
 }
@@ -176,8 +202,10 @@ k_kv_read(KvBatch b, KvCache c, KvRows out, int tokens, unsigned* status) {
     const int t0 = blockIdx.x * tokens;
     const int n = b.T - t0 < tokens ? b.T - t0 : tokens;
     cta_slots(b, c, t0, n, slots, status);
+    __syncthreads();
     const int per_head = c.dim >> 4;
     const int per_token = per_head * c.heads;
+#pragma unroll 2
     for (int u = threadIdx.x; u < n * per_token; u += kKvThreads) {
         const int i = u / per_token;
         const int64_t slot = slots[i];
