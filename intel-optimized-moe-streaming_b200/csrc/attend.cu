@@ -154,7 +154,7 @@ cudaError_t join_as(const AttendArgs& a, void* ws, int ctas, int M, cudaStream_t
 // rows: a few pieces, a warp per row.
 template <typename TO, int DP>
 cudaError_t join(const AttendArgs& a, void* ws, int ctas, int M, cudaStream_t s) {
-    return M == kFewRows ? join_as<TO, DP, 4>(a, ws, ctas, M, s)
+    return M <= 16 ? join_as<TO, DP, 4>(a, ws, ctas, M, s)
                          : join_as<TO, DP, 1>(a, ws, ctas, M, s);
 }
 
@@ -239,14 +239,15 @@ __global__ void __launch_bounds__(256) k_attend_expand(KvBatch b, KvCache c, __h
     }
 }
 
-// How a call runs.  Tiles of 16 rows up to 32 rows per sequence on average (a
-// tile reads the keys again), tiles of 128 or 256 beyond.  Those decode a Q8_0
+// How a call runs.  Tiles of 8 rows up to 8 rows per sequence on average, of 16
+// up to 32 (a tile reads the keys again), of 128 or 256 beyond.  Those decode a Q8_0
 // cache's values as often as a sequence has tiles, on warps that the softmax
 // needs (chunks of 2048 rows over 8k keys, 32/8 heads x 128: 444 us, expanded
 // first 260 us); from two tiles on the pages are expanded to binary16 in the
 // workspace, if the table's width bounds that by 1 GB.
 struct AttendPlan {
     bool many;
+    int rows;             // of a tile
     size_t base, plane;   // workspace of the kernel; bytes of an expanded plane, or 0
     size_t bytes() const { return base + 2 * plane; }
 };
@@ -256,9 +257,9 @@ AttendPlan attend_plan(const KvBatch& b, const KvCache& c, int group) {
     const int64_t rows = (int64_t)b.T * group;
     AttendPlan p{};
     p.many = rows > 32 * (int64_t)b.B;
-    p.base = align_up(p.many ? AttendWs::bytes(sm_count(), many_rows(dp), dp)
-                             : AttendWs::bytes(attend_few_ctas(), kFewRows, dp));
-    if (p.many && c.type == Q8_0 && rows > many_rows(dp) * (int64_t)b.B && b.max_pages > 0 &&
+    p.rows = p.many ? many_rows(dp) : rows > 8 * (int64_t)b.B ? 16 : 8;
+    p.base = align_up(AttendWs::bytes(p.many ? sm_count() : attend_few_ctas(), p.rows, dp));
+    if (p.many && c.type == Q8_0 && rows > p.rows * (int64_t)b.B && b.max_pages > 0 &&
         b.B <= 65535) {
         const uint64_t values =
             ((uint64_t)b.B * b.max_pages * c.heads << c.page_shift) * (uint64_t)c.dim;
@@ -276,7 +277,7 @@ size_t attend_workspace_bytes(const KvBatch& b, const KvCache& c, int q_heads) {
 
 cudaError_t launch_attend(const AttendArgs& a, void* ws, cudaStream_t s) {
     const AttendPlan p = attend_plan(a.b, a.c, a.group);
-    if (!p.many) return launch_attend_few(a, ws, s);
+    if (!p.many) return launch_attend_few(a, p.rows, ws, s);
     if (!p.plane) return launch_attend_many(a, ws, s);
     AttendArgs x = a;
     x.c.type = KV_F16;

@@ -88,10 +88,9 @@ cudaError_t launch_attend(const AttendArgs& a, void* ws, cudaStream_t s);
 // (the values beyond head_dim are zeros).
 inline int attend_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
-// Tiles of 16 rows (attend_few.cu): decoding and other calls of few rows.
-constexpr int kFewRows = 16;
+// Tiles of 8 or 16 rows (attend_few.cu): decoding and other calls of few rows.
 int attend_few_ctas();
-cudaError_t launch_attend_few(const AttendArgs& a, void* ws, cudaStream_t s);
+cudaError_t launch_attend_few(const AttendArgs& a, int rows, void* ws, cudaStream_t s);
 
 // Tiles of 256 rows (128 for a head dimension above 128) on tcgen05
 // (attend_many.cu): chunks of prompts.

@@ -2,27 +2,27 @@
 // sequence: single decoded tokens, drafted tokens, short chunks.
 //
 // Such a call reads every key and value once and does little with them, so
-// it is bound by HBM.  Tiles of 16 rows (the query heads of a group, times
-// tokens) are one M = 16 operand of mma.sync: with 8 heads to a group the
-// tensor cores do 16 multiply-adds per value read, far below their rate, while
-// the CUDA cores would need all of theirs.  tcgen05's smallest M is 64 and its
-// operands go through shared and tensor memory, which 16 rows do not repay.
+// it is bound by HBM.  A tile of 8 rows (the query heads of a group, times
+// tokens; 16 where sequences have more) is the N of mma.sync: scores come as
+// keys x rows, outputs as dimensions x rows, and no product is spent on rows
+// that are not there.  The CUDA cores would need all of their rate for 8 heads
+// to a group; tcgen05's smallest M is 64, and its operands go through shared
+// and tensor memory, which so few rows do not repay.
 //
 // A warp walks subtiles of 16 to 64 keys (8 KB) on its own: a ring of NS
 // shared-memory entries per warp (a subtile's keys, then its values) filled by
 // tensor copies with a 128-byte swizzle, no block barrier in the loop.  A
 // subtile is one chain of products, maximum, exponentials and products, about
 // 1900 cycles long however few keys it has, so it has as many as fit.
-// The scores of 16 rows x 16 G keys stay in registers as the accumulator, become
-// the A operand of the value product in place, and the running maximum, sum
-// and 16 x DP output are the warp's own until the tile ends; then the four
-// warps' sums are added through shared memory.  Two CTAs per SM, so that one
-// loads while the other starts or ends a tile.
+// The running maximum, sum and DP x 8 outputs stay in the warp's registers
+// until the tile ends; then the four warps' sums are added through shared
+// memory.  Probabilities change places between the products by movmatrix.  Two
+// CTAs per SM, so that one loads while the other starts or ends a tile.
 //
 // Q8_0: codes become binary16 by a byte permute (1024 + 128 + code, exact) and
 // one subtraction, times the block's scale, rounded once: the value of
 // scale * code in binary16.  The order of head dimensions within the key
-// product, and of output columns, is permuted so that a thread takes its codes
+// product, and of output rows, is permuted so that a thread takes its codes
 // as 16 consecutive bytes and no transposing load is needed.
 #include "attend_mma.cuh"
 #include "launch.h"
@@ -36,8 +36,10 @@ constexpr int kFewThreads = kFewWarps * 32;
 constexpr int kFewCost = 0;                      // of a tile, in units
 constexpr uint32_t kFewPolls = 1u << 21;
 
-template <int DP, int KIND>
+// NT: row tiles of 8.
+template <int DP, int KIND, int NT>
 struct Few {
+    static constexpr int M = 8 * NT;
     static constexpr bool Q8 = KIND == KIND_Q8;
     static constexpr int EB = Q8 ? 1 : 2;
     static constexpr int ROWB = DP * EB;                       // bytes of a cached row
@@ -54,21 +56,21 @@ struct Few {
     static constexpr int FIT = 104448 / (kFewWarps * (TILEB + SCALEB));
     static constexpr int NS = FIT > 8 ? 8 : FIT;
     static constexpr int VB = Q8 ? (DP >= 128 ? 16 : 8) : 8;   // codes a thread takes of a value row
-    static constexpr int TILES = DP / 8;
+    static constexpr int TILES = DP / 16;                      // output tiles of 16 dimensions
+    static constexpr bool QSM = NT * DP > 256;                 // queries in shared memory
     // binary16 probabilities are taken 2^15 times as large (the largest is
     // 2^15, below 65504), so that those down to 2^-29 keep all their bits
     static constexpr float SHIFT = KIND == KIND_BF16 ? 0.f : 15.f;
     static constexpr int PD = DP < 128 ? DP : 128;             // columns joined per pass
     static constexpr int o_scale = kFewWarps * NS * TILEB;
     static constexpr int o_q = o_scale + kFewWarps * NS * SCALEB;
-    static constexpr int o_bar = o_q + DP * 32;
+    static constexpr int o_bar = o_q + (QSM ? DP / 16 * NT * 32 * 8 : 0);
     static constexpr int o_m = o_bar + kFewWarps * NS * 8;
     static constexpr int o_l = o_m + kFewWarps * 16 * 4;
-    static constexpr int o_rs = o_l + kFewWarps * 16 * 4;
-    static constexpr int smem = o_rs + 16 * 4 + 1024;          // 1024: base alignment
+    static constexpr int smem = o_l + kFewWarps * 16 * 4 + 1024;   // 1024: base alignment
     static_assert(NS >= 3, "");
     static_assert(2 * (smem + 1024) <= 233472, "two CTAs per SM");
-    static_assert(kFewWarps * 16 * (PD + 4) * 4 <= o_q, "join buffer inside the ring");
+    static_assert(kFewWarps * M * (PD + 4) * 4 <= o_q, "join buffer inside the ring");
 };
 
 template <int KIND>
@@ -108,36 +110,45 @@ __device__ __forceinline__ bool odd_scale(__half s) {
     return (__half_as_ushort(s) & 0x7fffu) >= 0x6000u;
 }
 
-// Key of column n of an 8-key score tile.  Q8_0 swaps odd keys n and n ^ 4:
-// the 16-byte chunks that a quarter warp reads of the keys (columns 2 q and
-// 2 q + 1) and of the values (rows of the keys of the even, or the odd,
-// columns) then lie in different banks of the swizzled rows.
+// Key of row n of an 8-key score tile.  Q8_0 swaps odd keys n and n ^ 4: the
+// 16-byte chunks that a quarter warp reads of the keys (rows 2 q and 2 q + 1)
+// and of the values (those of the even, or the odd, rows) then lie in
+// different banks of the swizzled rows.
 template <int KIND>
-__device__ __forceinline__ int column_key(int n) {
+__device__ __forceinline__ int row_key(int n) {
     return KIND == KIND_Q8 ? n ^ ((n & 1) << 2) : n;
 }
 
-// Head dimension of output tile i, column n.
+// Head dimension of output tile i, row n (h: n + 8).
 template <int DP, int KIND>
-__device__ __forceinline__ int out_dim(int i, int n) {
-    using F = Few<DP, KIND>;
-    if constexpr (F::Q8) return (i / F::VB) * (F::VB * 8) + n * F::VB + i % F::VB;
-    return i * 8 + n;
+__device__ __forceinline__ int out_dim(int i, int n, int h) {
+    using F = Few<DP, KIND, 1>;
+    if constexpr (F::Q8)
+        return (i / (F::VB / 2)) * (F::VB * 8) + n * F::VB + i % (F::VB / 2) * 2 + h;
+    return i * 16 + n + 8 * h;
+}
+
+// Transposes an 8 x 8 matrix of 16-bit values held as accumulator pairs.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t t;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(t) : "r"(v));
+    return t;
 }
 
 // TQ: type of q and out.
-template <int DP, int KIND, typename TQ>
+template <int DP, int KIND, int NT, typename TQ>
 __global__ void __launch_bounds__(kFewThreads, 2)
 k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
              const __grid_constant__ AttendArgs a, void* wsp) {
-    using F = Few<DP, KIND>;
+    using F = Few<DP, KIND, NT>;
+    constexpr int M = F::M, R = 2 * NT;   // rows of the tile; rows of a thread
+    constexpr bool CONVERT = F::Q8 && std::is_same<TQ, __nv_bfloat16>::value;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint4* qf = reinterpret_cast<uint4*>(sm + F::o_q);
+    uint2* qf = reinterpret_cast<uint2*>(sm + F::o_q);
     float* sm_m = reinterpret_cast<float*>(sm + F::o_m);
     float* sm_l = reinterpret_cast<float*>(sm + F::o_l);
-    float* sm_rs = reinterpret_cast<float*>(sm + F::o_rs);
     float* joinb = reinterpret_cast<float*>(sm);
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -154,7 +165,7 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
 
     const int ctas = gridDim.x;
     AttendWs ws(wsp, ctas);
-    AttendCursor cur = attend_place<kFewRows, F::UNIT, kFewCost, kFewThreads>(
+    AttendCursor cur = attend_place<M, F::UNIT, kFewCost, kFewThreads>(
         a, *reinterpret_cast<AttendScratch*>(sm), blockIdx.x, ctas, a.status);
     fence_async_smem();   // the scratch lies in the ring
     AttendRecord rec{};
@@ -165,106 +176,11 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
     if (cur.left > 0) s = attend_seq(a, cur.seq, nullptr);
 
     while (cur.left > 0) {
-        const AttendPart part = attend_part<kFewRows, F::UNIT, kFewCost>(a, cur, s);
+        const AttendPart part = attend_part<M, F::UNIT, kFewCost>(a, cur, s);
         const int u0 = part.u0, take = part.take;
-        const int rows = s.n * a.group - cur.tile * kFewRows;   // valid rows: the first `rows`
-
-        // queries as A fragments; bf16 ones over a Q8_0 cache become binary16
-        // after an exact scaling of the row to a maximum in [1, 2)
-        if constexpr (F::Q8) {
-            for (int r = warp; r < 16; r += kFewWarps) {
-                float f = 1.f;
-                if constexpr (std::is_same<TQ, __nv_bfloat16>::value) {
-                    float top = 0.f;
-                    if (r < rows) {
-                        const int rr = cur.tile * kFewRows + r;
-                        const int tok = a.by_group.div(rr);
-                        const TQ* q = static_cast<const TQ*>(a.q) + (int64_t)(s.q0 + tok) * a.q_ts +
-                                      (int64_t)(cur.kvh * a.group + rr - tok * a.group) * a.q_hs;
-                        for (int d = lane; d < a.c.dim; d += 32) top = fmaxf(top, fabsf(kv_to_f<TQ>(q[d])));
-                    }
-                    top = warp_max(top);
-                    f = row_factor(top);
-                }
-                if (lane == 0) sm_rs[r] = f;
-            }
-            __syncthreads();
-        }
-        for (int i = tid; i < DP / 16 * 32; i += kFewThreads) {
-            const int st = i >> 5, l = i & 31, lr = l >> 2, lc = l & 3;
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int r = lr + (j & 1) * 8;
-                const int d = F::Q8 ? (st >> 2) * 64 + lc * 16 + (st & 3) * 4 + (j >> 1) * 2
-                                    : st * 16 + lc * 2 + (j >> 1) * 8;
-                w[j] = 0;
-                if (r < rows && d < a.c.dim) {
-                    const int rr = cur.tile * kFewRows + r;
-                    const int tok = a.by_group.div(rr);
-                    const TQ* q = static_cast<const TQ*>(a.q) + (int64_t)(s.q0 + tok) * a.q_ts +
-                                  (int64_t)(cur.kvh * a.group + rr - tok * a.group) * a.q_hs + d;
-                    w[j] = *reinterpret_cast<const uint32_t*>(q);
-                    if constexpr (F::Q8 && std::is_same<TQ, __nv_bfloat16>::value)
-                        w[j] = pack16<KIND_F16>(kv_to_f<TQ>(q[0]) * sm_rs[r],
-                                                kv_to_f<TQ>(q[1]) * sm_rs[r]);
-                }
-            }
-            const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-            qf[i] = make_uint4(w[0] ^ flip, w[1] ^ flip, w[2] ^ flip, w[3] ^ flip);
-        }
-        // the two rows of this thread: the keys they attend, the factor that
-        // takes a score to units of log 2
-        int lo[2], hi[2];
-        float mul[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = n8 + 8 * i;
-            lo[i] = hi[i] = 0;
-            if (r < rows)
-                attend_range(s.first + a.by_group.div(cur.tile * kFewRows + r), s.len, a.causal,
-                             a.window, lo[i], hi[i]);
-        }
-        const AttendTile tile = attend_tile(a, s, cur.tile * kFewRows, kFewRows);
+        const int rows = s.n * a.group - cur.tile * M;   // valid rows: the first `rows`
+        const AttendTile tile = attend_tile(a, s, cur.tile * M, M);
         const int t_lo = tile.t_lo, t_hi = tile.t_hi, all_lo = tile.all_lo, all_hi = tile.all_hi;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            mul[i] = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);   // 0: equal weights
-            if constexpr (F::Q8 && std::is_same<TQ, __nv_bfloat16>::value)
-                mul[i] /= sm_rs[n8 + 8 * i];
-        }
-        uint32_t qreg[DP <= 128 ? DP / 16 : 1][4];
-        if constexpr (DP <= 128) {
-#pragma unroll
-            for (int st = 0; st < DP / 16; ++st) {
-                const uint4 w = qf[st * 32 + lane];
-                qreg[st][0] = w.x;
-                qreg[st][1] = w.y;
-                qreg[st][2] = w.z;
-                qreg[st][3] = w.w;
-            }
-        }
-
-        auto q_at = [&](int st, uint32_t (&qa)[4]) {
-            if constexpr (DP <= 128) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) qa[i] = qreg[st][i];
-            } else {
-                const uint4 w = qf[st * 32 + lane];
-                qa[0] = w.x;
-                qa[1] = w.y;
-                qa[2] = w.z;
-                qa[3] = w.w;
-            }
-        };
-        float o[F::TILES][4];
-#pragma unroll
-        for (int i = 0; i < F::TILES; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-
         // A subtile is fetched in boxes of whole pages or parts of one; the
         // page ids of 32 boxes at a time are held one per lane (-1: nothing
         // there).
@@ -321,6 +237,95 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
 #pragma unroll 1
         for (int e = 0; e < F::NS; ++e) fetch(e);
 
+        // Queries as B operands: this thread's are of row n8 of each row tile;
+        // bf16 ones over a Q8_0 cache become binary16 after an exact scaling of
+        // the row to a maximum in [1, 2).  The four warps hold the same ones.
+        uint2 qreg[F::QSM ? 1 : DP / 16][NT];
+        float factor[NT];
+        {
+            const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const int r = t * 8 + n8;
+                const int rr = cur.tile * M + (r < rows ? r : 0);
+                const int tok = a.by_group.div(rr);
+                const TQ* q = static_cast<const TQ*>(a.q) + (int64_t)(s.q0 + tok) * a.q_ts +
+                              (int64_t)(cur.kvh * a.group + rr - tok * a.group) * a.q_hs;
+                auto pair = [&](int d) {
+                    return r < rows && d < a.c.dim ? *reinterpret_cast<const uint32_t*>(q + d) : 0u;
+                };
+                auto both = [&](int st) {   // the two registers of 16 dimensions
+                    const int d = F::Q8 ? (st >> 2) * 64 + c4 * 16 + (st & 3) * 4 : st * 16 + c4 * 2;
+                    return make_uint2(pair(d), pair(d + (F::Q8 ? 2 : 8)));
+                };
+                factor[t] = 1.f;
+                auto convert = [&](uint32_t w) {
+                    if constexpr (CONVERT)
+                        w = pack16<KIND_F16>(__uint_as_float(w << 16) * factor[t],
+                                             __uint_as_float(w & 0xffff0000u) * factor[t]);
+                    return w ^ flip;
+                };
+                uint2 w[DP / 16];
+#pragma unroll
+                for (int st = 0; st < DP / 16; ++st) w[st] = both(st);
+                if constexpr (CONVERT) {
+                    float top = 0.f;
+#pragma unroll
+                    for (int st = 0; st < DP / 16; ++st) {
+                        top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[st].x << 16)),
+                                               fabsf(__uint_as_float(w[st].x & 0xffff0000u))));
+                        top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[st].y << 16)),
+                                               fabsf(__uint_as_float(w[st].y & 0xffff0000u))));
+                    }
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    factor[t] = row_factor(top);
+                }
+#pragma unroll
+                for (int st = 0; st < DP / 16; ++st) {
+                    const uint2 x = make_uint2(convert(w[st].x), convert(w[st].y));
+                    if constexpr (F::QSM) {
+                        if ((st & 3) == warp) qf[(st * NT + t) * 32 + lane] = x;
+                    } else {
+                        qreg[st][t] = x;
+                    }
+                }
+            }
+            if constexpr (F::QSM) __syncthreads();
+        }
+        auto q_at = [&](int st, int t) {
+            if constexpr (F::QSM) return qf[(st * NT + t) * 32 + lane];
+            else return qreg[st][t];
+        };
+        // this thread's rows t * 8 + 2 c4 + e: the keys they attend, the factor
+        // that takes a score to units of log 2
+        int lo[R], hi[R];
+        float mul[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int r = i / 2 * 8 + c4 * 2 + (i & 1);
+            lo[i] = hi[i] = 0;
+            if (r < rows)
+                attend_range(s.first + a.by_group.div(cur.tile * M + r), s.len, a.causal, a.window,
+                             lo[i], hi[i]);
+            mul[i] = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);   // 0: equal weights
+            if constexpr (CONVERT)
+                mul[i] /= __shfl_sync(0xffffffffu, factor[i / 2], (c4 * 2 + (i & 1)) * 4);
+        }
+        float o[F::TILES][NT][4];
+#pragma unroll
+        for (int i = 0; i < F::TILES; ++i)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][t][e] = 0.f;
+        float m[R], l[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            m[i] = -INFINITY;
+            l[i] = 0.f;
+        }
+
 #pragma unroll 1
         for (int j = 0; j < take; ++j) {
             if (!((there >> (j & 31)) & 1)) {
@@ -329,27 +334,28 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
                 continue;
             }
             const int key0 = ((u0 + j) * kFewWarps + warp) * F::KEYS;
-            // ---- scores: 8-key column tiles
-            float p[2 * F::G][4] = {};
+            // ---- scores: 16 keys x 8 rows; element e: key (e >> 1) * 8 + n8,
+            // row 2 c4 + (e & 1)
+            float p[F::G][NT][4] = {};
             await();
             {
                 const unsigned char* kt = ring + out_slot * F::TILEB;
                 if constexpr (!F::Q8) {
                     const uint32_t kaddr = smem_u32(kt);
-                    const int key = (lane >> 4) * 8 + (lane & 7), half = (lane >> 3) & 1;
+                    const int key = lane & 15, half = lane >> 4;
 #pragma unroll
                     for (int st = 0; st < DP / 16; ++st) {
-                        uint32_t b[F::G][4], qa[4];
+                        uint32_t ka[F::G][4];
                         const int ch = (st & 3) * 2 + half;
 #pragma unroll
                         for (int g = 0; g < F::G; ++g)
-                            ldsm4<false>(b[g], kaddr + (st >> 2) * F::SLAB + (g * 16 + key) * 128 +
-                                                   ((ch ^ (key & 7)) << 4));
-                        q_at(st, qa);
+                            ldsm4<false>(ka[g], kaddr + (st >> 2) * F::SLAB + (g * 16 + key) * 128 +
+                                                    ((ch ^ (key & 7)) << 4));
 #pragma unroll
-                        for (int g = 0; g < F::G; ++g) {
-                            mma16816<KIND>(p[2 * g], qa, b[g][0], b[g][1]);
-                            mma16816<KIND>(p[2 * g + 1], qa, b[g][2], b[g][3]);
+                        for (int t = 0; t < NT; ++t) {
+                            const uint2 q = q_at(st, t);
+#pragma unroll
+                            for (int g = 0; g < F::G; ++g) mma16816<KIND>(p[g][t], ka[g], q.x, q.y);
                         }
                     }
                 } else {
@@ -357,28 +363,33 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
 #pragma unroll
                     for (int sp = 0; sp < DP / 64; ++sp) {
                         const int blk = sp * 2 + (c4 >> 1);
-                        uint32_t qa[4][4];
 #pragma unroll
-                        for (int st = 0; st < 4; ++st) q_at(sp * 4 + st, qa[st]);
+                        for (int g = 0; g < F::G; ++g) {
+                            uint32_t w[2][4];
+                            __half2 d[2];
 #pragma unroll
-                        for (int t = 0; t < 2 * F::G; ++t) {
-                            const int key = t * 8 + column_key<KIND>(n8);
-                            const int at = F::SLABB == 128
-                                               ? (sp >> 1) * F::SLAB + key * 128 +
-                                                     ((((sp & 1) * 4 + c4) ^ (key & 7)) << 4)
-                                               : key * 64 + c4 * 16;
-                            const uint4 w = *reinterpret_cast<const uint4*>(kt + at);
-                            const __half2 d = __half2half2(blk < nb ? ks[key * nb + blk]
-                                                                    : __ushort_as_half(0));
-                            uint32_t b0, b1;
-                            codes4(w.x, d, b0, b1);
-                            mma16816<KIND>(p[t], qa[0], b0, b1);
-                            codes4(w.y, d, b0, b1);
-                            mma16816<KIND>(p[t], qa[1], b0, b1);
-                            codes4(w.z, d, b0, b1);
-                            mma16816<KIND>(p[t], qa[2], b0, b1);
-                            codes4(w.w, d, b0, b1);
-                            mma16816<KIND>(p[t], qa[3], b0, b1);
+                            for (int h = 0; h < 2; ++h) {
+                                const int key = g * 16 + h * 8 + row_key<KIND>(n8);
+                                const int at = F::SLABB == 128
+                                                   ? (sp >> 1) * F::SLAB + key * 128 +
+                                                         ((((sp & 1) * 4 + c4) ^ (key & 7)) << 4)
+                                                   : key * 64 + c4 * 16;
+                                *reinterpret_cast<uint4*>(w[h]) =
+                                    *reinterpret_cast<const uint4*>(kt + at);
+                                d[h] = __half2half2(blk < nb ? ks[key * nb + blk]
+                                                             : __ushort_as_half(0));
+                            }
+#pragma unroll
+                            for (int st = 0; st < 4; ++st) {
+                                uint32_t ka[4];
+                                codes4(w[0][st], d[0], ka[0], ka[2]);
+                                codes4(w[1][st], d[1], ka[1], ka[3]);
+#pragma unroll
+                                for (int t = 0; t < NT; ++t) {
+                                    const uint2 q = q_at(sp * 4 + st, t);
+                                    mma16816<KIND>(p[g][t], ka, q.x, q.y);
+                                }
+                            }
                         }
                     }
                 }
@@ -390,25 +401,28 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
             const bool whole = key0 >= all_lo && key0 + F::KEYS <= all_hi;
             if (!whole) {
 #pragma unroll
-                for (int t = 0; t < 2 * F::G; ++t)
+                for (int g = 0; g < F::G; ++g)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int key = key0 + t * 8 + column_key<KIND>(c4 * 2 + (e & 1));
-                        if (key < lo[e >> 1] || key >= hi[e >> 1]) p[t][e] = -INFINITY;
-                    }
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int key = key0 + g * 16 + (e >> 1) * 8 + row_key<KIND>(n8);
+                            const int i = 2 * t + (e & 1);
+                            if (key < lo[i] || key >= hi[i]) p[g][t][e] = -INFINITY;
+                        }
             }
-            float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-            for (int t = 0; t < 2 * F::G; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], p[t][e]);
             bool grew = false;
-            float keep[2], base[2];
+            float keep[R], base[R];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-                const float mn = fmaxf(m[i], top[i] * mul[i]);
+            for (int i = 0; i < R; ++i) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int g = 0; g < F::G; ++g)
+                    top = fmaxf(fmaxf(top, p[g][i / 2][i & 1]), p[g][i / 2][2 + (i & 1)]);
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                const float mn = fmaxf(m[i], top * mul[i]);
                 base[i] = mn == -INFINITY ? 0.f : mn - F::SHIFT;
                 keep[i] = ex2(m[i] - (mn == -INFINITY ? 0.f : mn));
                 grew = grew || mn > m[i];
@@ -416,28 +430,28 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
             }
             if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) l[i] *= keep[i];
+                for (int i = 0; i < R; ++i) l[i] *= keep[i];
 #pragma unroll
-                for (int i = 0; i < F::TILES; ++i) {
-                    o[i][0] *= keep[0];
-                    o[i][1] *= keep[0];
-                    o[i][2] *= keep[1];
-                    o[i][3] *= keep[1];
-                }
+                for (int i = 0; i < F::TILES; ++i)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[i][t][e] *= keep[2 * t + (e & 1)];
             }
+            uint32_t pb[F::G][NT][2];   // probabilities as B operands: keys x rows
 #pragma unroll
-            for (int t = 0; t < 2 * F::G; ++t)
+            for (int g = 0; g < F::G; ++g)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    p[t][e] = ex2(fmaf(p[t][e], mul[e >> 1], -base[e >> 1]));
-                    l[e >> 1] += p[t][e];
+                for (int t = 0; t < NT; ++t) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int i = 2 * t + (e & 1);
+                        p[g][t][e] = ex2(fmaf(p[g][t][e], mul[i], -base[i]));
+                        l[i] += p[g][t][e];
+                    }
+                    pb[g][t][0] = transpose8(pack16<KIND>(p[g][t][0], p[g][t][1]));
+                    pb[g][t][1] = transpose8(pack16<KIND>(p[g][t][2], p[g][t][3]));
                 }
-            uint32_t pa[F::G][4];
-#pragma unroll
-            for (int t = 0; t < 2 * F::G; ++t) {
-                pa[t / 2][2 * (t & 1)] = pack16<KIND>(p[t][0], p[t][1]);
-                pa[t / 2][2 * (t & 1) + 1] = pack16<KIND>(p[t][2], p[t][3]);
-            }
             // ---- values
             await();
             unsigned char* vt = ring + out_slot * F::TILEB;
@@ -495,29 +509,28 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
                         }
                     };
 #pragma unroll
-                    for (int t = 0; t < 2 * F::G; ++t) {
+                    for (int gh = 0; gh < 2 * F::G; ++gh) {   // 8 keys at a time
 #pragma unroll 1
                         for (int k8 = 0; k8 < 8; ++k8) {
-                            const int col = column_key<KIND>(k8);   // its own inverse
-                            const int from = (lane & ~3) | (col >> 1);
-                            float pk[2];
+                            const int k = gh * 8 + k8;
+                            const int from = row_key<KIND>(k8) * 4 + c4;   // row_key undoes itself
+                            float pk[R];
+                            bool at[R];
 #pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const float x = __shfl_sync(0xffffffffu, p[t][2 * i], from);
-                                const float y = __shfl_sync(0xffffffffu, p[t][2 * i + 1], from);
-                                pk[i] = col & 1 ? y : x;
+                            for (int i = 0; i < R; ++i) {
+                                pk[i] = __shfl_sync(0xffffffffu,
+                                                    p[gh / 2][i / 2][(gh & 1) * 2 + (i & 1)], from);
+                                at[i] = key0 + k >= lo[i] && key0 + k < hi[i];
                             }
-                            const int k = t * 8 + k8;
-                            const bool at0 = key0 + k >= lo[0] && key0 + k < hi[0];
-                            const bool at1 = key0 + k >= lo[1] && key0 + k < hi[1];
 #pragma unroll
-                            for (int i = 0; i < F::TILES; ++i)
+                            for (int x = 0; x < F::TILES; ++x)
 #pragma unroll
-                                for (int e = 0; e < 2; ++e) {
-                                    const float v = odd_value(k, out_dim<DP, KIND>(i, c4 * 2 + e));
+                                for (int h = 0; h < 2; ++h) {
+                                    const float v = odd_value(k, out_dim<DP, KIND>(x, n8, h));
                                     if (v != 0.f) {   // NaN or infinite
-                                        if (at0) o[i][e] += pk[0] * v;
-                                        if (at1) o[i][2 + e] += pk[1] * v;
+#pragma unroll
+                                        for (int i = 0; i < R; ++i)
+                                            if (at[i]) o[x][i / 2][2 * h + (i & 1)] += pk[i] * v;
                                     }
                                 }
                         }
@@ -537,17 +550,18 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
             }
             if constexpr (!F::Q8) {
                 const uint32_t vaddr = smem_u32(vt);
-                const int key = ((lane >> 3) & 1) * 8 + (lane & 7), half = lane >> 4;
+                const int key = (lane >> 4) * 8 + (lane & 7), half = (lane >> 3) & 1;
 #pragma unroll
-                for (int d = 0; d < DP / 16; ++d) {
-                    const int ch = (d & 3) * 2 + half;
+                for (int x = 0; x < DP / 16; ++x) {
+                    const int ch = (x & 3) * 2 + half;
 #pragma unroll
                     for (int g = 0; g < F::G; ++g) {
-                        uint32_t b[4];
-                        ldsm4<true>(b, vaddr + (d >> 2) * F::SLAB + (g * 16 + key) * 128 +
-                                           ((ch ^ (key & 7)) << 4));
-                        mma16816<KIND>(o[2 * d], pa[g], b[0], b[1]);
-                        mma16816<KIND>(o[2 * d + 1], pa[g], b[2], b[3]);
+                        uint32_t va[4];
+                        ldsm4<true>(va, vaddr + (x >> 2) * F::SLAB + (g * 16 + key) * 128 +
+                                            ((ch ^ (key & 7)) << 4));
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+                            mma16816<KIND>(o[x][t], va, pb[g][t][0], pb[g][t][1]);
                     }
                 }
             } else {
@@ -561,7 +575,7 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
                         __half2 d[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const int key = g * 16 + column_key<KIND>(c4 * 2 + (i & 1)) + (i >> 1) * 8;
+                            const int key = g * 16 + row_key<KIND>(c4 * 2 + (i & 1)) + (i >> 1) * 8;
                             d[i] = __half2half2(blk < nb ? vs[key * nb + blk] : __ushort_as_half(0));
                             if constexpr (F::VB == 16)
                                 *reinterpret_cast<uint4*>(w[i]) = *reinterpret_cast<const uint4*>(
@@ -576,11 +590,15 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
 #pragma unroll
                             for (int i = 0; i < 4; ++i) codes4(w[i][q], d[i], x[i][0], x[i][1]);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const unsigned sel = e & 1 ? 0x7632u : 0x5410u;
-                                mma16816<KIND>(o[sl * F::VB + q * 4 + e], pa[g],
-                                               __byte_perm(x[0][e >> 1], x[1][e >> 1], sel),
-                                               __byte_perm(x[2][e >> 1], x[3][e >> 1], sel));
+                            for (int e = 0; e < 2; ++e) {
+                                const uint32_t va[4] = {__byte_perm(x[0][e], x[1][e], 0x5410),
+                                                        __byte_perm(x[0][e], x[1][e], 0x7632),
+                                                        __byte_perm(x[2][e], x[3][e], 0x5410),
+                                                        __byte_perm(x[2][e], x[3][e], 0x7632)};
+#pragma unroll
+                                for (int t = 0; t < NT; ++t)
+                                    mma16816<KIND>(o[sl * (F::VB / 2) + q * 2 + e][t], va,
+                                                   pb[g][t][0], pb[g][t][1]);
                             }
                         }
                     }
@@ -593,28 +611,29 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
 
         // ---- the warps' sums of the tile, or of this piece of it
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        for (int i = 0; i < R; ++i) {
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 4);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 8);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 16);
             m[i] -= F::SHIFT;   // l and o belong to this exponent
-            if (c4 == 0) {
-                sm_m[warp * 16 + n8 + 8 * i] = m[i];
-                sm_l[warp * 16 + n8 + 8 * i] = l[i];
+            if (n8 == 0) {
+                sm_m[warp * 16 + i / 2 * 8 + c4 * 2 + (i & 1)] = m[i];
+                sm_l[warp * 16 + i / 2 * 8 + c4 * 2 + (i & 1)] = l[i];
             }
         }
         __syncthreads();
-        float keep[2];
+        float keep[R];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < R; ++i) {
             float mm = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < kFewWarps; ++w) mm = fmaxf(mm, sm_m[w * 16 + n8 + 8 * i]);
+            for (int w = 0; w < kFewWarps; ++w)
+                mm = fmaxf(mm, sm_m[w * 16 + i / 2 * 8 + c4 * 2 + (i & 1)]);
             keep[i] = m[i] == -INFINITY ? 0.f : ex2(m[i] - mm);
-            if (lost) keep[i] = 0.f;
         }
         const bool full = part.begins && part.ends;
         const int which = part.begins;   // 1: tail slot, 0: head slot
-        float* slot = ws.slot(blockIdx.x, which, kFewRows, DP);
+        float* slot = ws.slot(blockIdx.x, which, M, DP);
         if (!full) {
             if (which) {
                 rec.tail = 1;
@@ -625,77 +644,84 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
                 rec.head = part.ends ? 2 : 1;
             }
         }
+        // row of this thread's quads in the second half, and what its sums need
+        const int qr = tid % M;
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kFewWarps; ++w) top = fmaxf(top, sm_m[w * 16 + qr]);
+#pragma unroll
+        for (int w = 0; w < kFewWarps; ++w) {
+            const float x = sm_m[w * 16 + qr];
+            sum += sm_l[w * 16 + qr] * (x == -INFINITY ? 0.f : ex2(x - top));
+        }
+        const int orow = cur.tile * M + (qr < rows ? qr : 0);
+        const int otok = a.by_group.div(orow);
+        const int oh = cur.kvh * a.group + orow - otok * a.group;
+        int l0, h0;
+        attend_range(s.first + otok, s.len, a.causal, a.window, l0, h0);
+        const bool none = l0 >= h0;
+        const float inv = none ? 0.f : 1.f / sum;
+        TQ* out = static_cast<TQ*>(a.out) + (int64_t)(s.q0 + otok) * a.o_ts + (int64_t)oh * a.o_hs;
 #pragma unroll
         for (int pass = 0; pass < DP / F::PD; ++pass) {
 #pragma unroll
-            for (int i = 0; i < F::TILES; ++i)
+            for (int x = 0; x < F::TILES; ++x)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int d = out_dim<DP, KIND>(i, c4 * 2 + e);
+                for (int h = 0; h < 2; ++h) {
+                    const int d = out_dim<DP, KIND>(x, n8, h);
                     if (d / F::PD == pass) {
-                        float* p = joinb + (warp * 16 + n8) * (F::PD + 4) + d % F::PD;
-                        p[0] = o[i][e] * keep[0];
-                        p[8 * (F::PD + 4)] = o[i][2 + e] * keep[1];
+#pragma unroll
+                        for (int i = 0; i < R; ++i)
+                            joinb[(warp * M + i / 2 * 8 + c4 * 2 + (i & 1)) * (F::PD + 4) + d % F::PD] =
+                                o[x][i / 2][2 * h + (i & 1)] * keep[i];
                     }
                 }
             __syncthreads();
-            for (int i = tid; i < 16 * F::PD / 4; i += kFewThreads) {
-                const int r = i / (F::PD / 4), x = i % (F::PD / 4) * 4;
+            // quads of columns, rows inside: a warp's partial sums fill lines
+            for (int i = tid; i < M * F::PD / 4; i += kFewThreads) {
+                const int x = i / M * 4;
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                float mm = -INFINITY, ll = 0.f;
 #pragma unroll
                 for (int w = 0; w < kFewWarps; ++w) {
                     const float4 t = *reinterpret_cast<const float4*>(
-                        joinb + (w * 16 + r) * (F::PD + 4) + x);
+                        joinb + (w * M + qr) * (F::PD + 4) + x);
                     v.x += t.x;
                     v.y += t.y;
                     v.z += t.z;
                     v.w += t.w;
-                    mm = fmaxf(mm, sm_m[w * 16 + r]);
                 }
                 const int d = pass * F::PD + x;
-#pragma unroll
-                for (int w = 0; w < kFewWarps; ++w)
-                    ll += sm_l[w * 16 + r] *
-                          (sm_m[w * 16 + r] == -INFINITY ? 0.f : ex2(sm_m[w * 16 + r] - mm));
                 if (!full) {
-                    *reinterpret_cast<float4*>(slot + (d / 4 * kFewRows + r) * 4) = v;
-                    if (d == 0) {
-                        slot[kFewRows * DP + 2 * r] = mm;
-                        slot[kFewRows * DP + 2 * r + 1] = ll;
-                    }
-                } else if (r < rows) {
-                    const int rr = cur.tile * kFewRows + r;
-                    const int tok = a.by_group.div(rr), h = cur.kvh * a.group + rr - tok * a.group;
-                    int l0, h0;
-                    attend_range(s.first + tok, s.len, a.causal, a.window, l0, h0);
-                    const bool none = l0 >= h0;
-                    const float inv = none ? 0.f : 1.f / ll;
-                    if (d < a.c.dim) {
-                        TQ y[4] = {kv_from_f<TQ>(v.x * inv), kv_from_f<TQ>(v.y * inv),
-                                   kv_from_f<TQ>(v.z * inv), kv_from_f<TQ>(v.w * inv)};
-                        TQ* out = static_cast<TQ*>(a.out) + (int64_t)(s.q0 + tok) * a.o_ts +
-                                  (int64_t)h * a.o_hs + d;
-                        *reinterpret_cast<uint2*>(out) = *reinterpret_cast<uint2*>(y);
-                    }
-                    if (a.lse && d == 0)
-                        a.lse[(int64_t)(s.q0 + tok) * a.q_heads + h] =
-                            none ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
+                    *reinterpret_cast<float4*>(slot + (d / 4 * M + qr) * 4) = v;
+                } else if (qr < rows && d < a.c.dim) {
+                    TQ y[4] = {kv_from_f<TQ>(v.x * inv), kv_from_f<TQ>(v.y * inv),
+                               kv_from_f<TQ>(v.z * inv), kv_from_f<TQ>(v.w * inv)};
+                    *reinterpret_cast<uint2*>(out + d) =
+                        none ? make_uint2(0, 0) : *reinterpret_cast<uint2*>(y);
                 }
             }
             fence_async_smem();   // the ring's next copies come after these writes
             __syncthreads();
         }
+        if (tid < M) {
+            if (!full) {
+                slot[M * DP + 2 * qr] = top;
+                slot[M * DP + 2 * qr + 1] = sum;
+            } else if (a.lse && qr < rows) {
+                a.lse[(int64_t)(s.q0 + otok) * a.q_heads + oh] =
+                    none ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+            }
+        }
         cur.left -= part.used;
-        if (cur.left > 0) attend_next<kFewRows>(a, cur, s);
+        if (cur.left > 0) attend_next<M>(a, cur, s);
     }
     if (lost) kv_flag(a.status, KV_TIMEOUT);
     if (tid == 0) ws.rec[blockIdx.x] = rec;
 }
 
-template <int DP, int KIND, typename TQ>
+template <int DP, int KIND, int NT, typename TQ>
 cudaError_t launch_few(const AttendArgs& a, void* ws, cudaStream_t s) {
-    using F = Few<DP, KIND>;
+    using F = Few<DP, KIND, NT>;
     CUtensorMap kmap, vmap;
     const int box = a.c.page_size < F::KEYS ? a.c.page_size : F::KEYS;
     if (!attend_map(&kmap, a.c, a.c.k, F::SLABB / F::EB, box) ||
@@ -705,34 +731,40 @@ cudaError_t launch_few(const AttendArgs& a, void* ws, cudaStream_t s) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess && (dev < 0 || dev >= 64 || !raised[dev])) {
-        e = cudaFuncSetAttribute(k_attend_few<DP, KIND, TQ>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 F::smem);
+        e = cudaFuncSetAttribute(k_attend_few<DP, KIND, NT, TQ>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, F::smem);
         if (e == cudaSuccess && dev >= 0 && dev < 64) raised[dev] = true;
     }
     if (e != cudaSuccess) return e;
-    k_attend_few<DP, KIND, TQ><<<attend_few_ctas(), kFewThreads, F::smem, s>>>(kmap, vmap, a, ws);
+    k_attend_few<DP, KIND, NT, TQ>
+        <<<attend_few_ctas(), kFewThreads, F::smem, s>>>(kmap, vmap, a, ws);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    return launch_attend_join(a, ws, attend_few_ctas(), kFewRows, DP, s);
+    return launch_attend_join(a, ws, attend_few_ctas(), F::M, DP, s);
 }
 
-template <int DP>
+template <int DP, int NT>
+cudaError_t launch_kind(const AttendArgs& a, void* ws, cudaStream_t s) {
+    if (a.c.type == KV_F16) return launch_few<DP, KIND_F16, NT, __half>(a, ws, s);
+    if (a.c.type == KV_BF16) return launch_few<DP, KIND_BF16, NT, __nv_bfloat16>(a, ws, s);
+    if (a.type == KV_F16) return launch_few<DP, KIND_Q8, NT, __half>(a, ws, s);
+    return launch_few<DP, KIND_Q8, NT, __nv_bfloat16>(a, ws, s);
+}
+
+template <int NT>
 cudaError_t launch_dim(const AttendArgs& a, void* ws, cudaStream_t s) {
-    if (a.c.type == KV_F16) return launch_few<DP, KIND_F16, __half>(a, ws, s);
-    if (a.c.type == KV_BF16) return launch_few<DP, KIND_BF16, __nv_bfloat16>(a, ws, s);
-    if (a.type == KV_F16) return launch_few<DP, KIND_Q8, __half>(a, ws, s);
-    return launch_few<DP, KIND_Q8, __nv_bfloat16>(a, ws, s);
+    const int dp = attend_dim(a.c.dim);
+    if (dp == 64) return launch_kind<64, NT>(a, ws, s);
+    if (dp == 128) return launch_kind<128, NT>(a, ws, s);
+    return launch_kind<256, NT>(a, ws, s);
 }
 
 }  // namespace
 
 int attend_few_ctas() { return 2 * sm_count(); }
 
-cudaError_t launch_attend_few(const AttendArgs& a, void* ws, cudaStream_t s) {
-    const int dp = attend_dim(a.c.dim);
-    if (dp == 64) return launch_dim<64>(a, ws, s);
-    if (dp == 128) return launch_dim<128>(a, ws, s);
-    return launch_dim<256>(a, ws, s);
+cudaError_t launch_attend_few(const AttendArgs& a, int rows, void* ws, cudaStream_t s) {
+    return rows == 8 ? launch_dim<1>(a, ws, s) : launch_dim<2>(a, ws, s);
 }
 
 }  // namespace moeb200
