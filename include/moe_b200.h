@@ -461,9 +461,10 @@ typedef struct moe_b200_kv_batch {
 } moe_b200_kv_batch;
 
 /* status (device int32, may be NULL) receives 0 or a sum of these: a page id
- * outside the cache was met (the rows of that page are skipped), a length
- * reaches past the page table (the rest is skipped), a bounded device-side
- * wait gave up (the outputs are not valid). */
+ * outside the cache was met, a length reaches past the page table (rows there
+ * are neither written nor read; an attention output of that sequence is not
+ * valid, other sequences are not affected), a bounded device-side wait gave up
+ * (no output is valid). */
 #define MOE_B200_KV_BAD_PAGE 1
 #define MOE_B200_KV_BAD_LENGTH 2
 #define MOE_B200_KV_TIMEOUT 4
@@ -509,8 +510,12 @@ MOE_B200_API int moe_b200_attend_workspace(const moe_b200_kv_cache* cache,
  * that attends no token gets zeros and -infinity; rows behind the last
  * sequence are left as they are.  Tokens that a row does not attend never
  * reach its result, whatever they hold.  Scores, softmax and sums are fp32;
- * Q8_0 values enter as scale * code rounded to binary16, probabilities as
- * 16-bit values. */
+ * Q8_0 values enter as scale * code rounded to binary16 (a scale of 512 or
+ * more can overflow it; moe_b200_kv_write stores none), probabilities as
+ * 16-bit values.  Two kernels, three for many rows per sequence over a Q8_0
+ * cache whose expanded pages (4 bytes a value pair for max_pages pages of
+ * every sequence, part of the workspace) stay within 1 GB.  Results do not
+ * depend on other calls and repeat bit for bit. */
 MOE_B200_API int moe_b200_attend(const moe_b200_kv_cache* cache, const moe_b200_kv_batch* batch,
                                  int32_t type, const void* q, int64_t q_token_stride,
                                  int64_t q_head_stride, int32_t q_heads, void* out,

@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(256) k_attend_expand(KvBatch b, KvCache c, __h
     const int first = page << c.page_shift;
     // pages behind the sequence, or before the first row's window
     if (first >= len || n <= 0) return;
-    if (window > 0 && first + c.page_size <= len - n - window + 1) return;
+    if (window > 0 && (int64_t)first + c.page_size <= (int64_t)len - n - window + 1) return;
     const int id = kv_page(b, c, seq, page, status);
     if (id < 0) return;
     const int units = (c.heads << c.page_shift) * c.dim >> 4;

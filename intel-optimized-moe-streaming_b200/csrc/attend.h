@@ -110,7 +110,7 @@ cudaError_t launch_attend_join(const AttendArgs& a, void* ws, int ctas, int M, i
 __host__ __device__ __forceinline__ void attend_range(int pos, int len, int causal, int window,
                                                       int& lo, int& hi) {
     hi = causal && pos + 1 < len ? pos + 1 : len;
-    lo = window > 0 && pos - window + 1 > 0 ? pos - window + 1 : 0;
+    lo = window > 0 && pos >= window ? pos - window + 1 : 0;
     if (hi < lo) hi = lo;
 }
 
@@ -124,7 +124,8 @@ struct AttendSeq {
 __device__ __forceinline__ AttendSeq attend_seq(const AttendArgs& a, int b, unsigned* status) {
     AttendSeq s;
     int q0 = __ldg(a.b.q_start + b), q1 = __ldg(a.b.q_start + b + 1);
-    const int raw = __ldg(a.b.kv_lens + b);
+    int raw = __ldg(a.b.kv_lens + b);
+    raw = raw > 0 ? raw : 0;
     q0 = q0 > 0 ? q0 : 0;
     q1 = q1 < a.b.T ? q1 : a.b.T;
     s.q0 = q0;
@@ -223,7 +224,7 @@ __device__ AttendCursor attend_place(const AttendArgs& a, AttendScratch& scratch
             q.len = __shfl_sync(0xffffffffu, s.len, from);
             q.first = __shfl_sync(0xffffffffu, s.first, from);
             const int n = __shfl_sync(0xffffffffu, tiles, from);
-            int part = 0;
+            int64_t part = 0;
             for (int t = lane; t < n; t += 32) {
                 int lo, hi;
                 attend_units<M, KT>(a, q, t, lo, hi);

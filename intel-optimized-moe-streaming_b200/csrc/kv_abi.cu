@@ -89,28 +89,40 @@ int moe_b200_kv_write(const moe_b200_kv_cache* cache, const moe_b200_kv_batch* b
                       const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
                       int64_t v_token_stride, int64_t v_head_stride, int32_t* status,
                       void* stream) {
-    return kv_rows(true, cache, batch, type, const_cast<void*>(k), k_token_stride, k_head_stride,
-                   const_cast<void*>(v), v_token_stride, v_head_stride, status, stream);
+    try {
+        return kv_rows(true, cache, batch, type, const_cast<void*>(k), k_token_stride, k_head_stride,
+                       const_cast<void*>(v), v_token_stride, v_head_stride, status, stream);
+    } catch (...) {
+        return ST_INTERNAL;
+    }
 }
 
 int moe_b200_kv_read(const moe_b200_kv_cache* cache, const moe_b200_kv_batch* batch, int32_t type,
                      void* k, int64_t k_token_stride, int64_t k_head_stride, void* v,
                      int64_t v_token_stride, int64_t v_head_stride, int32_t* status,
                      void* stream) {
-    return kv_rows(false, cache, batch, type, k, k_token_stride, k_head_stride, v, v_token_stride,
-                   v_head_stride, status, stream);
+    try {
+        return kv_rows(false, cache, batch, type, k, k_token_stride, k_head_stride, v, v_token_stride,
+                       v_head_stride, status, stream);
+    } catch (...) {
+        return ST_INTERNAL;
+    }
 }
 
 int moe_b200_attend_workspace(const moe_b200_kv_cache* cache, const moe_b200_kv_batch* batch,
                               int32_t q_heads, size_t* bytes) {
-    KvCache c;
-    KvBatch b;
-    int st = check_cache(cache, &c);
-    if (st == ST_OK) st = check_batch(batch, &b);
-    if (st != ST_OK) return st;
-    if (!bytes || q_heads < 1 || q_heads % c.heads) return ST_ARG;
-    *bytes = attend_workspace_bytes(b, c, q_heads);
-    return ST_OK;
+    try {
+        KvCache c;
+        KvBatch b;
+        int st = check_cache(cache, &c);
+        if (st == ST_OK) st = check_batch(batch, &b);
+        if (st != ST_OK) return st;
+        if (!bytes || q_heads < 1 || q_heads % c.heads) return ST_ARG;
+        *bytes = attend_workspace_bytes(b, c, q_heads);
+        return ST_OK;
+    } catch (...) {
+        return ST_INTERNAL;
+    }
 }
 
 int moe_b200_attend(const moe_b200_kv_cache* cache, const moe_b200_kv_batch* batch, int32_t type,
@@ -118,43 +130,47 @@ int moe_b200_attend(const moe_b200_kv_cache* cache, const moe_b200_kv_batch* bat
                     void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse,
                     float scale, int32_t causal, int32_t window, void* workspace,
                     size_t workspace_bytes, int32_t* status, void* stream) {
-    AttendArgs a{};
-    int st = check_cache(cache, &a.c);
-    if (st == ST_OK) st = check_batch(batch, &a.b);
-    if (st != ST_OK) return st;
-    if (type != KV_F16 && type != KV_BF16) return ST_TYPE;
-    if (a.c.type != Q8_0 && a.c.type != type) return ST_TYPE;
-    if (q_heads < 1 || q_heads > 65536 || q_heads % a.c.heads) return ST_ARG;
-    if ((causal != 0 && causal != 1) || window < 0 || (window > 0 && !causal)) return ST_ARG;
-    if (!(scale >= -3.402823466e38f && scale <= 3.402823466e38f)) return ST_ARG;
-    if ((int64_t)a.b.T * q_heads > 0x7fffffffll) return ST_ARG;
-    if (a.b.T > 0 && (!q || !out || !workspace)) return ST_ARG;
-    if (!rows_aligned(q, q_token_stride, q_head_stride, 2) ||
-        !rows_aligned(out, out_token_stride, out_head_stride, 2) || ((uintptr_t)lse & 3u) ||
-        ((uintptr_t)status & 3u) || ((uintptr_t)workspace & 255u))
-        return ST_ALIGN;
-    if (a.b.T > 0 && workspace_bytes < attend_workspace_bytes(a.b, a.c, q_heads))
-        return ST_WORKSPACE;
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    st = clear_status(status, s);
-    if (st != ST_OK || a.b.T == 0 || a.b.B == 0) return st;
-    a.q = q;
-    a.out = out;
-    a.lse = lse;
-    a.q_ts = q_token_stride;
-    a.q_hs = q_head_stride;
-    a.o_ts = out_token_stride;
-    a.o_hs = out_head_stride;
-    a.type = type;
-    a.q_heads = q_heads;
-    a.group = q_heads / a.c.heads;
-    a.by_group = FastDiv(a.group);
-    a.scale = scale;
-    a.causal = causal;
-    a.window = window;
-    a.status = reinterpret_cast<unsigned*>(status);
-    const cudaError_t e = launch_attend(a, workspace, s);
-    return e == cudaSuccess ? ST_OK : cuda_fail(e);
+    try {
+        AttendArgs a{};
+        int st = check_cache(cache, &a.c);
+        if (st == ST_OK) st = check_batch(batch, &a.b);
+        if (st != ST_OK) return st;
+        if (type != KV_F16 && type != KV_BF16) return ST_TYPE;
+        if (a.c.type != Q8_0 && a.c.type != type) return ST_TYPE;
+        if (q_heads < 1 || q_heads > 65536 || q_heads % a.c.heads) return ST_ARG;
+        if ((causal != 0 && causal != 1) || window < 0 || (window > 0 && !causal)) return ST_ARG;
+        if (!(scale >= -3.402823466e38f && scale <= 3.402823466e38f)) return ST_ARG;
+        if ((int64_t)a.b.T * q_heads > 0x7fffffffll) return ST_ARG;
+        if (a.b.T > 0 && (!q || !out || !workspace)) return ST_ARG;
+        if (!rows_aligned(q, q_token_stride, q_head_stride, 2) ||
+            !rows_aligned(out, out_token_stride, out_head_stride, 2) || ((uintptr_t)lse & 3u) ||
+            ((uintptr_t)status & 3u) || ((uintptr_t)workspace & 255u))
+            return ST_ALIGN;
+        if (a.b.T > 0 && workspace_bytes < attend_workspace_bytes(a.b, a.c, q_heads))
+            return ST_WORKSPACE;
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        st = clear_status(status, s);
+        if (st != ST_OK || a.b.T == 0 || a.b.B == 0) return st;
+        a.q = q;
+        a.out = out;
+        a.lse = lse;
+        a.q_ts = q_token_stride;
+        a.q_hs = q_head_stride;
+        a.o_ts = out_token_stride;
+        a.o_hs = out_head_stride;
+        a.type = type;
+        a.q_heads = q_heads;
+        a.group = q_heads / a.c.heads;
+        a.by_group = FastDiv(a.group);
+        a.scale = scale;
+        a.causal = causal;
+        a.window = window;
+        a.status = reinterpret_cast<unsigned*>(status);
+        const cudaError_t e = launch_attend(a, workspace, s);
+        return e == cudaSuccess ? ST_OK : cuda_fail(e);
+    } catch (...) {
+        return ST_INTERNAL;
+    }
 }
 
 }  // extern "C"

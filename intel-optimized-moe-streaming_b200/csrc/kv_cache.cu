@@ -133,7 +133,7 @@ __device__ __forceinline__ void cta_slots(const KvBatch& b, const KvCache& c, in
     int64_t slot = -2;
     if (q0 <= t && t < q1) {
         slot = -1;
-        const int pos = __ldg(b.kv_lens + s) - q1 + t;
+        const int pos = max(__ldg(b.kv_lens + s), 0) - q1 + t;
         if (pos >= 0) {
             const int page = kv_page(b, c, s, pos >> c.page_shift, status);
             if (page >= 0)

@@ -304,6 +304,98 @@ def test_repeats_are_equal():
         assert torch.equal(cache.attend(batch, q), first)
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16", "q8_f16"])
+@pytest.mark.parametrize("dim,new,kv", [(256, [64], [2560]), (256, [129], [700]),
+                                        (128, [300], [2560]), (64, [400, 3], [900, 800])])
+def test_split_tiles_repeat(dim, new, kv, kind):
+    """Short stretches of many tiles per CTA: every start and end of a tile
+    meets every phase of the pipeline; twenty runs, one result."""
+    cache, batch, q = build(new, kv, 64, 1, dim, 8, kind, seed=21)
+    first = cache.attend(batch, q)
+    check(cache, batch, q, first, None, new, kv, dim ** -0.5)
+    for _ in range(20):
+        assert torch.equal(cache.attend(batch, q), first)
+
+
+@pytest.mark.parametrize("kind", ["q8_f16", "q8_bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_quantised_chunk_under_a_wide_table(dim, kind):
+    """A page table so wide that the pages are not expanded in the workspace:
+    the kernel decodes the codes of several tiles itself, to the same bits."""
+    new, kv = [200, 90], [700, 95]
+    cache, batch, q = build(new, kv, 256, 2, dim, 8, kind, seed=22)
+    narrow = cache.attend(batch, q)
+    check(cache, batch, q, narrow, None, new, kv, dim ** -0.5)
+    wide = torch.full((2, 1100 * 256 // dim), -1, dtype=torch.int32, device=DEV)
+    wide[:, :batch.max_pages] = batch.page_table
+    out = cache.attend(KVBatch(batch.q_start, batch.kv_lens, wide), q)
+    assert torch.equal(out, narrow)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3])
+@pytest.mark.parametrize("kind", ["f16", "bf16", "q8_bf16"])
+@pytest.mark.parametrize("name", ["decode", "drafts", "chunk", "chunk_256"])
+def test_unusual_scales(name, kind, scale):
+    """Zero: the mean of the attended values; negative: the smallest products
+    weigh most."""
+    new, kv, page, heads, dim, q_heads = CASES[name]
+    cache, batch, q = build(new, kv, page, heads, dim, q_heads, kind, seed=15)
+    out = cache.attend(batch, q, scale=scale, window=(1 << 31) - 1)
+    check(cache, batch, q, out, None, new, kv, scale)
+
+
+def test_many_short_sequences():
+    """More sequences than threads, empty ones among them (at both ends), and
+    one long; rows of one sequence reaching other tiles than their neighbours."""
+    new = [0, 0] + [i % 3 for i in range(700)] + [40] + [1] * 50 + [0]
+    kv = [n + (7 * i) % 90 for i, n in enumerate(new)]
+    for kind in ("bf16", "q8_f16"):
+        cache, batch, q = build(new, kv, 16, 2, 64, 4, kind, seed=16)
+        lse = torch.empty(q.shape[:2], device=DEV)
+        out = cache.attend(batch, q, lse=lse)
+        check(cache, batch, q, out, lse, new, kv, 0.125)
+
+
+@pytest.mark.parametrize("n", [1, 70])
+def test_shared_pages(n):
+    """Two sequences whose tables share the pages of a common beginning."""
+    kv = [64 + n, 64 + n]
+    cache, batch, q = build([n, n], kv, 16, 2, 128, 8, "f16", seed=17)
+    batch.page_table[1, :4] = batch.page_table[0, :4]
+    out = cache.attend(batch, q)
+    check(cache, batch, q, out, None, [n, n], kv, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("n", [1, 100])
+def test_other_stream(n):
+    cache, batch, q = build([n], [900], 16, 2, 128, 8, "q8_bf16", seed=18)
+    want = cache.attend(batch, q)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    outs = [cache.attend(batch, q, stream=s) for _ in range(4)]
+    s.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("n", [1, 3, 90])
+def test_infinite_scores(n, kind):
+    """Rows whose scores are all minus infinity have no softmax: NaN, as in
+    the definition; a single such key gets no weight."""
+    cache, batch, q = build([n, n], [n + 200, n + 200], 16, 1, 64, 4, kind, seed=19)
+    q.abs_()
+    cache.k[batch.page_table[0].long()] = -float("inf")
+    pg = int(batch.page_table[1, 2])
+    cache.k[pg, 0, 5] = -float("inf")
+    out = cache.attend(batch, q)
+    assert out[:n].isnan().all()
+    assert out[n:].isfinite().all()
+    clean = cache.k.clone()
+    cache.k[pg, 0, 5] = torch.finfo(cache.k.dtype).min / 64
+    assert torch.equal(cache.attend(batch, q)[n:], out[n:])
+    cache.k.copy_(clean)
+
+
 @pytest.mark.parametrize("kind", ["f16", "q8_bf16"])
 def test_serving_run(kind):
     """A prompt in chunks, then single tokens: write and attend step by step,
