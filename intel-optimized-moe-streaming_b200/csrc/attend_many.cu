@@ -3,14 +3,15 @@
 //
 // 4 D operations per (row, key, head) against 2 D values read per key of a
 // whole tile: bound by the tensor cores, and next to them by the exponentials
-// (128 x 128 scores take 1024 cycles of an SM's special function units, the
+// (128 x 128 scores take 1043 cycles of an SM's special function units, the
 // two products of a 128-value head 1024 cycles of its tensor core).
 //
 // A CTA (one per SM) holds the query tile of a group's rows -- two of 128 rows
 // for head dimensions up to 128, one above -- and walks units of 128 keys.
 // Tensor memory has the two score tiles S (128 columns each) and the output
 // sums O (2 x DP columns, or 256); the probabilities overwrite their scores as
-// 16-bit values and are the value product's A operand from there.
+// 16-bit values, 64 keys at a time, and are the value product's A operand from
+// there.
 //   warps 0-7   softmax: a thread owns a row (one of two tiles; or, with one
 //               tile, half the columns of a row, the two halves agreeing on
 //               the maximum through shared memory).  The maximum in use is
@@ -20,12 +21,20 @@
 //   warp 8      copies: a ring of NST stages of up to 32 KB (keys x 64-value
 //               slabs, 128-byte swizzle) filled by tensor copies, one lane per
 //               page piece and slab
-//   warp 9      one lane issues all products: with two tiles S_t(j + 1) follows
-//               the value product of tile t, so that a tile's softmax runs
-//               under the other tile's products; with one tile S(j + 1) comes
-//               before the value product of j
+//   warp 9      issues all products: with two tiles S_t(j + 1) follows the
+//               value product of tile t, so that a tile's softmax runs under
+//               the other tile's products; with one tile there are two score
+//               buffers and S(j + 1) comes before the value product of j
+//   warps 10-11 look through the values of units that not all rows attend
 //   warps 12-15 (Q8_0) instead of the copies: codes are loaded a stage ahead
 //               into registers, become binary16 and go to the ring
+// Measured (1965 MHz at the start, power-capped below it later): 2048 rows
+// over 8k keys, 32/8 heads x 128, 230 us = 1047 TFLOP/s, 3550 cycles a unit of
+// two tiles: 470 maximum, 1690 exponentials (1400 alone: the tiles' phases
+// meet), 200 hand-over, 1190 until the next scores, which wait for the last
+// half of the value product because P stands on S.  4096 rows over 16k keys,
+// 16/2 heads x 256, 920 us = 1046 TFLOP/s, 3300 cycles a unit: 128 KB of keys
+// and values through the ring per unit and SM, 8.4 TB/s out of L2 in all.
 #include "attend_mma.cuh"
 #include "launch.h"
 
@@ -685,7 +694,7 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             // products' operands are then known to be uniform and stay in
             // uniform registers.  Issued by a lane that branched off alone,
             // each took about 120 cycles, twice what a 128 x 128 x 16 product
-            // needs (256-row tiles of 128 values: 940 -> TF TFLOP/s).
+            // needs.
             uint32_t it = 0, seg = 0;
             int stage0 = 0;
             auto wait_stage = [&](int n) {

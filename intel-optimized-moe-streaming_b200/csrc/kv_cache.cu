@@ -13,7 +13,10 @@
 // two threads own a Q8_0 block.  A CTA looks up the slots of its up to 32
 // tokens, one lane per token, then all its threads walk the units of those
 // tokens, keys and values in the same iteration so that both loads are in
-// flight.
+// flight.  Measured, 105k tokens x 8 heads x 128: write as Q8_0 139 us (4.75
+// TB/s), read back as bfloat16 125 us (5.3 TB/s); with 16 tokens looked up by
+// two rounds of a warp each, and no row loaded before its slot is known, 150 us
+// and 127 us.
 #include <type_traits>
 
 #include "kv.cuh"
