@@ -189,7 +189,7 @@ struct AttendScratch {
 
 // Finds the stretch of CTA `cta` of `ctas`.  A tile is COST + units long (COST:
 // what starting and ending it takes, in units; a cut inside that part gives
-// the whole tile to the later CTA), once per key/value head.  A thread sums
+// the whole tile to the later CTA), once per key/value head.  A lane sums
 // its share of the sequences, the tiles of a long one being spread over its
 // warp; a block scan places the shares, and the warp whose share holds the
 // stretch's start walks to it.  Returns in every thread; left = 0: nothing to
@@ -199,13 +199,17 @@ template <int M, int KT, int COST, int THREADS>
 __device__ AttendCursor attend_place(const AttendArgs& a, AttendScratch& scratch, int cta,
                                      int ctas, unsigned* status) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int share = (a.b.B + THREADS - 1) / THREADS;
+    // consecutive sequences to a warp, and of these to a lane
+    constexpr int WARPS = THREADS / 32;
+    const int per_warp = (a.b.B + WARPS - 1) / WARPS, share = (per_warp + 31) / 32;
+    const int warp_end = min((warp + 1) * per_warp, a.b.B);
+    const int b_lane = warp * per_warp + lane * share;
     int64_t mine = 0;
     for (int i = 0; i < share; ++i) {
-        const int b = tid * share + i;
+        const int b = b_lane + i;
         AttendSeq s{};
         int tiles = 0;
-        if (b < a.b.B) {
+        if (b < warp_end) {
             s = attend_seq(a, b, cta == 0 ? status : nullptr);
             tiles = attend_tiles<M>(a, s);
         }
@@ -252,21 +256,30 @@ __device__ AttendCursor attend_place(const AttendArgs& a, AttendScratch& scratch
         if (w < warp) before += scratch.warp_total[w];
         total += scratch.warp_total[w];
     }
-    const int64_t least = COST + 1;
-    int64_t active = (total + least - 1) / least;
-    active = active < ctas ? active : ctas;
+    // equal stretches, the first `rest` one longer; a tile with a unit is at
+    // least COST + 1 long.  Lines below 2^32, all but the longest, are divided
+    // in 32 bits.
     int64_t start = -1, end = -1;
-    if (cta < active) {
-        start = total * cta / active;
-        end = total * (cta + 1) / active;
+    if (total <= 0xffffffffll) {
+        const uint32_t n = (uint32_t)total, most = (n + COST) / (COST + 1);
+        const uint32_t active = most < (uint32_t)ctas ? most : (uint32_t)ctas;
+        if ((uint32_t)cta < active) {
+            const uint32_t each = n / active, rest = n - each * active;
+            start = (int64_t)each * cta + ((uint32_t)cta < rest ? (uint32_t)cta : rest);
+            end = start + each + ((uint32_t)cta < rest);
+        }
+    } else {
+        const int64_t each = total / ctas, rest = total - each * ctas;
+        start = each * cta + (cta < rest ? cta : rest);
+        end = start + each + (cta < rest);
     }
     const unsigned owner = __ballot_sync(0xffffffffu, start >= before && start < before + mine);
     if (owner) {
         const int from = __ffs(owner) - 1;
         int64_t skip = start - __shfl_sync(0xffffffffu, before, from);
-        const int b0 = (warp * 32 + from) * share;
+        const int b0 = warp * per_warp + from * share;
         bool done = false;
-        for (int b = b0; b < b0 + share && b < a.b.B && !done; ++b) {
+        for (int b = b0; b < b0 + share && b < warp_end && !done; ++b) {
             const AttendSeq s = attend_seq(a, b, nullptr);
             const int tiles = attend_tiles<M>(a, s);
             for (int t0 = 0; t0 < tiles && !done; t0 += 32) {

@@ -133,6 +133,13 @@ __device__ __forceinline__ int out_dim(int i, int n, int h) {
     return i * 16 + n + 8 * h;
 }
 
+// A pair of 16-bit values, in its place among the copies.
+__device__ __forceinline__ uint32_t ldg_first(const void* p) {
+    uint32_t v;
+    asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+
 // Transposes an 8 x 8 matrix of 16-bit values held as accumulator pairs.
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
     uint32_t t;
@@ -238,57 +245,61 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
             out_slot = out_slot + 1 == F::NS ? 0 : out_slot + 1;
             out_phase ^= out_slot == 0;
         };
+        // Queries as B operands: this thread's are of row n8 of each row tile;
+        // bf16 ones over a Q8_0 cache become binary16 after an exact scaling of
+        // the row to a maximum in [1, 2).  The four warps hold the same ones.
+        // They are asked for before the ring's first copies, which would keep
+        // them waiting until all of those have come (5 us over 33 sequences).
+        uint2 qraw[NT][DP / 16];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int r = t * 8 + n8;
+            const int rr = cur.tile * M + (r < rows ? r : 0);
+            const int tok = a.by_group.div(rr);
+            const TQ* q = static_cast<const TQ*>(a.q) + (int64_t)(s.q0 + tok) * a.q_ts +
+                          (int64_t)(cur.kvh * a.group + rr - tok * a.group) * a.q_hs;
+#pragma unroll
+            for (int st = 0; st < DP / 16; ++st) {   // the two registers of 16 dimensions
+                const int d = F::Q8 ? (st >> 2) * 64 + c4 * 16 + (st & 3) * 4 : st * 16 + c4 * 2;
+                const int d2 = d + (F::Q8 ? 2 : 8);
+                qraw[t][st].x = r < rows && d < a.c.dim ? ldg_first(q + d) : 0u;
+                qraw[t][st].y = r < rows && d2 < a.c.dim ? ldg_first(q + d2) : 0u;
+            }
+        }
         look_up(0);
 #pragma unroll 1
         for (int e = 0; e < F::NS; ++e) fetch(e);
 
-        // Queries as B operands: this thread's are of row n8 of each row tile;
-        // bf16 ones over a Q8_0 cache become binary16 after an exact scaling of
-        // the row to a maximum in [1, 2).  The four warps hold the same ones.
         uint2 qreg[F::QSM ? 1 : DP / 16][NT];
         float factor[NT];
         {
             const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const int r = t * 8 + n8;
-                const int rr = cur.tile * M + (r < rows ? r : 0);
-                const int tok = a.by_group.div(rr);
-                const TQ* q = static_cast<const TQ*>(a.q) + (int64_t)(s.q0 + tok) * a.q_ts +
-                              (int64_t)(cur.kvh * a.group + rr - tok * a.group) * a.q_hs;
-                auto pair = [&](int d) {
-                    return r < rows && d < a.c.dim ? *reinterpret_cast<const uint32_t*>(q + d) : 0u;
-                };
-                auto both = [&](int st) {   // the two registers of 16 dimensions
-                    const int d = F::Q8 ? (st >> 2) * 64 + c4 * 16 + (st & 3) * 4 : st * 16 + c4 * 2;
-                    return make_uint2(pair(d), pair(d + (F::Q8 ? 2 : 8)));
-                };
                 factor[t] = 1.f;
+                if constexpr (CONVERT) {
+                    float top = 0.f;
+#pragma unroll
+                    for (int st = 0; st < DP / 16; ++st) {
+                        const uint2 w = qraw[t][st];
+                        top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w.x << 16)),
+                                               fabsf(__uint_as_float(w.x & 0xffff0000u))));
+                        top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w.y << 16)),
+                                               fabsf(__uint_as_float(w.y & 0xffff0000u))));
+                    }
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    factor[t] = row_factor(top);
+                }
                 auto convert = [&](uint32_t w) {
                     if constexpr (CONVERT)
                         w = pack16<KIND_F16>(__uint_as_float(w << 16) * factor[t],
                                              __uint_as_float(w & 0xffff0000u) * factor[t]);
                     return w ^ flip;
                 };
-                uint2 w[DP / 16];
-#pragma unroll
-                for (int st = 0; st < DP / 16; ++st) w[st] = both(st);
-                if constexpr (CONVERT) {
-                    float top = 0.f;
-#pragma unroll
-                    for (int st = 0; st < DP / 16; ++st) {
-                        top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[st].x << 16)),
-                                               fabsf(__uint_as_float(w[st].x & 0xffff0000u))));
-                        top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[st].y << 16)),
-                                               fabsf(__uint_as_float(w[st].y & 0xffff0000u))));
-                    }
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    factor[t] = row_factor(top);
-                }
 #pragma unroll
                 for (int st = 0; st < DP / 16; ++st) {
-                    const uint2 x = make_uint2(convert(w[st].x), convert(w[st].y));
+                    const uint2 x = make_uint2(convert(qraw[t][st].x), convert(qraw[t][st].y));
                     if constexpr (F::QSM) {
                         if ((st & 3) == warp) qf[(st * NT + t) * 32 + lane] = x;
                     } else {
