@@ -187,15 +187,16 @@ struct AttendScratch {
     AttendCursor found;
 };
 
-// Finds the stretch of CTA `cta` of `ctas`.  A tile is COST + units long (COST:
-// what starting and ending it takes, in units; a cut inside that part gives
-// the whole tile to the later CTA), once per key/value head.  A lane sums
+// Finds the stretch of CTA `cta` of `ctas`, none shorter than LEAST.  A tile is
+// COST + units long (COST: what starting and ending it takes, in units; a cut
+// inside that part gives the whole tile to the later CTA), once per key/value
+// head.  A lane sums
 // its share of the sequences, the tiles of a long one being spread over its
 // warp; a block scan places the shares, and the warp whose share holds the
 // stretch's start walks to it.  Returns in every thread; left = 0: nothing to
 // do.  The scratch is shared memory that the caller may use for something else
 // afterwards.
-template <int M, int KT, int COST, int THREADS>
+template <int M, int KT, int COST, int LEAST, int THREADS>
 __device__ AttendCursor attend_place(const AttendArgs& a, AttendScratch& scratch, int cta,
                                      int ctas, unsigned* status) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -256,12 +257,11 @@ __device__ AttendCursor attend_place(const AttendArgs& a, AttendScratch& scratch
         if (w < warp) before += scratch.warp_total[w];
         total += scratch.warp_total[w];
     }
-    // equal stretches, the first `rest` one longer; a tile with a unit is at
-    // least COST + 1 long.  Lines below 2^32, all but the longest, are divided
-    // in 32 bits.
+    // equal stretches, the first `rest` one longer.  Lines below 2^32, all but
+    // the longest, are divided in 32 bits.
     int64_t start = -1, end = -1;
     if (total <= 0xffffffffll) {
-        const uint32_t n = (uint32_t)total, most = (n + COST) / (COST + 1);
+        const uint32_t n = (uint32_t)total, most = (n + LEAST - 1) / LEAST;
         const uint32_t active = most < (uint32_t)ctas ? most : (uint32_t)ctas;
         if ((uint32_t)cta < active) {
             const uint32_t each = n / active, rest = n - each * active;

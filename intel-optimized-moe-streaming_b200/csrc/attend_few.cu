@@ -24,10 +24,10 @@
 // scale * code in binary16.  The order of head dimensions within the key
 // product, and of output rows, is permuted so that a thread takes its codes
 // as 16 consecutive bytes and no transposing load is needed.
-// Measured: 64 contexts of 3.5k tokens, 32/8 heads x 128, bf16: 167 us, 5.44
-// TB/s (HBM); 24 contexts of 18k tokens, 16/2 heads x 256, Q8_0: 115 us, 4.12
-// TB/s (some 1400 instructions a warp and 32 keys, most of them decoding, at
-// two warps a scheduler); one context of 1000 tokens: 15 us (the start of two
+// Measured: 64 contexts of 3.5k tokens, 32/8 heads x 128, bf16: 151 us, 6.03
+// TB/s (HBM); 33 x 5 drafted rows over 5 to 3000 tokens, 28/4 x 128, binary16:
+// 32 us; 24 contexts of 18k tokens, 16/2 heads x 256, Q8_0: 111 us, 4.28 TB/s (some 1400 instructions a warp and 32 keys, most of them decoding, at
+// two warps a scheduler); one context of 1000 tokens: 14 us (the start of two
 // kernels, 16 pieces a head).
 #include "attend_mma.cuh"
 #include "launch.h"
@@ -38,7 +38,12 @@ namespace {
 
 constexpr int kFewWarps = 4;
 constexpr int kFewThreads = kFewWarps * 32;
-constexpr int kFewCost = 0;                      // of a tile, in units
+// Starting a tile (its queries, the ring's first copies) and ending it (the join
+// of the warps) take about as long as two units: with 0, 1, 2, 3, 4 the 33 x 5
+// drafted rows took 52, 41, 40, 40, 42 us, the 64 ragged contexts 181, 176, 173,
+// 175, 173, the 24 contexts in Q8_0 122, 115, 114, 116, 116 (single calls after
+// a flush of L2).
+constexpr int kFewCost = 2;
 constexpr uint32_t kFewPolls = 1u << 21;
 
 // NT: row tiles of 8.
@@ -177,7 +182,7 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
 
     const int ctas = gridDim.x;
     AttendWs ws(wsp, ctas);
-    AttendCursor cur = attend_place<M, F::UNIT, kFewCost, kFewThreads>(
+    AttendCursor cur = attend_place<M, F::UNIT, kFewCost, 1, kFewThreads>(
         a, *reinterpret_cast<AttendScratch*>(sm), blockIdx.x, ctas, a.status);
     fence_async_smem();   // the scratch lies in the ring
     AttendRecord rec{};
@@ -189,6 +194,7 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
 
     while (cur.left > 0) {
         const AttendPart part = attend_part<M, F::UNIT, kFewCost>(a, cur, s);
+        if (part.take <= 0) break;   // the stretch ends before the tile's first unit
         const int u0 = part.u0, take = part.take;
         const int rows = s.n * a.group - cur.tile * M;   // valid rows: the first `rows`
         const AttendTile tile = attend_tile(a, s, cur.tile * M, M);

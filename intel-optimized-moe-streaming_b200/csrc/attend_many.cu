@@ -301,7 +301,7 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
     const int ctas = gridDim.x;
     AttendWs ws(wsp, ctas);
     Walk<DP, KIND> w;
-    w.cur = attend_place<F::M, kManyKeys, kManyCost, F::THREADS>(
+    w.cur = attend_place<F::M, kManyKeys, kManyCost, kManyCost + 1, F::THREADS>(
         a, *reinterpret_cast<AttendScratch*>(sm), blockIdx.x, ctas, a.status);
     fence_async_smem();   // the scratch lies where the queries go
     tc_fence_before();
