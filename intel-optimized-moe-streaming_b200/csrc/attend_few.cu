@@ -25,10 +25,11 @@
 // product, and of output rows, is permuted so that a thread takes its codes
 // as 16 consecutive bytes and no transposing load is needed.
 // Measured: 64 contexts of 3.5k tokens, 32/8 heads x 128, bf16: 151 us, 6.03
-// TB/s (HBM); 33 x 5 drafted rows over 5 to 3000 tokens, 28/4 x 128, binary16:
-// 32 us; 24 contexts of 18k tokens, 16/2 heads x 256, Q8_0: 111 us, 4.28 TB/s (some 1400 instructions a warp and 32 keys, most of them decoding, at
-// two warps a scheduler); one context of 1000 tokens: 14 us (the start of two
-// kernels, 16 pieces a head).
+// TB/s (HBM); 33 x 5 drafted rows over 5 to 3000 tokens, 16/8 x 64, binary16:
+// 32 us, 3.39 TB/s; 24 contexts of 18k tokens, 16/2 heads x 256, Q8_0: 111 us,
+// 4.28 TB/s (some 1400 instructions a warp and 32 keys, most of them decoding,
+// at two warps a scheduler); one context of 1000 tokens: 14 us (the start of
+// two kernels, 16 pieces a head).
 #include "attend_mma.cuh"
 #include "launch.h"
 
@@ -45,6 +46,9 @@ constexpr int kFewThreads = kFewWarps * 32;
 // a flush of L2).
 constexpr int kFewCost = 2;
 constexpr uint32_t kFewPolls = 1u << 21;
+
+// Codes that a thread takes of a Q8_0 value row.
+template <int DP> constexpr int kFewCodes = DP >= 128 ? 16 : 8;
 
 // NT: row tiles of 8.
 template <int DP, int KIND, int NT>
@@ -65,7 +69,6 @@ struct Few {
     // ring entries: at most 102 KB per CTA (two CTAs share an SM), and 8
     static constexpr int FIT = 104448 / (kFewWarps * (TILEB + SCALEB));
     static constexpr int NS = FIT > 8 ? 8 : FIT;
-    static constexpr int VB = Q8 ? (DP >= 128 ? 16 : 8) : 8;   // codes a thread takes of a value row
     static constexpr int TILES = DP / 16;                      // output tiles of 16 dimensions
     static constexpr bool QSM = NT * DP > 256;                 // queries in shared memory
     // binary16 probabilities are taken 2^15 times as large (the largest is
@@ -134,7 +137,8 @@ template <int DP, int KIND>
 __device__ __forceinline__ int out_dim(int i, int n, int h) {
     using F = Few<DP, KIND, 1>;
     if constexpr (F::Q8)
-        return (i / (F::VB / 2)) * (F::VB * 8) + n * F::VB + i % (F::VB / 2) * 2 + h;
+        constexpr int C = kFewCodes<DP>;
+        return (i / (C / 2)) * (C * 8) + n * C + i % (C / 2) * 2 + h;
     return i * 16 + n + 8 * h;
 }
 
@@ -587,10 +591,10 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
                     }
                 }
             } else {
-                constexpr int W = F::VB / 4;   // 32-bit words of codes per key
+                constexpr int W = kFewCodes<DP> / 4;   // 32-bit words of codes per key
 #pragma unroll
-                for (int sl = 0; sl < DP / (F::VB * 8); ++sl) {
-                    const int blk = (sl * F::VB * 8 + n8 * F::VB) >> 5;
+                for (int sl = 0; sl < DP / (kFewCodes<DP> * 8); ++sl) {
+                    const int blk = (sl * kFewCodes<DP> * 8 + n8 * kFewCodes<DP>) >> 5;
 #pragma unroll
                     for (int g = 0; g < F::G; ++g) {
                         uint32_t w[4][W];
@@ -599,7 +603,7 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
                         for (int i = 0; i < 4; ++i) {
                             const int key = g * 16 + row_key<KIND>(c4 * 2 + (i & 1)) + (i >> 1) * 8;
                             d[i] = __half2half2(blk < nb ? vs[key * nb + blk] : __ushort_as_half(0));
-                            if constexpr (F::VB == 16)
+                            if constexpr (kFewCodes<DP> == 16)
                                 *reinterpret_cast<uint4*>(w[i]) = *reinterpret_cast<const uint4*>(
                                     vt + sl * F::SLAB + key * 128 + ((n8 ^ (key & 7)) << 4));
                             else
@@ -619,7 +623,7 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
                                                         __byte_perm(x[2][e], x[3][e], 0x7632)};
 #pragma unroll
                                 for (int t = 0; t < NT; ++t)
-                                    mma16816<KIND>(o[sl * (F::VB / 2) + q * 2 + e][t], va,
+                                    mma16816<KIND>(o[sl * (kFewCodes<DP> / 2) + q * 2 + e][t], va,
                                                    pb[g][t][0], pb[g][t][1]);
                             }
                         }

@@ -102,25 +102,6 @@ __device__ __forceinline__ uint64_t umma_desc_nmajor(uint32_t saddr, uint32_t sl
            ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
-// Two multiply-adds, two additions in one issue slot (of the softmax warps,
-// that have no other to spare: 3% of a chunk's time against plain ones).
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;"
-        : "=l"(reinterpret_cast<uint64_t&>(d))
-        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)),
-          "l"(reinterpret_cast<uint64_t&>(c)));
-    return d;
-}
-
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 d;
-    asm("add.rn.f32x2 %0, %1, %2;"
-        : "=l"(reinterpret_cast<uint64_t&>(d))
-        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-    return d;
-}
-
 __device__ __forceinline__ void shfl_swap(uint4& keep, uint4& give, int mask, bool upper) {
     // the lane with the bit clear gives `give` and takes the partner's `keep`
     uint32_t* k = reinterpret_cast<uint32_t*>(&keep);

@@ -13,10 +13,11 @@
 // two threads own a Q8_0 block.  A CTA looks up the slots of its up to 32
 // tokens, one lane per token, then all its threads walk the units of those
 // tokens, keys and values in the same iteration so that both loads are in
-// flight.  Measured, 105k tokens x 8 heads x 128: write as Q8_0 139 us (4.75
-// TB/s), read back as bfloat16 125 us (5.3 TB/s); with 16 tokens looked up by
-// two rounds of a warp each, and no row loaded before its slot is known, 150 us
-// and 127 us.
+// flight.  Measured, 105k tokens x 8 heads x 128: write as Q8_0 127 us (5.2
+// TB/s), read back as bfloat16 121 us (5.5 TB/s).  Issue slots are the next
+// bound: with a division per unit, single fp32 operations and conversions of
+// the codes, 138 us and 125 us; with stores that pass the caches, 129 us and
+// 123 us.
 #include <type_traits>
 
 #include "kv.cuh"
@@ -77,11 +78,11 @@ __device__ __forceinline__ uint32_t top_bits(const Vec16<T>& x) {
 }
 
 // One thread's half of a Q8_0 block: codes of its 16 values and the block's
-// scale (the other half sits in the neighbouring lane; both lanes must call).
+// scale (the other half sits in the neighbouring lane; the whole warp must call).
 template <typename T>
-__device__ __forceinline__ __half quantise16(const Vec16<T>& x, Vec16<int8_t>& q, unsigned mask) {
+__device__ __forceinline__ __half quantise16(const Vec16<T>& x, Vec16<int8_t>& q) {
     uint32_t top = top_bits(x);
-    top = max(top, __shfl_xor_sync(mask, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     if (top >= 0x7f800000u) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) q.v[i] = 0;
@@ -90,27 +91,65 @@ __device__ __forceinline__ __half quantise16(const Vec16<T>& x, Vec16<int8_t>& q
     const float want = __half2float(__float2half_ru(__fdiv_rn(__uint_as_float(top), 127.f)));
     const float step = fminf(want, kKvScaleMax);
     const float inv = step > 0.f ? __frcp_rn(step) : 0.f;
-    const float limit = want > kKvScaleMax ? 127.f : INFINITY;   // |x / step| <= 127 otherwise
+    const float2 inv2 = make_float2(inv, inv), minus = make_float2(-step, -step);
+    const float2 whole = make_float2(12582912.f, 12582912.f), none = make_float2(0.f, 0.f);
     uint32_t* out = reinterpret_cast<uint32_t*>(q.v);
+    auto codes = [&](auto clamp) {
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        uint32_t n[4];
+        for (int w = 0; w < 4; ++w) {
+            uint32_t n[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            // x / step: x times the reciprocal, and one step of Newton's
-            // correction, whose remainder the fused multiply-add gives exactly:
-            // off by 2^-46 before its rounding, so ties stay ties
-            const float f = kv_to_f<T>(x.v[4 * w + i]);
-            const float y = f * inv;
-            float c = fmaf(fmaf(-y, step, f), inv, y);
-            if (limit == 127.f) c = fminf(fmaxf(c, -127.f), 127.f);
-            // nearest integer, ties to even: 1.5 * 2^23 leaves no fraction bits
-            n[i] = __float_as_uint(c + 12582912.f);
+            for (int i = 0; i < 4; i += 2) {
+                // x / step: x times the reciprocal, and one step of Newton's
+                // correction, whose remainder the fused multiply-add gives
+                // exactly: off by 2^-46 before its rounding, so ties stay ties
+                const float2 f = make_float2(kv_to_f<T>(x.v[4 * w + i]),
+                                             kv_to_f<T>(x.v[4 * w + i + 1]));
+                const float2 y = fma2(f, inv2, none);
+                float2 c = fma2(fma2(y, minus, f), inv2, y);
+                if constexpr (decltype(clamp)::value) {
+                    c.x = fminf(fmaxf(c.x, -127.f), 127.f);
+                    c.y = fminf(fmaxf(c.y, -127.f), 127.f);
+                }
+                // nearest integer, ties to even: 1.5 * 2^23 leaves no fraction bits
+                c = add2(c, whole);
+                n[i] = __float_as_uint(c.x);
+                n[i + 1] = __float_as_uint(c.y);
+            }
+            out[w] = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040),
+                                 0x5410);
         }
-        out[w] = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
-    }
+    };
+    if (want > kKvScaleMax) codes(std::true_type{});   // |x / step| <= 127 otherwise
+    else codes(std::false_type{});
     return __float2half_rn(step);
 }
+
+// A thread's units of 16 values among a CTA's tokens, kKvThreads apart: token i,
+// head h, values from d on; stepped by carries, without a division.
+struct KvUnit {
+    int i, h, d;           // d in units of 16
+    int di, dh, dd;
+    __device__ __forceinline__ KvUnit(int u, int per_head, int heads) {
+        const int per_token = per_head * heads;
+        auto split = [&](int n, int& a, int& b, int& c) {
+            a = n / per_token;
+            b = (n - a * per_token) / per_head;
+            c = n - a * per_token - b * per_head;
+        };
+        split(u, i, h, d);
+        split(kKvThreads, di, dh, dd);
+    }
+    __device__ __forceinline__ void next(int per_head, int heads) {
+        d += dd;
+        const int up = d >= per_head;
+        d -= up ? per_head : 0;
+        h += dh + up;
+        const int over = h >= heads;
+        h -= over ? heads : 0;
+        i += di + over;
+    }
+};
 
 // Slot (page * heads * page_size + row, in rows of one head; -1: none, -2:
 // behind the last sequence) of the CTA's tokens: the first warp searches the
@@ -148,51 +187,45 @@ __device__ __forceinline__ void cta_slots(const KvBatch& b, const KvCache& c, in
 
 // TI: type of the rows, TC: type of the cache (int8_t: Q8_0).
 template <typename TI, typename TC>
-__global__ void __launch_bounds__(kKvThreads)
+__global__ void __launch_bounds__(kKvThreads, sizeof(TI) == 4 ? 2 : 4)
 k_kv_write(KvBatch b, KvCache c, KvRows in, int tokens, unsigned* status) {
     __shared__ int64_t slots[kKvMaxTokens];
     const int t0 = blockIdx.x * tokens;
     const int n = b.T - t0 < tokens ? b.T - t0 : tokens;
     const int per_head = c.dim >> 4;
-    const int per_token = per_head * c.heads;
+    const int units = n * per_head * c.heads;
     // a unit's rows are loaded while the one before it is stored, the first
     // while the slots are looked up
-    Vec16<TI> x[2];
-    int i = 0, h = 0, d = 0;
-    auto load = [&](int u) {
-        i = u / per_token;
-        const int r = u - i * per_token;
-        h = r / per_head;
-        d = (r - h * per_head) << 4;
-        load16(x[0], static_cast<const TI*>(in.k) + (t0 + i) * in.k_ts + h * in.k_hs + d);
-        load16(x[1], static_cast<const TI*>(in.v) + (t0 + i) * in.v_ts + h * in.v_hs + d);
+    Vec16<TI> x[2] = {};
+    KvUnit at(threadIdx.x, per_head, c.heads);
+    auto load = [&] {
+        const int h = at.h, d = at.d << 4;
+        load16(x[0], static_cast<const TI*>(in.k) + (t0 + at.i) * in.k_ts + h * in.k_hs + d);
+        load16(x[1], static_cast<const TI*>(in.v) + (t0 + at.i) * in.v_ts + h * in.v_hs + d);
     };
-    const int units = n * per_token;
     int u = threadIdx.x;
-    if (u < units) load(u);
+    if (u < units) load();
     cta_slots(b, c, t0, n, slots, status);
     __syncthreads();
-    while (u < units) {
-        const int64_t slot = slots[i];
-        const int64_t row = slot + ((int64_t)h << c.page_shift);
-        const int at = d;
+    for (; (u & ~31) < units; u += kKvThreads) {   // whole warps: two lanes share a block
+        const int64_t slot = u < units ? slots[at.i] : -1;
+        const int64_t row = slot + ((int64_t)at.h << c.page_shift);
+        const int d = at.d << 4;
         const Vec16<TI> y0 = x[0], y1 = x[1];
-        u += kKvThreads;
-        if (u < units) load(u);
-        if (slot < 0) continue;   // both lanes of a block share the token
-        const unsigned mask = __activemask();
+        at.next(per_head, c.heads);
+        if (u + kKvThreads < units) load();
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             const Vec16<TI>& v = w ? y1 : y0;
             Vec16<TC> y;
             if constexpr (sizeof(TC) == 1) {
-                const __half s = quantise16(v, y, mask);
-                if (!(at & 16)) (w ? c.vs : c.ks)[row * (c.dim >> 5) + (at >> 5)] = s;
+                const __half s = quantise16(v, y);
+                if (slot >= 0 && !(d & 16)) (w ? c.vs : c.ks)[row * (c.dim >> 5) + (d >> 5)] = s;
             } else {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) y.v[j] = kv_from_f<TC>(kv_to_f<TI>(v.v[j]));
             }
-            store16(static_cast<TC*>(w ? c.v : c.k) + row * c.dim + at, y);
+            if (slot >= 0) store16(static_cast<TC*>(w ? c.v : c.k) + row * c.dim + d, y);
         }
     }
 }
@@ -207,15 +240,13 @@ k_kv_read(KvBatch b, KvCache c, KvRows out, int tokens, unsigned* status) {
     cta_slots(b, c, t0, n, slots, status);
     __syncthreads();
     const int per_head = c.dim >> 4;
-    const int per_token = per_head * c.heads;
+    const int units = n * per_head * c.heads;
+    KvUnit at(threadIdx.x, per_head, c.heads);
 #pragma unroll 2
-    for (int u = threadIdx.x; u < n * per_token; u += kKvThreads) {
-        const int i = u / per_token;
+    for (int u = threadIdx.x; u < units; u += kKvThreads, at.next(per_head, c.heads)) {
+        const int i = at.i, h = at.h, d = at.d << 4;
         const int64_t slot = slots[i];
         if (slot == -2) continue;   // behind the last sequence: left as it is
-        const int r = u - i * per_token;
-        const int h = r / per_head;
-        const int d = (r - h * per_head) << 4;
         const int64_t row = slot + ((int64_t)h << c.page_shift);
         Vec16<TC> x[2];
         float s[2] = {0.f, 0.f};
@@ -229,15 +260,28 @@ k_kv_read(KvBatch b, KvCache c, KvRows out, int tokens, unsigned* status) {
         }
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-            Vec16<TO> y;
+            Vec16<TO> y{};
+            if (slot >= 0) {
+                if constexpr (sizeof(TC) == 1) {
+                    // a code as fp32: 2^23 + 128 + code by a byte permute, less
+                    // 2^23 + 128 (a conversion runs at a quarter of their rate)
+                    const uint32_t* q = reinterpret_cast<const uint32_t*>(x[w].v);
+                    const float2 off = make_float2(-8388736.f, -8388736.f);
+                    const float2 s2 = make_float2(s[w], s[w]), none = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                float f;
-                if constexpr (sizeof(TC) == 1)
-                    f = s[w] * (float)x[w].v[j];
-                else
-                    f = kv_to_f<TC>(x[w].v[j]);
-                y.v[j] = kv_from_f<TO>(slot >= 0 ? f : 0.f);
+                    for (int j = 0; j < 16; j += 2) {
+                        const uint32_t p = q[j / 4] ^ 0x80808080u;
+                        float2 f;
+                        f.x = __uint_as_float(__byte_perm(p, 0x4b000000u, 0x7440 + j % 4));
+                        f.y = __uint_as_float(__byte_perm(p, 0x4b000000u, 0x7441 + j % 4));
+                        f = fma2(add2(f, off), s2, none);
+                        y.v[j] = kv_from_f<TO>(f.x);
+                        y.v[j + 1] = kv_from_f<TO>(f.y);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) y.v[j] = kv_from_f<TO>(kv_to_f<TC>(x[w].v[j]));
+                }
             }
             TO* p = w ? static_cast<TO*>(out.v) + (t0 + i) * out.v_ts + h * out.v_hs + d
                       : static_cast<TO*>(out.k) + (t0 + i) * out.k_ts + h * out.k_hs + d;
