@@ -136,9 +136,8 @@ __device__ __forceinline__ int row_key(int n) {
 template <int DP, int KIND>
 __device__ __forceinline__ int out_dim(int i, int n, int h) {
     using F = Few<DP, KIND, 1>;
-    if constexpr (F::Q8)
-        constexpr int C = kFewCodes<DP>;
-        return (i / (C / 2)) * (C * 8) + n * C + i % (C / 2) * 2 + h;
+    constexpr int C = kFewCodes<DP>;
+    if constexpr (F::Q8) return (i / (C / 2)) * (C * 8) + n * C + i % (C / 2) * 2 + h;
     return i * 16 + n + 8 * h;
 }
 
