@@ -508,7 +508,7 @@ MOE_B200_API int moe_b200_attend_workspace(const moe_b200_kv_cache* cache,
  * unless that is Q8_0), strides as for moe_b200_kv_write.  lse ([tokens x
  * q_heads] fp32, or NULL) receives the logarithm of the softmax sum.  A row
  * that attends no token gets zeros and -infinity; rows behind the last
- * sequence are left as they are.  Tokens that a row does not attend never
+ * sequence are left as they are.  out may be q itself.  Tokens that a row does not attend never
  * reach its result, whatever they hold.  Scores, softmax and sums are fp32;
  * Q8_0 values enter as scale * code rounded to binary16 (a scale of 512 or
  * more can overflow it; moe_b200_kv_write stores none), probabilities as

@@ -240,12 +240,27 @@ __global__ void __launch_bounds__(256) k_attend_expand(KvBatch b, KvCache c, __h
     }
 }
 
-// How a call runs.  Tiles of 8 rows up to 8 rows per sequence on average, of 16
-// up to 32 (a tile reads the keys again), of 128 or 256 beyond.  Those decode a Q8_0
-// cache's values as often as a sequence has tiles, on warps that the softmax
-// needs (chunks of 2048 rows over 8k keys, 32/8 heads x 128: 444 us, expanded
-// first 260 us); from two tiles on the pages are expanded to binary16 in the
-// workspace, if the table's width bounds that by 1 GB.
+// Rows per sequence and key/value head, on average, up to which attend_few.cu
+// is the faster one.  16 sequences of 8000 tokens, two key/value heads, us:
+//                  rows   16: few, many    32: few, many    64: few, many
+//   16-bit, 64 wide        32, 46           36, 46           46, 46
+//   16-bit, 128            46, 52           60, 52           85, 54
+//   16-bit, 256            79, 71 (8 rows: 72, 71)           192, 77
+//   Q8_0, 128              42, 95           58, 97           91, 97
+//   Q8_0, 256              67, 140          97, 142          161, 145 (48: 128, 142)
+// One sequence, or 64 of 1000 tokens, give the same order or differ by 2 us.
+int few_rows(int dp, bool q8) {
+    if (q8) return dp > 128 ? 48 : 64;
+    return dp > 128 ? 8 : dp > 64 ? 16 : 64;
+}
+
+// How a call runs.  Few rows: tiles of 8 up to 8 rows per sequence, of 16 beyond
+// (a tile reads the keys again; 16 rows x 128 as above: 56 us in tiles of 8, 46
+// in one of 16; 8 rows: 42 and 44).  Many rows: tiles of 128 or 256.  Those
+// decode a Q8_0 cache's values as often as a sequence has tiles, on warps that
+// the softmax needs (chunks of 2048 rows over 8k keys, 32/8 heads x 128: 444 us,
+// expanded first 260 us); from two tiles on the pages are expanded to binary16
+// in the workspace, if the table's width bounds that by 1 GB.
 struct AttendPlan {
     bool many;
     int rows;             // of a tile
@@ -257,7 +272,7 @@ AttendPlan attend_plan(const KvBatch& b, const KvCache& c, int group) {
     const int dp = attend_dim(c.dim);
     const int64_t rows = (int64_t)b.T * group;
     AttendPlan p{};
-    p.many = rows > 32 * (int64_t)b.B;
+    p.many = rows > few_rows(dp, c.type == Q8_0) * (int64_t)b.B;
     p.rows = p.many ? many_rows(dp) : rows > 8 * (int64_t)b.B ? 16 : 8;
     p.base = align_up(AttendWs::bytes(p.many ? sm_count() : attend_few_ctas(), p.rows, dp));
     if (p.many && c.type == Q8_0 && rows > p.rows * (int64_t)b.B && b.max_pages > 0 &&

@@ -770,8 +770,12 @@ cudaError_t launch_few(const AttendArgs& a, void* ws, cudaStream_t s) {
 
 template <int DP, int NT>
 cudaError_t launch_kind(const AttendArgs& a, void* ws, cudaStream_t s) {
-    if (a.c.type == KV_F16) return launch_few<DP, KIND_F16, NT, __half>(a, ws, s);
-    if (a.c.type == KV_BF16) return launch_few<DP, KIND_BF16, NT, __nv_bfloat16>(a, ws, s);
+    // 16 rows of more than 128 values: attend_many.cu, unless Q8_0
+    if constexpr (NT == 1 || DP <= 128) {
+        if (a.c.type == KV_F16) return launch_few<DP, KIND_F16, NT, __half>(a, ws, s);
+        if (a.c.type == KV_BF16) return launch_few<DP, KIND_BF16, NT, __nv_bfloat16>(a, ws, s);
+    }
+    if (a.c.type != Q8_0) return cudaErrorInvalidValue;
     if (a.type == KV_F16) return launch_few<DP, KIND_Q8, NT, __half>(a, ws, s);
     return launch_few<DP, KIND_Q8, NT, __nv_bfloat16>(a, ws, s);
 }

@@ -255,7 +255,8 @@ class PagedKVCache:
         tokens; ``lse`` (fp32 [tokens, q_heads], contiguous) receives the
         logarithm of the softmax sum.  Rows without a token get zeros and
         -inf; rows behind the last sequence are left as they are (``out`` is
-        allocated uninitialised when not given)."""
+        allocated uninitialised when not given).  ``out`` may be ``q``; no
+        gradient is recorded."""
         other = self._elsewhere(stream)
         if other is not None:
             with other:

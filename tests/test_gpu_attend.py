@@ -377,6 +377,44 @@ def test_other_stream(n):
     assert all(torch.equal(o, want) for o in outs)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows", [8, 9, 16, 17, 48, 49, 64, 65])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_numbers_of_rows_between_the_kernels(dim, rows, kind):
+    """Every tile height on both sides of the sizes at which it changes."""
+    new, kv = [rows, rows - 3, rows + 3], [rows + 600, rows - 3, 900]
+    cache, batch, q = build(new, kv, 32, 1, dim, 1, kind, seed=34)
+    lse = torch.empty(q.shape[:2], device=DEV)
+    check(cache, batch, q, cache.attend(batch, q, lse=lse), lse, new, kv, dim ** -0.5)
+
+
+@pytest.mark.parametrize("kind", ["f16", "q8_bf16"])
+@pytest.mark.parametrize("n", [1, 5, 300])
+def test_two_streams_at_once(n, kind):
+    """Calls that run side by side have workspaces of their own."""
+    parts = []
+    for seed in (31, 32):
+        cache, batch, q = build([n, 2], [n + 900 + seed, 40], 16, 2, 128, 8, kind, seed=seed)
+        parts.append((cache, batch, q, cache.attend(batch, q), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(10):
+        for i, (cache, batch, q, _, stream) in enumerate(parts):
+            outs[i].append(cache.attend(batch, q, stream=stream))
+    torch.cuda.synchronize()
+    for i, (_, _, _, want, _) in enumerate(parts):
+        assert all(torch.equal(o, want) for o in outs[i])
+
+
+@pytest.mark.parametrize("kind", ["f16", "q8_bf16"])
+@pytest.mark.parametrize("dim,n", [(64, 1), (128, 4), (128, 700), (256, 300)])
+def test_output_in_place_of_the_queries(dim, n, kind):
+    cache, batch, q = build([n, 1, 3], [n + 1500, 700, 3], 32, 2, dim, 8, kind, seed=33)
+    want = cache.attend(batch, q)
+    got = cache.attend(batch, q, out=q)
+    assert got.data_ptr() == q.data_ptr() and torch.equal(got, want)
+
+
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
 @pytest.mark.parametrize("n", [1, 3, 90])
 def test_infinite_scores(n, kind):
