@@ -461,10 +461,10 @@ typedef struct moe_b200_kv_batch {
 } moe_b200_kv_batch;
 
 /* status (device int32, may be NULL) receives 0 or a sum of these: a page id
- * outside the cache was met, a length reaches past the page table (rows there
- * are neither written nor read; an attention output of that sequence is not
- * valid, other sequences are not affected), a bounded device-side wait gave up
- * (no output is valid). */
+ * outside the cache was met, a length reaches past the page table or, for
+ * attention, past 2^31 - 65536 (rows there are neither written nor read; an
+ * attention output of that sequence is not valid, other sequences are not
+ * affected), a bounded device-side wait gave up (no output is valid). */
 #define MOE_B200_KV_BAD_PAGE 1
 #define MOE_B200_KV_BAD_LENGTH 2
 #define MOE_B200_KV_TIMEOUT 4

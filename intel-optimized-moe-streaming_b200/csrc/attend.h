@@ -116,6 +116,10 @@ __host__ __device__ __forceinline__ void attend_range(int pos, int len, int caus
 
 #ifdef __CUDACC__
 
+// Longest sequence: a key's number, rounded up to the units that a kernel looks
+// ahead to, stays below 2^31.
+constexpr int64_t kAttendKeys = 0x7fff0000;
+
 struct AttendSeq {
     int q0, n;        // first row of the batch, number of rows
     int len, first;   // cached tokens; position of the first row
@@ -131,7 +135,8 @@ __device__ __forceinline__ AttendSeq attend_seq(const AttendArgs& a, int b, unsi
     s.q0 = q0;
     s.n = q1 > q0 ? q1 - q0 : 0;
     s.first = raw - s.n;
-    const int64_t cap = (int64_t)a.b.max_pages << a.c.page_shift;
+    int64_t cap = (int64_t)a.b.max_pages << a.c.page_shift;
+    cap = cap < kAttendKeys ? cap : kAttendKeys;
     s.len = raw;
     if (raw > cap) {
         kv_flag(status, KV_BAD_LENGTH);

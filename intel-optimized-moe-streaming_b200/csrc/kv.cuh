@@ -66,16 +66,6 @@ __device__ __forceinline__ int kv_find_seq(const KvBatch& b, int t) {
     return (__ldg(b.q_start + lo) <= t && t < __ldg(b.q_start + lo + 1)) ? lo : -1;
 }
 
-// Cached length of a sequence, at most what its row of the page table holds.
-__device__ __forceinline__ int kv_length(const KvBatch& b, const KvCache& c, int seq,
-                                         unsigned* status) {
-    const int len = __ldg(b.kv_lens + seq);
-    const int64_t cap = (int64_t)b.max_pages << c.page_shift;
-    if (len <= cap) return len;
-    kv_flag(status, KV_BAD_LENGTH);
-    return (int)cap;
-}
-
 // Page id of a logical page of a sequence, or -1 (and a status bit) when it
 // lies outside the table or the cache.
 __device__ __forceinline__ int kv_page(const KvBatch& b, const KvCache& c, int seq, int page,

@@ -477,3 +477,28 @@ def test_offsets_past_32_bits():
         assert torch.equal(rk, k) and torch.equal(rv, v)
         q = torch.randn(n, 16, dim, device=DEV).half()
         check(cache, batch, q, cache.attend(batch, q), None, [n], [150], dim ** -0.5)
+
+
+def test_the_longest_sequence():
+    """2^31 - 65536 cached tokens, all in one page that the table names eight
+    million times: what attention over that page once gives.  A thread adds up
+    226k probabilities and 113k products in fp32, each off by at most 2^-23 of
+    the sum.  One token more is refused."""
+    cache = PagedKVCache.empty(1, 256, 1, 32, F16, DEV)
+    g = torch.Generator(device=DEV).manual_seed(36)
+    cache.k.copy_(torch.randn(cache.k.shape, generator=g, device=DEV))
+    cache.v.copy_(torch.randn(cache.v.shape, generator=g, device=DEV) + 1)
+    q = torch.randn((1, 1, 32), generator=g, device=DEV).half()
+    table = torch.zeros((1, 1 << 23), dtype=torch.int32, device=DEV)
+    start = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([(1 << 31) - 65536], dtype=torch.int32, device=DEV)
+    status = torch.full((1,), 99, dtype=torch.int32, device=DEV)
+    out = cache.attend(KVBatch(start, lens, table), q, status=status)
+    assert status.item() == 0
+    w = torch.softmax(cache.k[0, 0].double() @ q[0, 0].double() * 32 ** -0.5, 0)
+    want = w @ cache.v[0, 0].double()
+    tol = ((226e3 + 113e3) * 2 ** -23 + 2 * K.HALF[torch.float16]) * want.abs().max()
+    assert (out[0, 0].double() - want).abs().max() <= tol
+    lens += 1
+    cache.attend(KVBatch(start, lens, table), q, status=status)
+    assert status.item() == _lib.KV_BAD_LENGTH
