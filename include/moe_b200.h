@@ -486,7 +486,8 @@ MOE_B200_API int moe_b200_kv_write(const moe_b200_kv_cache* cache, const moe_b20
 /* The mirror of moe_b200_kv_write: the cached values at the batch's rows,
  * rounded to `type`, into k and v.  With q_start the running sum of kv_lens
  * it gathers whole sequences.  Rows at negative positions or in refused
- * pages read as zeros; rows behind the last sequence are left as they are. */
+ * pages read as zeros; rows behind the last sequence are left as they are.  The
+ * rows of k and v must not overlap. */
 MOE_B200_API int moe_b200_kv_read(const moe_b200_kv_cache* cache, const moe_b200_kv_batch* batch,
                                   int32_t type, void* k, int64_t k_token_stride,
                                   int64_t k_head_stride, void* v, int64_t v_token_stride,
@@ -508,14 +509,15 @@ MOE_B200_API int moe_b200_attend_workspace(const moe_b200_kv_cache* cache,
  * unless that is Q8_0), strides as for moe_b200_kv_write.  lse ([tokens x
  * q_heads] fp32, or NULL) receives the logarithm of the softmax sum.  A row
  * that attends no token gets zeros and -infinity; rows behind the last
- * sequence are left as they are.  out may be q itself.  Tokens that a row does not attend never
- * reach its result, whatever they hold.  Scores, softmax and sums are fp32;
- * Q8_0 values enter as scale * code rounded to binary16 (a scale of 512 or
- * more can overflow it; moe_b200_kv_write stores none), probabilities as
- * 16-bit values.  Two kernels, three for many rows per sequence over a Q8_0
- * cache whose expanded pages (4 bytes a value pair for max_pages pages of
- * every sequence, part of the workspace) stay within 1 GB.  Results do not
- * depend on other calls and repeat bit for bit. */
+ * sequence are left as they are.  The rows of out must not overlap; out may be
+ * q itself.  Tokens that a row does not attend never reach its result,
+ * whatever they hold.  Scores, softmax and sums are fp32; Q8_0 values enter as
+ * scale * code rounded to binary16 (a scale of 512 or more can overflow it;
+ * moe_b200_kv_write stores none), probabilities as 16-bit values.  Two
+ * kernels, three for many rows per sequence over a Q8_0 cache whose expanded
+ * pages (4 bytes a value pair for max_pages pages of every sequence, part of
+ * the workspace) stay within 1 GB.  Results do not depend on other calls and
+ * repeat bit for bit. */
 MOE_B200_API int moe_b200_attend(const moe_b200_kv_cache* cache, const moe_b200_kv_batch* batch,
                                  int32_t type, const void* q, int64_t q_token_stride,
                                  int64_t q_head_stride, int32_t q_heads, void* out,

@@ -174,6 +174,9 @@ class PagedKVCache:
         if heads == 1:
             hs = 0
         ptr = t.data_ptr()
+        if output and ((shape[0] > 1 and ts < self.head_dim)
+                       or (heads > 1 and hs < self.head_dim)):
+            raise ValueError(f"{what} must have rows that do not overlap")
         if ds != 1 or (ptr | ts * _BYTES[t.dtype] | hs * _BYTES[t.dtype]) & 15:
             if output:
                 raise ValueError(f"{what} must have contiguous, 16-byte aligned head rows")

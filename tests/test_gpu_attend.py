@@ -502,3 +502,14 @@ def test_the_longest_sequence():
     lens += 1
     cache.attend(KVBatch(start, lens, table), q, status=status)
     assert status.item() == _lib.KV_BAD_LENGTH
+
+
+def test_overlapping_outputs_are_refused():
+    cache, batch, q = build([2], [20], 16, 2, 64, 4, "f16")
+    one = torch.empty(1, 4, 64, device=DEV, dtype=torch.float16)
+    rows = torch.empty(2, 1, 64, device=DEV, dtype=torch.float16)
+    for out in (one.expand(2, 4, 64), rows.expand(2, 4, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            cache.attend(batch, q, out=out)
+        with pytest.raises(ValueError, match="overlap"):
+            cache.read(batch, out=(out[:, :2], torch.empty_like(out[:, :2])))
