@@ -127,6 +127,11 @@ __device__ __forceinline__ void bar_sync() {
     asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory");
 }
 
+template <int N>
+__device__ __forceinline__ void bar_sync(int id) {
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
+}
+
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
                  "r"(valid ? 16 : 0)
@@ -384,6 +389,7 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                 }
                 tmem_wait_st();
             }
+            tc_fence_before();
             bar_sync<2, 256>();
 #pragma unroll
             for (int h = 0; h < F::KPARTS; ++h)
@@ -427,6 +433,7 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
 #pragma unroll
                 for (int c = 0; c < F::OC / 32; ++c) tmem_st32(t_o + c * 32, z);
                 tmem_wait_st();
+                tc_fence_before();   // with one tile, the maximum's barrier follows
             }
 #pragma unroll 1
             for (int j = 0; j < take; ++j, ++it) {
@@ -509,6 +516,16 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                         tmem_st16(t_o + c * 16, o);
                     }
                     tmem_wait_st();
+                    // With one tile the value product of the first 64 keys goes
+                    // to both halves of O and starts when warps 0-3 hand over:
+                    // each of them meets the warp that rescales the other half
+                    // of its rows.  Both come here together: the maximum in use
+                    // and the new one are the same in both.
+                    if constexpr (F::NQ == 1) {
+                        tc_fence_before();
+                        bar_sync<64>(3 + quarter);
+                        tc_fence_after();
+                    }
                 }
                 if (grow) m = top;
                 const float base = m == -INFINITY ? 0.f : m - F::SHIFT;

@@ -1,0 +1,52 @@
+"""Calls of the attention at the edges of what its documentation allows.  The
+allowed errors are those of test_gpu_attend.py."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from flash_moe_b200.formats import Q8_0
+from flash_moe_b200.paged_kv import KVBatch
+from test_gpu_attend import DEV, KINDS, build, check
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("window", [0, 300])
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,heads,q_heads,wide", [(64, 1, 4, False), (128, 2, 8, False),
+                                                    (160, 1, 4, False), (256, 2, 8, False),
+                                                    (256, 1, 4, True)])
+def test_maxima_that_grow_in_every_unit(dim, heads, q_heads, wide, kind, window):
+    """Keys whose scores rise by 12 powers of two from one 128-key unit to the
+    next, so that every unit replaces every row's maximum and rescales its
+    sums; a window adds rows that meet their first key in a later unit.  Every
+    run gives the same bits."""
+    new, kv = [300, 40, 129], [2600, 1500, 129]
+    cache, batch, q = build(new, kv, 32, heads, dim, q_heads, kind, seed=40)
+    if wide:   # a table too wide for expanded pages: codes decoded on their way
+        table = torch.full((3, 70000 // heads), -1, dtype=torch.int32, device=DEV)
+        table[:, :batch.max_pages] = batch.page_table
+        batch = KVBatch(batch.q_start, batch.kv_lens, table)
+    scale = 0.125
+    g = torch.Generator(device=DEV).manual_seed(47)
+    q = (1 + 0.1 * torch.randn(q.shape, generator=g, device=DEV)).to(q.dtype)
+    for b, length in enumerate(kv):
+        pos = torch.arange(length, device=DEV)
+        # q . k * scale * log2(e) = 12 per 128 keys
+        rise = pos * (12 / 128) / (dim * scale * 1.4427)
+        pages, rows = batch.page_table[b].long()[pos // 32], pos % 32
+        noise = 0.05 * torch.randn((length, heads, dim), generator=g, device=DEV)
+        k = rise[:, None, None] + noise
+        if cache.type == Q8_0:
+            blocks = k.unflatten(-1, (-1, 32))
+            step = (blocks.abs().amax(-1) / 120).clamp(min=1e-4).half()
+            cache.k[pages, :, rows] = (blocks / step[..., None]).round().flatten(-2).to(torch.int8)
+            cache.k_scales[pages, :, rows] = step
+        else:
+            cache.k[pages, :, rows] = k.to(cache.k.dtype)
+    lse = torch.empty(q.shape[:2], device=DEV)
+    first = cache.attend(batch, q, scale=scale, window=window, lse=lse)
+    check(cache, batch, q, first, lse, new, kv, scale, window=window)
+    for _ in range(30):
+        assert torch.equal(cache.attend(batch, q, scale=scale, window=window), first)
