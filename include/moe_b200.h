@@ -451,7 +451,8 @@ typedef struct moe_b200_kv_cache {
  * Position p lives in row p % page_size of page
  * page_table[b * table_stride + p / page_size] (max_pages entries a row).
  * Rows at negative positions and rows behind q_start[sequences] belong to no
- * cached token. */
+ * cached token.  With fewer than q_start[sequences] tokens the rows that are
+ * not given are left out and the others stay at their positions. */
 typedef struct moe_b200_kv_batch {
     int32_t sequences, tokens, max_pages, reserved;
     int64_t table_stride;

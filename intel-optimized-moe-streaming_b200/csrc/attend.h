@@ -127,14 +127,15 @@ struct AttendSeq {
 
 __device__ __forceinline__ AttendSeq attend_seq(const AttendArgs& a, int b, unsigned* status) {
     AttendSeq s;
-    int q0 = __ldg(a.b.q_start + b), q1 = __ldg(a.b.q_start + b + 1);
+    int q0 = __ldg(a.b.q_start + b);
+    const int end = __ldg(a.b.q_start + b + 1);   // may lie behind the given rows
     int raw = __ldg(a.b.kv_lens + b);
     raw = raw > 0 ? raw : 0;
     q0 = q0 > 0 ? q0 : 0;
-    q1 = q1 < a.b.T ? q1 : a.b.T;
+    const int q1 = end < a.b.T ? end : a.b.T;
     s.q0 = q0;
     s.n = q1 > q0 ? q1 - q0 : 0;
-    s.first = raw - s.n;
+    s.first = s.n > 0 ? raw - (end - q0) : raw;
     int64_t cap = (int64_t)a.b.max_pages << a.c.page_shift;
     cap = cap < kAttendKeys ? cap : kAttendKeys;
     s.len = raw;

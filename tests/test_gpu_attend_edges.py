@@ -50,3 +50,22 @@ def test_maxima_that_grow_in_every_unit(dim, heads, q_heads, wide, kind, window)
     check(cache, batch, q, first, lse, new, kv, scale, window=window)
     for _ in range(30):
         assert torch.equal(cache.attend(batch, q, scale=scale, window=window), first)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new,kv,given", [([5], [40], 3), ([3, 4], [70, 90], 4),
+                                          ([200], [500], 130), ([40, 300], [60, 900], 170)])
+def test_fewer_rows_than_the_batch(new, kv, given, kind):
+    """Rows that are not given are not computed; the others stay at the
+    positions that the batch gives them."""
+    cache, batch, q = build(new, kv, 16, 2, 128, 8, kind, seed=41)
+    left, part, length = given, [], []
+    for n, k in zip(new, kv):
+        part.append(min(n, left))
+        length.append(k - (n - part[-1]))   # a causal row sees no further
+        left -= part[-1]
+    for window in (0, 50):
+        out = cache.attend(batch, q[:given], window=window)
+        check(cache, batch, q[:given], out, None, part, length, 128 ** -0.5, window=window)
+    out = cache.attend(batch, q[:given], causal=False)
+    check(cache, batch, q[:given], out, None, part, kv, 128 ** -0.5, causal=False)
