@@ -512,7 +512,8 @@ MOE_B200_API int moe_b200_attend_workspace(const moe_b200_kv_cache* cache,
  * that attends no token gets zeros and -infinity; rows behind the last
  * sequence are left as they are.  The rows of out must not overlap; out may be
  * q itself.  Tokens that a row does not attend never reach its result,
- * whatever they hold.  Scores, softmax and sums are fp32; Q8_0 values enter as
+ * whatever they hold, and table entries of pages that lie before every row's
+ * window are not looked at.  Scores, softmax and sums are fp32; Q8_0 values enter as
  * scale * code rounded to binary16 (a scale of 512 or more can overflow it;
  * moe_b200_kv_write stores none), probabilities as 16-bit values.  Two
  * kernels, three for many rows per sequence over a Q8_0 cache whose expanded

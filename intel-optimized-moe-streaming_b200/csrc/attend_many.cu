@@ -846,10 +846,14 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             const int pieces = kManyKeys / piece;
             while (w.open(a)) {
                 const int take = w.take;
-                // lane i: page of the unit's i-th piece
+                const AttendTile tile = attend_tile(a, w.s, w.cur.tile * F::M, F::M);
+                // lane i: page of the unit's i-th piece, if some row attends a
+                // key of it (the table need not name pages that none does)
                 auto page_at = [&](int j) {
                     const int key = (w.u0 + j) * kManyKeys + lane * piece;
-                    if (j >= take || lane >= pieces || key >= w.s.len) return -1;
+                    if (j >= take || lane >= pieces || key >= w.s.len || key >= tile.t_hi ||
+                        key + piece <= tile.t_lo)
+                        return -1;
                     return kv_page(a.b, a.c, w.cur.seq, key >> a.c.page_shift, a.status);
                 };
                 auto fill = [&](int n, const CUtensorMap* map, int page_id, int key0, int keys,
@@ -903,9 +907,12 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
             // page ids of a unit's pieces, one per lane; one unit's (with two
             // stages per unit two units') are kept
             const int piece_shift = a.c.page_shift < 7 ? a.c.page_shift : 7;
+            const AttendTile tile = attend_tile(a, w.s, w.cur.tile * F::M, F::M);
             auto page_ids = [&](int j) {
                 const int key = (w.u0 + j) * kManyKeys + (lane << piece_shift);
-                if (j >= take || lane >= (kManyKeys >> piece_shift) || key >= w.s.len) return -1;
+                if (j >= take || lane >= (kManyKeys >> piece_shift) || key >= w.s.len ||
+                    key >= tile.t_hi || key + (1 << piece_shift) <= tile.t_lo)
+                    return -1;
                 return kv_page(a.b, a.c, w.cur.seq, key >> a.c.page_shift, a.status);
             };
             int ids[F::KPARTS];

@@ -69,3 +69,20 @@ def test_fewer_rows_than_the_batch(new, kv, given, kind):
         check(cache, batch, q[:given], out, None, part, length, 128 ** -0.5, window=window)
     out = cache.attend(batch, q[:given], causal=False)
     check(cache, batch, q[:given], out, None, part, kv, 128 ** -0.5, causal=False)
+
+
+@pytest.mark.parametrize("kind", ["f16", "q8_bf16"])
+@pytest.mark.parametrize("dim,new", [(64, 1), (128, 5), (128, 60), (128, 200),
+                                     (256, 1), (256, 20), (256, 200)])
+def test_pages_behind_the_window(dim, new, kind):
+    """Table entries of pages that lie before every row's window may name no
+    page."""
+    kv, window = [new + 300, new + 411], 100
+    cache, batch, q = build([new, new], kv, 16, 2, dim, 8, kind, seed=42)
+    status = torch.full((1,), 99, dtype=torch.int32, device=DEV)
+    want = cache.attend(batch, q, window=window)
+    for b, length in enumerate(kv):
+        batch.page_table[b, :(length - new - window + 1) // 16] = -1
+    out = cache.attend(batch, q, window=window, status=status)
+    assert status.item() == 0
+    assert torch.equal(out, want)
