@@ -333,9 +333,10 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
             if (r < rows)
                 attend_range(s.first + a.by_group.div(cur.tile * M + r), s.len, a.causal, a.window,
                              lo[i], hi[i]);
-            mul[i] = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);   // 0: equal weights
+            float f = 1.f;
             if constexpr (CONVERT)
-                mul[i] /= __shfl_sync(0xffffffffu, factor[i / 2], (c4 * 2 + (i & 1)) * 4);
+                f = __shfl_sync(0xffffffffu, factor[i / 2], (c4 * 2 + (i & 1)) * 4);
+            mul[i] = score_factor(a.scale, f);
         }
         float o[F::TILES][NT][4];
 #pragma unroll

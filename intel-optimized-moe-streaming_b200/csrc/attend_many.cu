@@ -443,8 +443,9 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                 await(&bars->s_full[buf], ph);
                 tc_fence_after();
                 if (j == 0) {
-                    mul = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);   // 0: equal weights
-                    if constexpr (QueryRows<DP, KIND, TQ>::CONVERT) mul /= fac[trow];
+                    float f = 1.f;
+                    if constexpr (QueryRows<DP, KIND, TQ>::CONVERT) f = fac[trow];
+                    mul = score_factor(a.scale, f);
                 }
                 const int key0 = (u0 + j) * kManyKeys;
                 const bool whole = key0 >= tile.all_lo && key0 + kManyKeys <= tile.all_hi;

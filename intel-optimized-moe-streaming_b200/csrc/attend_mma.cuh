@@ -75,6 +75,13 @@ __device__ __forceinline__ float row_factor(float top) {
     return e > 1 && e < 254 ? __uint_as_float((254u - e) << 23) : 1.f;
 }
 
+// What takes a score to units of log 2, for a query row held times `factor`.
+// Not zero, or keys that a row does not attend (-infinity) would become NaN: at
+// 1e-37 all scores are equal, as with 0.  Not infinite: scores of zero stay zero.
+__device__ __forceinline__ float score_factor(float scale, float factor) {
+    return fminf(fmaxf(fabsf(scale) / factor * kLog2e, 1e-37f), 3.402823466e38f);
+}
+
 // 32 lanes x 32 consecutive 32-bit columns of tensor memory.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* v) {
     asm volatile(

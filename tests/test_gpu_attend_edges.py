@@ -7,7 +7,7 @@ import torch
 
 from flash_moe_b200.formats import Q8_0
 from flash_moe_b200.paged_kv import KVBatch
-from test_gpu_attend import DEV, KINDS, build, check
+from test_gpu_attend import CASES, DEV, KINDS, build, check
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +86,16 @@ def test_pages_behind_the_window(dim, new, kind):
     out = cache.attend(batch, q, window=window, status=status)
     assert status.item() == 0
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("scale,size", [(0.0, 1e-9), (1e-38, 1e-20), (3e38, 0.0), (-3e38, 0.0)])
+@pytest.mark.parametrize("name", ["drafts", "chunk", "chunk_256"])
+def test_vanishing_scores(name, scale, size, kind):
+    """Scores of zero, or so small that they do not matter: the mean of the
+    attended values, whatever the scale and the size of the queries."""
+    new, kv, page, heads, dim, q_heads = CASES[name]
+    cache, batch, q = build(new, kv, page, heads, dim, q_heads, kind, seed=43)
+    q = (q.float().clamp(-3, 3) * size).to(q.dtype)
+    out = cache.attend(batch, q, scale=scale)
+    check(cache, batch, q, out, None, new, kv, 0.0)
