@@ -69,10 +69,12 @@ __device__ __forceinline__ bool odd16x8(const uint4& v) {   // in eight values
 
 // Power of two that takes a row maximum of magnitude `top` to [1, 2) (1 for
 // zero, subnormal, infinite and NaN rows): a bfloat16 row times it is exact
-// in binary16 but for values 2^-14 times smaller than the maximum.
+// in binary16 but for values 2^-14 times smaller than the maximum.  Rows from
+// 2^113 on are taken to [2^15, 2^16), below binary16's largest value, so that
+// the factor is a normal number and scale / factor finite up to scales of 2^15.
 __device__ __forceinline__ float row_factor(float top) {
     const uint32_t e = __float_as_uint(top) >> 23;
-    return e > 1 && e < 254 ? __uint_as_float((254u - e) << 23) : 1.f;
+    return e > 1 && e < 255 ? __uint_as_float(((e < 240 ? 254u : 269u) - e) << 23) : 1.f;
 }
 
 // What takes a score to units of log 2, for a query row held times `factor`.

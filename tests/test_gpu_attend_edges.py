@@ -99,3 +99,16 @@ def test_vanishing_scores(name, scale, size, kind):
     q = (q.float().clamp(-3, 3) * size).to(q.dtype)
     out = cache.attend(batch, q, scale=scale)
     check(cache, batch, q, out, None, new, kv, 0.0)
+
+
+@pytest.mark.parametrize("top", [2.0 ** 112, 2.0 ** 113, 2.0 ** 126, 2.0 ** 127])
+@pytest.mark.parametrize("name", ["drafts", "chunk", "chunk_256"])
+def test_large_queries_over_codes(name, top):
+    """bf16 queries up to the largest finite ones over a Q8_0 cache."""
+    new, kv, page, heads, dim, q_heads = CASES[name]
+    cache, batch, q = build(new, kv, page, heads, dim, q_heads, "q8_bf16", seed=44)
+    cache.k_scales.fill_(2.0 ** -20)
+    q = (q.float().clamp(-1.9, 1.9) * top).bfloat16()
+    scale = 2.0 ** 10 / top
+    out = cache.attend(batch, q, scale=scale)
+    check(cache, batch, q, out, None, new, kv, scale)
