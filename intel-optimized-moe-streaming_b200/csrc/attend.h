@@ -193,7 +193,8 @@ struct AttendScratch {
     AttendCursor found;
 };
 
-// Finds the stretch of CTA `cta` of `ctas`, none shorter than LEAST.  A tile is
+// Finds the stretch of CTA `cta` of `ctas`; a short line is cut into no more
+// than length / LEAST stretches, rounded up.  A tile is
 // COST + units long (COST: what starting and ending it takes, in units; a cut
 // inside that part gives the whole tile to the later CTA), once per key/value
 // head.  A lane sums
@@ -302,11 +303,13 @@ __device__ AttendCursor attend_place(const AttendArgs& a, AttendScratch& scratch
                     if (lane >= o) upto += up;
                 }
                 if (skip >= upto - n && skip < upto) {
-                    const int at = (int)(skip - (upto - n)), size = hi - lo + COST;
+                    // all heads' units of a long tile may pass 2^31
+                    const int64_t at = skip - (upto - n);
+                    const int size = hi - lo + COST;
                     scratch.found.seq = b;
                     scratch.found.tile = t0 + lane;
-                    scratch.found.kvh = at / size;
-                    scratch.found.unit = at % size;
+                    scratch.found.kvh = (int)(at / size);
+                    scratch.found.unit = (int)(at % size);
                     scratch.found.left = end - start;
                 }
                 const int64_t all = __shfl_sync(0xffffffffu, upto, 31);

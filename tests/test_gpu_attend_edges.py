@@ -112,3 +112,18 @@ def test_large_queries_over_codes(name, top):
     scale = 2.0 ** 10 / top
     out = cache.attend(batch, q, scale=scale)
     check(cache, batch, q, out, None, new, kv, scale)
+
+
+def test_the_longest_sequence_with_many_heads():
+    """The units of all heads of one tile pass 2^31.  The long sequence's table
+    names its last page only, so that the rest is passed over quickly; that
+    page is all that its rows get, and the next sequence is as ever."""
+    heads, dim, length = 272, 32, (1 << 31) - 65536
+    cache, small, q = build([1, 1], [256, 77], 256, heads, dim, heads, "f16", seed=48)
+    table = torch.full((2, 1 << 23), -1, dtype=torch.int32, device=DEV)
+    table[0, length // 256 - 1] = small.page_table[0, 0]
+    table[1, 0] = small.page_table[1, 0]
+    lens = torch.tensor([length, 77], dtype=torch.int32, device=DEV)
+    lse = torch.empty(q.shape[:2], device=DEV)
+    out = cache.attend(KVBatch(small.q_start, lens, table), q, lse=lse)
+    check(cache, small, q, out, lse, [1, 1], [256, 77], dim ** -0.5)
