@@ -79,6 +79,21 @@ def _raw_stream(index: int) -> int:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 
 
+def _overlap(n: int, ns: int, m: int, ms: int, length: int) -> bool:
+    """Whether two of the n x m rows of ``length`` values at i ns + j ms share
+    a value."""
+    if n <= 1 or m <= 1:
+        return (n > 1 and ns < length) or (m > 1 and ms < length)
+    if ns < length or ms < length:
+        return True
+    if ns >= (m - 1) * ms + length or ms >= (n - 1) * ns + length:
+        return False
+    # neither axis lies within a step of the other: rows j apart meet rows i or
+    # i + 1 apart
+    return any((i < n and r < length) or (i + 1 < n and ns - r < length)
+               for i, r in (divmod(j * ms, ns) for j in range(1, m)))
+
+
 class PagedKVCache:
     """Keys and values [num_pages, kv_heads, page_size, head_dim]: fp16, bf16,
     or int8 codes with binary16 scales [..., head_dim / 32] (Q8_0 arithmetic:
@@ -174,8 +189,7 @@ class PagedKVCache:
         if heads == 1:
             hs = 0
         ptr = t.data_ptr()
-        if output and ((shape[0] > 1 and ts < self.head_dim)
-                       or (heads > 1 and hs < self.head_dim)):
+        if output and _overlap(shape[0], ts, heads, hs, self.head_dim):
             raise ValueError(f"{what} must have rows that do not overlap")
         if ds != 1 or (ptr | ts * _BYTES[t.dtype] | hs * _BYTES[t.dtype]) & 15:
             if output:
