@@ -288,6 +288,7 @@ class PagedKVCache:
             raise ValueError("q and the batch must be on the cache's device")
         if window < 0 or (window and not causal):
             raise ValueError("window must be positive, and needs causal")
+        window = min(window, 0x7fffffff)   # wider than any sequence: no limit
         tokens = shape[0]
         if out is None:
             out = q.new_empty(shape)

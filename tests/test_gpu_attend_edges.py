@@ -127,3 +127,10 @@ def test_the_longest_sequence_with_many_heads():
     lse = torch.empty(q.shape[:2], device=DEV)
     out = cache.attend(KVBatch(small.q_start, lens, table), q, lse=lse)
     check(cache, small, q, out, lse, [1, 1], [256, 77], dim ** -0.5)
+
+
+@pytest.mark.parametrize("kind", ["f16", "q8_f16"])
+@pytest.mark.parametrize("window", [1 << 31, 1 << 32, (1 << 32) + 5])
+def test_windows_wider_than_any_sequence(window, kind):
+    cache, batch, q = build([3, 100], [40, 300], 16, 2, 64, 4, kind, seed=45)
+    assert torch.equal(cache.attend(batch, q, window=window), cache.attend(batch, q))
