@@ -515,7 +515,9 @@ MOE_B200_API int moe_b200_attend_workspace(const moe_b200_kv_cache* cache,
  * whatever they hold, and table entries of pages that lie before every row's
  * window are not looked at.  Scores, softmax and sums are fp32; Q8_0 values enter as
  * scale * code rounded to binary16 (a scale of 512 or more can overflow it;
- * moe_b200_kv_write stores none), probabilities as 16-bit values.  Two
+ * moe_b200_kv_write stores none), probabilities as 16-bit values.  Scores
+ * (scale * q . k) of more than 4e7 in magnitude lie 4 and more apart in fp32:
+ * a row that has one may get NaN.  Two
  * kernels, three for many rows per sequence over a Q8_0 cache whose expanded
  * pages (4 bytes a value pair for max_pages pages of every sequence, part of
  * the workspace) stay within 1 GB.  Results do not depend on other calls and

@@ -72,7 +72,9 @@ struct Few {
     static constexpr int TILES = DP / 16;                      // output tiles of 16 dimensions
     static constexpr bool QSM = NT * DP > 256;                 // queries in shared memory
     // binary16 probabilities are taken 2^15 times as large (the largest is
-    // 2^15, below 65504), so that those down to 2^-29 keep all their bits
+    // 2^15, below 65504), so that those down to 2^-29 keep all their bits.  The
+    // maximum and what is taken off the scores are rounded up, so that this holds
+    // for large scores too, whose neighbours in fp32 lie far apart (at 2^25, 4).
     static constexpr float SHIFT = KIND == KIND_BF16 ? 0.f : 15.f;
     static constexpr int PD = DP < 128 ? DP : 128;             // columns joined per pass
     static constexpr int o_scale = kFewWarps * NS * TILEB;
@@ -345,7 +347,7 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[i][t][e] = 0.f;
-        float m[R], l[R];
+        float m[R], l[R];   // the maximum less SHIFT; the sum, which belongs to it
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             m[i] = -INFINITY;
@@ -448,9 +450,9 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                const float mn = fmaxf(m[i], top * mul[i]);
-                base[i] = mn == -INFINITY ? 0.f : mn - F::SHIFT;
-                keep[i] = ex2(m[i] - (mn == -INFINITY ? 0.f : mn));
+                const float mn = fmaxf(m[i], __fadd_ru(__fmul_ru(top, mul[i]), -F::SHIFT));
+                base[i] = mn == -INFINITY ? 0.f : mn;
+                keep[i] = ex2(m[i] - base[i]);
                 grew = grew || mn > m[i];
                 m[i] = mn;
             }
@@ -641,7 +643,6 @@ k_attend_few(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ C
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 4);
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 8);
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 16);
-            m[i] -= F::SHIFT;   // l and o belong to this exponent
             if (n8 == 0) {
                 sm_m[warp * 16 + i / 2 * 8 + c4 * 2 + (i & 1)] = m[i];
                 sm_l[warp * 16 + i / 2 * 8 + c4 * 2 + (i & 1)] = l[i];

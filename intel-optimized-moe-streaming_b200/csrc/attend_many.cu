@@ -61,7 +61,9 @@ struct Many {
     static constexpr int NST = DP == 64 ? 8 : 5;
     static constexpr int OC = NQ == 2 ? DP : DP / 2;     // output columns of a thread
     static constexpr int THREADS = Q8 ? 512 : 384;
-    // binary16 probabilities: 2^7 of the maximum in use, at most 2^15
+    // binary16 probabilities: 2^7 of the maximum in use, at most 2^15.  The
+    // maximum and what is taken off the scores are rounded up, so that this holds
+    // for large scores too, whose neighbours in fp32 lie far apart (at 2^25, 4).
     static constexpr float SHIFT = KIND == KIND_BF16 ? 0.f : 7.f;
     static constexpr int o_stage = QB;
     static constexpr int o_bar = QB + NST * STAGEB;
@@ -424,7 +426,8 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                 warp_lo = max(warp_lo, __shfl_xor_sync(0xffffffffu, warp_lo, o));
                 warp_hi = min(warp_hi, __shfl_xor_sync(0xffffffffu, warp_hi, o));
             }
-            float m = -INFINITY, l = 0.f;
+            float m = -INFINITY, l = 0.f;   // what is taken off the scores (the
+                                            // maximum in use less SHIFT); their sum
             float mul = 0.f;
             {   // O starts from zeros
                 uint32_t z[32];
@@ -494,14 +497,15 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                 }
                 highest(va);
                 highest(vb);
-                float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * mul;
+                float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
+                top = __fadd_ru(__fmul_ru(top, mul), -F::SHIFT);
                 if constexpr (F::NQ == 1) {
                     float* xm = xmax + (it & 1) * 256;
                     xm[wg * 128 + row] = top;
                     bar_sync<1, 256>();
                     top = fmaxf(top, xm[(wg ^ 1) * 128 + row]);
                 }
-                const bool grow = top > m + kManyGrow || (m == -INFINITY && top > m);
+                const bool grow = top > __fadd_rd(m, kManyGrow) || (m == -INFINITY && top > m);
                 if (__any_sync(0xffffffffu, grow && j > 0)) {
                     const float f = grow ? ex2(m - top) : 1.f;
                     l *= f;
@@ -529,7 +533,7 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                     }
                 }
                 if (grow) m = top;
-                const float base = m == -INFINITY ? 0.f : m - F::SHIFT;
+                const float base = m == -INFINITY ? 0.f : m;
                 const float2 scale2 = make_float2(mul, mul), base2 = make_float2(-base, -base);
                 float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
                 // 32 scores to probabilities, in 16 columns at `at`
@@ -614,7 +618,6 @@ k_attend_many(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ 
                     rec.head = ends ? 2 : 1;
                 }
             }
-            m -= F::SHIFT;
             const bool valid = trow < rows;
             const bool none = lo >= hi;
             const float inv = none ? 0.f : 1.f / l;

@@ -5,6 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from kv_cases import gather
 from flash_moe_b200.formats import Q8_0
 from flash_moe_b200.paged_kv import KVBatch
 from test_gpu_attend import CASES, DEV, KINDS, build, check
@@ -134,3 +135,76 @@ def test_the_longest_sequence_with_many_heads():
 def test_windows_wider_than_any_sequence(window, kind):
     cache, batch, q = build([3, 100], [40, 300], 16, 2, 64, 4, kind, seed=45)
     assert torch.equal(cache.attend(batch, q, window=window), cache.attend(batch, q))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size", [1e3, 1e6, 1e9])
+@pytest.mark.parametrize("name", ["decode", "decode_256", "drafts", "chunk", "chunk_256"])
+def test_large_scores(name, size, kind):
+    """One key's score stands out by so much that it takes all the weight, at
+    sizes where neighbouring fp32 numbers are far apart."""
+    new, kv, page, heads, dim, q_heads = CASES[name]
+    cache, batch, q = build(new, kv, page, heads, dim, q_heads, kind, seed=46)
+    q = torch.ones_like(q)
+    target = cache.k if cache.k_scales is None else cache.k_scales
+    target.abs_()
+    if cache.type == Q8_0:
+        cache.k.fill_(100)
+    out = cache.attend(batch, q, scale=size)
+    assert out.isfinite().all()
+    lo = 0
+    for b, (n, length) in enumerate(zip(new, kv)):
+        k = gather(cache.k, cache.k_scales, batch.page_table[b], length, page)
+        v = gather(cache.v, cache.v_scales, batch.page_table[b], length, page)
+        s = k.sum(-1)                       # [length, heads]
+        for i in range(n):
+            hi = length - n + i + 1
+            if hi < 2:
+                continue
+            top = s[:hi].topk(2, dim=0)
+            # sums of dim terms in fp32, and the rounding of score and maximum
+            sure = (top.values[0] - top.values[1]) * size > 40 + (dim + 4) * 2.0 ** -22 * top.values[0] * size
+            want = v[top.indices[0], torch.arange(heads, device=DEV)]
+            got = out[lo + i].view(heads, -1, dim).double()
+            err = (got - want[:, None]).abs().amax(-1).amax(-1)
+            assert (err[sure] <= 2.0 ** -7 * want.abs().amax(-1)[sure]).all(), (b, i)
+        lo += n
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("largest", [1e5, 1e7, 4e7])
+@pytest.mark.parametrize("name", ["decode", "decode_256", "drafts", "chunk", "chunk_256"])
+def test_large_scores(name, largest, kind):
+    """Scores up to the largest documented ones: a key whose score stands out
+    takes all the weight, and every row stays finite."""
+    new, kv, page, heads, dim, q_heads = CASES[name]
+    cache, batch, q = build(new, kv, page, heads, dim, q_heads, kind, seed=46)
+    q = torch.ones_like(q)
+    target = cache.k if cache.k_scales is None else cache.k_scales
+    target.abs_()
+    if cache.type == Q8_0:
+        cache.k.fill_(100)
+    kv_rows = [[gather(c, s, batch.page_table[b], n, page) for c, s in
+                ((cache.k, cache.k_scales), (cache.v, cache.v_scales))] for b, n in enumerate(kv)]
+    scale = largest / max(k.sum(-1).max().item() for k, _ in kv_rows)
+    for sign in (1, -1):
+        out = cache.attend(batch, q, scale=sign * scale)
+        assert out.isfinite().all()
+        at = torch.arange(heads, device=DEV)
+        lo = 0
+        for b, (n, length) in enumerate(zip(new, kv)):
+            k, v = kv_rows[b]
+            s = k.sum(-1) * sign * scale                 # [length, heads]
+            for i in range(n):
+                hi = length - n + i + 1
+                if hi < 2:
+                    continue
+                top = s[:hi].topk(2, dim=0)
+                # sums of dim fp32 terms, two roundings to the maximum's magnitude
+                slack = (dim + 4) * 2.0 ** -22 * s[:hi].abs().amax(0)
+                sure = top.values[0] - top.values[1] > 40 + slack
+                want = v[top.indices[0], at]
+                err = (out[lo + i].view(heads, -1, dim).double() - want[:, None]).abs()
+                tol = 2.0 ** -7 * want.abs().amax(-1)
+                assert (err.amax(-1).amax(-1)[sure] <= tol[sure]).all(), (b, i)
+            lo += n
