@@ -301,7 +301,7 @@ template <bool WRITE, typename A, typename B>
 cudaError_t launch_rows(const KvBatch& b, const KvCache& c, const KvRows& r, unsigned* status,
                         cudaStream_t s) {
     const int n = tokens_per_cta(b.T);
-    const int grid = (b.T + n - 1) / n;
+    const int grid = (b.T - 1) / n + 1;   // up to 2^31 - 1 rows
     if constexpr (WRITE)
         k_kv_write<A, B><<<grid, kKvThreads, 0, s>>>(b, c, r, n, status);
     else
