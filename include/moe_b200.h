@@ -507,20 +507,20 @@ MOE_B200_API int moe_b200_attend_workspace(const moe_b200_kv_cache* cache,
  * kv_heads): all of them (causal 0), or those up to the row's own position
  * (causal 1) and, when window > 0, only the last `window` of these.  q and
  * out [tokens][q_heads][head_dim] of `type` F16 or BF16 (the cache's own type
- * unless that is Q8_0), strides as for moe_b200_kv_write.  lse ([tokens x
- * q_heads] fp32, or NULL) receives the logarithm of the softmax sum.  A row
- * that attends no token gets zeros and -infinity; rows behind the last
- * sequence are left as they are.  The rows of out must not overlap; out may be
- * q itself.  Tokens that a row does not attend never reach its result,
- * whatever they hold, and table entries of pages that lie before every row's
- * window are not looked at.  Scores, softmax and sums are fp32; Q8_0 values enter as
- * scale * code rounded to binary16 (a scale of 512 or more can overflow it;
- * moe_b200_kv_write stores none), probabilities as 16-bit values.  Scores
- * (scale * q . k) of more than 4e7 in magnitude lie 4 and more apart in fp32:
- * a row that has one may get NaN.  Two
- * kernels, three for many rows per sequence over a Q8_0 cache whose expanded
- * pages (4 bytes a value pair for max_pages pages of every sequence, part of
- * the workspace) stay within 1 GB.  Results do not depend on other calls and
+ * unless that is Q8_0), tokens * q_heads up to 2^31 - 256, strides as for
+ * moe_b200_kv_write.  lse ([tokens x q_heads] fp32, or NULL) receives the
+ * logarithm of the softmax sum.  A row that attends no token gets zeros and
+ * -infinity; rows behind the last sequence are left as they are.  The rows of
+ * out must not overlap; out may be q itself.  Tokens that a row does not attend
+ * never reach its result, whatever they hold, and table entries of pages that
+ * lie before every row's window are not looked at.  Scores, softmax and sums
+ * are fp32; Q8_0 values enter as scale * code rounded to binary16 (a scale of
+ * 512 or more can overflow it; moe_b200_kv_write stores none), probabilities as
+ * 16-bit values.  Scores (scale * q . k) of more than 4e7 in magnitude lie 4
+ * and more apart in fp32: a row that has one may get NaN.  Two kernels, three
+ * for many rows per sequence over a Q8_0 cache whose expanded pages (4 bytes a
+ * value pair for max_pages pages of every sequence, part of the workspace) stay
+ * within 1 GB.  Results do not depend on other calls and
  * repeat bit for bit. */
 MOE_B200_API int moe_b200_attend(const moe_b200_kv_cache* cache, const moe_b200_kv_batch* batch,
                                  int32_t type, const void* q, int64_t q_token_stride,

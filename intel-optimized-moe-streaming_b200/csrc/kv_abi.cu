@@ -140,7 +140,8 @@ int moe_b200_attend(const moe_b200_kv_cache* cache, const moe_b200_kv_batch* bat
         if (q_heads < 1 || q_heads > 65536 || q_heads % a.c.heads) return ST_ARG;
         if ((causal != 0 && causal != 1) || window < 0 || (window > 0 && !causal)) return ST_ARG;
         if (!(scale >= -3.402823466e38f && scale <= 3.402823466e38f)) return ST_ARG;
-        if ((int64_t)a.b.T * q_heads > 0x7fffffffll) return ST_ARG;
+        // a head group's rows are counted up to whole tiles of 256 in 32 bits
+        if ((int64_t)a.b.T * q_heads > 0x7fffff00ll) return ST_ARG;
         if (a.b.T > 0 && (!q || !out || !workspace)) return ST_ARG;
         if (!rows_aligned(q, q_token_stride, q_head_stride, 2) ||
             !rows_aligned(out, out_token_stride, out_head_stride, 2) || ((uintptr_t)lse & 3u) ||
