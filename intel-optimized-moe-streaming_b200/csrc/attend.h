@@ -7,9 +7,17 @@
 // and each CTA takes an equal stretch of it, so a CTA holds at most one tile
 // that began in an earlier CTA (its head) and one that ends in a later CTA
 // (its tail); such pieces leave their unnormalised sums in the workspace and
-// k_attend_join adds them up in CTA order.  The cut balances batches of any
-// mixture of lengths, costs at most two partial tiles per CTA, and needs no
-// length on the host.
+// k_attend_join adds them up in CTA order.  The cut balances units whatever the
+// lengths, costs at most two partial tiles per CTA, and needs no length on the
+// host.  (It does not choose the kernel: that is one for the call, attend.cu.)
+//
+// Held in 16 bits, because the matrix instructions take no wider operands of
+// these types: the probabilities (the softmax sum adds them unrounded; a second
+// operand for what is cut off would double the value products), Q8_0 values
+// (scale * code) and bfloat16 queries over them.  Error of the outputs against 64
+// bits, in units of what rounding the output alone gives: 1.1 to 1.4; Q8_0 into
+// binary16, where the rounded keys weigh most, 1.5 to 2.5.  Everything else is
+// fp32.
 #pragma once
 
 #include "kv.cuh"

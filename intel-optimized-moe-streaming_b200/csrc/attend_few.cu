@@ -26,10 +26,10 @@
 // as 16 consecutive bytes and no transposing load is needed.
 // Measured: 64 contexts of 3.5k tokens, 32/8 heads x 128, bf16: 151 us, 6.03
 // TB/s (HBM); 33 x 5 drafted rows over 5 to 3000 tokens, 16/8 x 64, binary16:
-// 32 us, 3.39 TB/s; 24 contexts of 18k tokens, 16/2 heads x 256, Q8_0: 111 us,
-// 4.28 TB/s (some 1400 instructions a warp and 32 keys, most of them decoding,
-// at two warps a scheduler); one context of 1000 tokens: 14 us (the start of
-// two kernels, 16 pieces a head).
+// 32 us, 3.35 TB/s; 24 contexts of 18k tokens, 16/2 heads x 256, Q8_0: 109 us,
+// 4.36 TB/s (some 1400 instructions a warp and 32 keys, most of them decoding;
+// issue slots 45% used: two warps a scheduler wait on their own chains); one
+// context of 1000 tokens: 14 us (the start of two kernels, 16 pieces a head).
 #include "attend_mma.cuh"
 #include "launch.h"
 
